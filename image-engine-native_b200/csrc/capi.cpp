@@ -13,6 +13,7 @@
 #include "realesrgan.h"
 #include "birefnet.h"
 #include "lama.h"
+#include "ops.h"
 #include "scunet.h"
 
 using namespace iec;
@@ -159,6 +160,13 @@ struct BatchPipe {
 };
 
 }  // namespace iec
+
+struct iec_ops {
+  static constexpr uint32_t TAG = 0x4f505338;  // "OPS8"
+  uint32_t tag = TAG;
+  std::unique_ptr<Device> device;
+  ~iec_ops() { tag = 0; }
+};
 
 struct iec_scunet {
   static constexpr uint32_t TAG = 0x53434e54;  // "SCNT"
@@ -689,6 +697,243 @@ iec_status iec_birefnet_run_batch(iec_birefnet* model, const uint8_t* images, si
 }
 
 namespace {
+bool valid_ops(const iec_ops* h) { return h && h->tag == iec_ops::TAG && h->device; }
+
+void need_ops(const iec_ops* h) {
+  need(h, "ops");
+  if (!valid_ops(h)) throw Error(ERR_INPUT, "ops is not a handle of the operators");
+}
+}  // namespace
+
+iec_status iec_ops_open(const iec_options* options, iec_ops** out) {
+  return guard([&] {
+    need(out, "out");
+    *out = nullptr;
+    auto h = std::make_unique<iec_ops>();
+    h->device = std::make_unique<Device>(to_options(options));
+    *out = h.release();
+  });
+}
+
+void iec_ops_free(iec_ops* ops) {
+  if (valid_ops(ops)) delete ops;
+}
+
+const char* iec_ops_device_name(const iec_ops* ops) { return valid_ops(ops) ? ops->device->name().c_str() : ""; }
+
+namespace {
+
+cudaStream_t ops_stream(Device& d, void* stream) { return stream ? static_cast<cudaStream_t>(stream) : d.stream(); }
+
+void check_dtype(int dtype) {
+  if (dtype < IEC_F16 || dtype > IEC_F32) throw Error(ERR_INPUT, "unknown value type " + std::to_string(dtype));
+}
+
+void check_act(int act) {
+  if (act < IEC_ACT_NONE || act > IEC_ACT_SILU) throw Error(ERR_INPUT, "unknown activation " + std::to_string(act));
+}
+
+// `p` is not null and a multiple of `bytes`.
+void need_aligned(const void* p, size_t bytes, const char* what) {
+  need(p, what);
+  if (reinterpret_cast<uintptr_t>(p) % bytes)
+    throw Error(ERR_INPUT, std::string(what) + " is not aligned to " + std::to_string(bytes) + " bytes");
+}
+
+// `v` rows (or columns): at most `most`.
+void check_count(size_t v, size_t most, const char* what) {
+  if (v > most) throw Error(ERR_INPUT, std::to_string(v) + " " + what + ": more than " + std::to_string(most));
+}
+
+// Rows `stride` apart that hold `length` values each do not overlap, and
+// their offsets stay within 2^48 elements.
+void check_stride(size_t stride, size_t length, size_t rows, const char* what) {
+  if (rows > 1 && stride < length)
+    throw Error(ERR_INPUT, std::string(what) + " of " + std::to_string(stride) + " is shorter than a row of " +
+                               std::to_string(length));
+  if (rows > 1 && stride > ((size_t)1 << 48) / rows) throw Error(ERR_INPUT, std::string(what) + " is too large");
+}
+
+constexpr size_t MAX_ROWS = (size_t)INT32_MAX - 1024, MAX_COLS = (size_t)1 << 20;
+
+NormSpec norm_spec(const void* x, int dtype, size_t n, size_t pixels, size_t c, size_t x_stride, size_t x_map_stride,
+                   size_t groups, const float* gamma, const float* beta, float eps, int act) {
+  check_dtype(dtype);
+  check_act(act);
+  check_count(c, MAX_COLS, "channels");
+  check_count(n, 65535, "maps");
+  check_count(pixels, MAX_ROWS, "pixels");
+  if (n) check_count(pixels, MAX_ROWS / n, "pixels per map of the batch");
+  if (groups == 0 || c == 0 || c % groups)
+    throw Error(ERR_INPUT, std::to_string(groups) + " groups do not divide " + std::to_string(c) + " channels");
+  if (!(eps >= 0.0f) || eps > 3e38f) throw Error(ERR_INPUT, "eps is negative or not finite");
+  if (n && pixels) {
+    need_aligned(x, dtype_bytes(dtype), "x");
+    check_stride(x_stride, c, pixels, "x_stride");
+    check_stride(x_map_stride, c, n, "x_map_stride");
+  }
+  if (gamma) need_aligned(gamma, 4, "gamma");
+  if (beta) need_aligned(beta, 4, "beta");
+  NormSpec p;
+  p.x = x;
+  p.dtype = dtype;
+  p.n = (int)n;
+  p.c = (int)c;
+  p.groups = (int)groups;
+  p.pixels = (long long)pixels;
+  p.x_stride = (long long)x_stride;
+  p.x_map_stride = (long long)x_map_stride;
+  p.gamma = gamma;
+  p.beta = beta;
+  p.eps = eps;
+  p.act = act;
+  return p;
+}
+
+Fp8Out fp8_out(uint8_t* codes, size_t code_stride, float* scales, size_t scale_stride, size_t rows, size_t k,
+               size_t block_rows) {
+  Fp8Out q;
+  if (rows && k) {
+    need(codes, "codes");
+    need_aligned(scales, 4, "scales");
+    check_stride(code_stride, k, rows, "code_stride");
+    check_stride(scale_stride, (rows + block_rows - 1) / block_rows, (k + 127) / 128, "scale_stride");
+  }
+  q.codes = codes;
+  q.code_stride = code_stride;
+  q.scales = scales;
+  q.scale_stride = scale_stride;
+  return q;
+}
+
+}  // namespace
+
+iec_status iec_ops_sync(iec_ops* ops, void* stream) {
+  return guard([&] {
+    need_ops(ops);
+    DeviceScope scope(*ops->device);
+    ops->device->sync(ops_stream(*ops->device, stream));
+  });
+}
+
+iec_status iec_ops_group_norm(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
+                              size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
+                              const float* beta, float eps, int act, void* out, size_t out_stride,
+                              size_t out_map_stride, void* stream) {
+  return guard([&] {
+    need_ops(ops);
+    NormSpec p = norm_spec(x, dtype, n, pixels, c, x_stride, x_map_stride, groups, gamma, beta, eps, act);
+    if (n && pixels) {
+      need_aligned(out, dtype_bytes(dtype), "out");
+      check_stride(out_stride, c, pixels, "out_stride");
+      check_stride(out_map_stride, c, n, "out_map_stride");
+    }
+    p.out = out;
+    p.out_stride = (long long)out_stride;
+    p.out_map_stride = (long long)out_map_stride;
+    DeviceScope scope(*ops->device);
+    group_norm(*ops->device, p, ops_stream(*ops->device, stream));
+  });
+}
+
+iec_status iec_ops_group_norm_fp8(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
+                                  size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
+                                  const float* beta, float eps, int act, uint8_t* codes, size_t code_stride,
+                                  float* scales, size_t scale_stride, void* stream) {
+  return guard([&] {
+    need_ops(ops);
+    NormSpec p = norm_spec(x, dtype, n, pixels, c, x_stride, x_map_stride, groups, gamma, beta, eps, act);
+    p.q = fp8_out(codes, code_stride, scales, scale_stride, n * pixels, c, 1);
+    DeviceScope scope(*ops->device);
+    group_norm(*ops->device, p, ops_stream(*ops->device, stream));
+  });
+}
+
+iec_status iec_ops_quantize_fp8(iec_ops* ops, const void* x, int dtype, size_t rows, size_t k, size_t x_stride,
+                                size_t block_rows, uint8_t* codes, size_t code_stride, float* scales,
+                                size_t scale_stride, void* stream) {
+  return guard([&] {
+    need_ops(ops);
+    check_dtype(dtype);
+    check_count(rows, MAX_ROWS, "rows");
+    check_count(k, MAX_COLS, "values a row");
+    if (block_rows != 1 && block_rows != 128)
+      throw Error(ERR_INPUT, "blocks of " + std::to_string(block_rows) + " rows: 1 or 128 are");
+    if (rows && k) {
+      need_aligned(x, dtype_bytes(dtype), "x");
+      check_stride(x_stride, k, rows, "x_stride");
+    }
+    QuantSpec p;
+    p.x = x;
+    p.dtype = dtype;
+    p.rows = (long long)rows;
+    p.k = (int)k;
+    p.x_stride = (long long)x_stride;
+    p.block_rows = (int)block_rows;
+    p.q = fp8_out(codes, code_stride, scales, scale_stride, rows, k, block_rows);
+    DeviceScope scope(*ops->device);
+    quantize_fp8(*ops->device, p, ops_stream(*ops->device, stream));
+  });
+}
+
+iec_status iec_ops_matmul_fp8(iec_ops* ops, const uint8_t* a, size_t a_stride, const float* a_scales,
+                              size_t a_scale_stride, const uint8_t* w, size_t w_stride, const float* w_scales,
+                              size_t w_scale_stride, const float* bias, const void* residual,
+                              size_t residual_stride, size_t m, size_t n, size_t k, int act, int dtype, void* out,
+                              size_t out_stride, void* stream) {
+  return guard([&] {
+    need_ops(ops);
+    check_dtype(dtype);
+    check_act(act);
+    check_count(m, MAX_ROWS, "rows");
+    check_count(n, MAX_COLS, "columns");
+    check_count(k, MAX_COLS, "values a row");
+    if (m && n) {
+      need_aligned(out, dtype_bytes(dtype), "out");
+      check_stride(out_stride, n, m, "out_stride");
+      if (residual) {
+        need_aligned(residual, dtype_bytes(dtype), "residual");
+        check_stride(residual_stride, n, m, "residual_stride");
+      }
+      if (bias) need_aligned(bias, 4, "bias");
+    }
+    if (m && n && k) {
+      need_aligned(a, 16, "a");
+      need_aligned(w, 16, "w");
+      need_aligned(a_scales, 4, "a_scales");
+      need_aligned(w_scales, 4, "w_scales");
+      check_stride(a_stride, k, m, "a_stride");
+      check_stride(w_stride, k, n, "w_stride");
+      check_stride(a_scale_stride, m, (k + 127) / 128, "a_scale_stride");
+      check_stride(w_scale_stride, (n + 127) / 128, (k + 127) / 128, "w_scale_stride");
+      if ((m > 1 && a_stride % 16) || (n > 1 && w_stride % 16))
+        throw Error(ERR_INPUT, "a_stride and w_stride must be multiples of 16 bytes");
+    }
+    Fp8MatmulSpec p;
+    p.a = a;
+    p.w = w;
+    p.a_scales = a_scales;
+    p.w_scales = w_scales;
+    p.a_stride = (long long)a_stride;
+    p.w_stride = (long long)w_stride;
+    p.a_scale_stride = (long long)a_scale_stride;
+    p.w_scale_stride = (long long)w_scale_stride;
+    p.bias = bias;
+    p.residual = residual;
+    p.residual_stride = (long long)residual_stride;
+    p.out = out;
+    p.out_stride = (long long)out_stride;
+    p.m = (int)m;
+    p.n = (int)n;
+    p.k = (int)k;
+    p.act = act;
+    p.dtype = dtype;
+    DeviceScope scope(*ops->device);
+    matmul_fp8(*ops->device, p, ops_stream(*ops->device, stream));
+  });
+}
+
+namespace {
 // The device of a model handle of any kind (by its type tag), or null.
 Device* handle_device(void* handle) {
   if (!handle) return nullptr;
@@ -697,6 +942,7 @@ Device* handle_device(void* handle) {
   if (tag == iec_lama::TAG) return &static_cast<iec_lama*>(handle)->model->device();
   if (tag == iec_birefnet::TAG) return &static_cast<iec_birefnet*>(handle)->model->device();
   if (tag == iec_realesrgan::TAG) return &static_cast<iec_realesrgan*>(handle)->model->device();
+  if (tag == iec_ops::TAG) return static_cast<iec_ops*>(handle)->device.get();
   return nullptr;
 }
 }  // namespace

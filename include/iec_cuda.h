@@ -314,6 +314,89 @@ iec_status iec_birefnet_run_batch(iec_birefnet* model, const uint8_t* images, si
  * rounding. */
 iec_status iec_birefnet_set_fused(iec_birefnet* model, int on);
 
+/* --------------------------------------------------------------- operators
+ * Single operators on DEVICE pointers, for networks built next to the four
+ * models above (no counterpart in the reference): group normalisation over
+ * channels-last maps, and layers in 8-bit floating point. All work is queued
+ * on `stream` (a cudaStream_t; NULL: the handle's own stream, which does not
+ * order itself with any other; cudaStreamLegacy names the legacy default
+ * stream) and the calls return without waiting. Sizes of zero are allowed
+ * and queue nothing where they leave nothing to write. Strides count
+ * elements; rows may be further apart than they are long (a channel slice
+ * of a wider map), never overlap.
+ *
+ * 8-bit rows. A matrix of `rows` x `k` values is kept as e4m3 codes, row by
+ * row, and f32 scales of its blocks of 128 values along k, block by block:
+ * scales[b * scale_stride + r] is block b's scale of row r (block_rows 1) or
+ * of rows 128 r .. 128 r + 127 (block_rows 128, the layout of weights). A
+ * value is code * scale. */
+typedef struct iec_ops iec_ops;
+
+/* Types of the values at a device pointer. */
+typedef enum iec_dtype { IEC_F16 = 0, IEC_BF16 = 1, IEC_F32 = 2 } iec_dtype;
+
+/* Activations: v, max(v, 0), v Phi(v), 1 / (1 + e^-v), v / (1 + e^-v). */
+typedef enum iec_act {
+  IEC_ACT_NONE = 0,
+  IEC_ACT_RELU = 1,
+  IEC_ACT_GELU = 2,
+  IEC_ACT_SIGMOID = 3,
+  IEC_ACT_SILU = 4
+} iec_act;
+
+/* A handle of one GPU: its stream, its scratch and its error state. */
+iec_status iec_ops_open(const iec_options* options, iec_ops** out);
+void iec_ops_free(iec_ops* ops);
+const char* iec_ops_device_name(const iec_ops* ops);
+
+/* Wait (bounded) for the work queued on `stream` (NULL: the handle's) and
+ * report what went wrong in it. */
+iec_status iec_ops_sync(iec_ops* ops, void* stream);
+
+/* Group normalisation with an activation, channels last. `x` holds `n` maps
+ * of `pixels` pixels of `c` channels (pixel p of map i at x + i *
+ * x_map_stride + p * x_stride), `groups` divides c. Over the pixels and the
+ * c / groups channels of each group of a map
+ *   out = act((x - mean) / sqrt(variance + eps) * gamma[channel] + beta[channel]),
+ * the variance without Bessel's correction; `gamma`, `beta` (c floats) may
+ * be NULL (1 and 0). Sums are f32; the result is rounded once to `dtype`,
+ * the type of `x` and `out`. `out` may be `x` itself with its strides. */
+iec_status iec_ops_group_norm(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
+                              size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
+                              const float* beta, float eps, int act, void* out, size_t out_stride,
+                              size_t out_map_stride, void* stream);
+
+/* iec_ops_group_norm with its result, in f32, stored as 8-bit rows of c
+ * values (block_rows 1), one per pixel, map after map: what
+ * iec_ops_matmul_fp8 takes as `a`. */
+iec_status iec_ops_group_norm_fp8(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
+                                  size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
+                                  const float* beta, float eps, int act, uint8_t* codes, size_t code_stride,
+                                  float* scales, size_t scale_stride, void* stream);
+
+/* `rows` x `k` values of `dtype` as 8-bit rows: over each block (of
+ * `block_rows` 1 or 128 rows and 128 values along k, fewer at the edges)
+ *   scale = amax / 448, code = e4m3(x * (448 / amax)), amax = max |x|,
+ * rounded to nearest even. A block whose amax is below 2^-100 gets scale 1
+ * and zero codes. A NaN or an infinity in a block makes its scale NaN or
+ * infinite, and all its values read back as NaN. */
+iec_status iec_ops_quantize_fp8(iec_ops* ops, const void* x, int dtype, size_t rows, size_t k, size_t x_stride,
+                                size_t block_rows, uint8_t* codes, size_t code_stride, float* scales,
+                                size_t scale_stride, void* stream);
+
+/* out (m x n of `dtype`) = act(a w^T + bias) + residual for 8-bit rows `a`
+ * (m x k, block_rows 1) and `w` (n x k, block_rows 128): a linear layer, or
+ * a 1x1 convolution over channels-last pixels. The products of a block of
+ * 128 along k are summed, scaled by both its scales and added up in f32;
+ * the result is rounded once. `bias` (n floats) and `residual` (m x n of
+ * `dtype`, may be `out` itself with its stride) may be NULL. `a` and `w`
+ * must start on 16 bytes, with strides a multiple of 16. */
+iec_status iec_ops_matmul_fp8(iec_ops* ops, const uint8_t* a, size_t a_stride, const float* a_scales,
+                              size_t a_scale_stride, const uint8_t* w, size_t w_stride, const float* w_scales,
+                              size_t w_scale_stride, const float* bias, const void* residual,
+                              size_t residual_stride, size_t m, size_t n, size_t k, int act, int dtype, void* out,
+                              size_t out_stride, void* stream);
+
 /* Launch timing (measurement hooks, no counterpart in the reference).
  * iec_set_launch_timing(model, 1) on any model handle (SCUNet, LaMa,
  * BiRefNet; Real-ESRGAN has its own hooks above) starts a new record: every
