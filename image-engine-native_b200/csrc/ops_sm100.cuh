@@ -46,6 +46,20 @@ __device__ __forceinline__ float op_act_any(float v, int act) {
   return v;
 }
 
+// The activation of N values, one branch for all of them.
+template <int N>
+__device__ __forceinline__ void op_act_n(float* v, int act) {
+#define IEC_OP_ACT(A_)                                  \
+  if (act == A_) {                                      \
+    _Pragma("unroll") for (int e = 0; e < N; e++) v[e] = op_act<A_>(v[e]); \
+  }
+  IEC_OP_ACT(OP_RELU)
+  else IEC_OP_ACT(OP_GELU)
+  else IEC_OP_ACT(OP_SIGMOID)
+  else IEC_OP_ACT(OP_SILU)
+#undef IEC_OP_ACT
+}
+
 constexpr int FP8_BLOCK = 128;  // values along k that share a scale
 
 // The magnitudes' bits order as unsigned integers the way the magnitudes do,

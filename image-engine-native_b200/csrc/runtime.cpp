@@ -427,7 +427,8 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 void encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
-                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box) {
+                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                       CUtensorMapSwizzle swizzle) {
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     cudaDriverEntryPointQueryResult q;
@@ -445,7 +446,7 @@ void encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, con
     if (i + 1 < rank) gstride[i] = strides_bytes[i];
   }
   CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(ERR_GPU, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
 }

@@ -314,7 +314,8 @@ void launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cu
 // cuTensorMapEncodeTiled through the runtime's driver entry point (so the
 // library does not link libcuda and still loads on a machine without it).
 void encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
-                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box);
+                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                       CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
 int device_count();
 

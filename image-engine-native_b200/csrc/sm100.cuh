@@ -206,6 +206,15 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// Tiled 2-D tensor load into this CTA's shared memory; c0 * element size a multiple of 16.
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 // Tiled 3-D tensor load into this CTA's shared memory; c0 * element size a multiple of 16.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
                                             int c2) {
@@ -266,6 +275,18 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
       : "memory");
 }
 
+// D[tmem] (+)= A[smem desc] x B[smem desc]^T, 8-bit floating-point inputs
+// (32 values along K per instruction), f32 accumulators.
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive on `bar` once every MMA this thread issued before has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -314,6 +335,16 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// The same wait, naming the 16 registers of a load before it, so that no use
+// of them is moved above it.
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 // 32 lanes x 16 columns of 32 bits: thread t gets lane (taddr.lane + t),
 // columns taddr.col .. +15.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
@@ -350,6 +381,29 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
   d |= (uint64_t)1 << 46;  // descriptor version for sm_100
   // base offset 0, absolute LBO mode 0, layout type 0 = SWIZZLE_NONE
   return d;
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle, K-major: rows of 128
+// bytes, groups of 8 rows 1024 bytes apart, the tile on a 1024-byte boundary
+// (the layout a TMA load with CU_TENSOR_MAP_SWIZZLE_128B writes). A step of
+// 32 bytes along K adds 2 to the descriptor.
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)1 << 16;            // leading offset: not used by swizzled layouts
+  d |= (uint64_t)(1024 >> 4) << 32;  // stride between groups of 8 rows
+  d |= (uint64_t)1 << 46;            // descriptor version for sm_100
+  d |= (uint64_t)2 << 61;            // layout type SWIZZLE_128B
+  return d;
+}
+
+// Instruction descriptor of kind::f8f6f4: e4m3 A and B, both K-major, f32 D.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(uint32_t m, uint32_t n) {
+  return (1u << 4)              // D format f32
+         | (0u << 7)            // A format e4m3
+         | (0u << 10)           // B format e4m3
+         | ((n >> 3) << 17)     // N / 8
+         | ((m >> 4) << 24);    // M / 16
 }
 
 // Instruction descriptor of kind::f16: f16 A and B, both K-major, f32 D.
