@@ -756,37 +756,37 @@ void check_stride(size_t stride, size_t length, size_t rows, const char* what) {
 
 constexpr size_t MAX_ROWS = (size_t)INT32_MAX - 1024, MAX_COLS = (size_t)1 << 20;
 
-NormSpec norm_spec(const void* x, int dtype, size_t n, size_t pixels, size_t c, size_t x_stride, size_t x_map_stride,
-                   size_t groups, const float* gamma, const float* beta, float eps, int act) {
-  check_dtype(dtype);
-  check_act(act);
-  check_count(c, MAX_COLS, "channels");
-  check_count(n, 65535, "maps");
-  check_count(pixels, MAX_ROWS, "pixels");
-  if (n) check_count(pixels, MAX_ROWS / n, "pixels per map of the batch");
-  if (groups == 0 || c == 0 || c % groups)
-    throw Error(ERR_INPUT, std::to_string(groups) + " groups do not divide " + std::to_string(c) + " channels");
-  if (!(eps >= 0.0f) || eps > 3e38f) throw Error(ERR_INPUT, "eps is negative or not finite");
-  if (n && pixels) {
-    need_aligned(x, dtype_bytes(dtype), "x");
-    check_stride(x_stride, c, pixels, "x_stride");
-    check_stride(x_map_stride, c, n, "x_map_stride");
+NormSpec norm_spec(const iec_group_norm_args* a) {
+  need(a, "args");
+  check_dtype(a->dtype);
+  check_act(a->act);
+  check_count(a->c, MAX_COLS, "channels");
+  check_count(a->n, 65535, "maps");
+  check_count(a->pixels, MAX_ROWS, "pixels");
+  if (a->n) check_count(a->pixels, MAX_ROWS / a->n, "pixels a map of the batch");
+  if (a->groups == 0 || a->c == 0 || a->c % a->groups)
+    throw Error(ERR_INPUT, std::to_string(a->groups) + " groups do not divide " + std::to_string(a->c) + " channels");
+  if (!(a->eps >= 0.0f) || a->eps > 3e38f) throw Error(ERR_INPUT, "eps is negative or not finite");
+  if (a->n && a->pixels) {
+    need_aligned(a->x, dtype_bytes(a->dtype), "x");
+    check_stride(a->x_stride, a->c, a->pixels, "x_stride");
+    check_stride(a->x_map_stride, a->c, a->n, "x_map_stride");
   }
-  if (gamma) need_aligned(gamma, 4, "gamma");
-  if (beta) need_aligned(beta, 4, "beta");
+  if (a->gamma) need_aligned(a->gamma, 4, "gamma");
+  if (a->beta) need_aligned(a->beta, 4, "beta");
   NormSpec p;
-  p.x = x;
-  p.dtype = dtype;
-  p.n = (int)n;
-  p.c = (int)c;
-  p.groups = (int)groups;
-  p.pixels = (long long)pixels;
-  p.x_stride = (long long)x_stride;
-  p.x_map_stride = (long long)x_map_stride;
-  p.gamma = gamma;
-  p.beta = beta;
-  p.eps = eps;
-  p.act = act;
+  p.x = a->x;
+  p.dtype = a->dtype;
+  p.n = (int)a->n;
+  p.c = (int)a->c;
+  p.groups = (int)a->groups;
+  p.pixels = (long long)a->pixels;
+  p.x_stride = (long long)a->x_stride;
+  p.x_map_stride = (long long)a->x_map_stride;
+  p.gamma = a->gamma;
+  p.beta = a->beta;
+  p.eps = a->eps;
+  p.act = a->act;
   return p;
 }
 
@@ -816,118 +816,111 @@ iec_status iec_ops_sync(iec_ops* ops, void* stream) {
   });
 }
 
-iec_status iec_ops_group_norm(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
-                              size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
-                              const float* beta, float eps, int act, void* out, size_t out_stride,
-                              size_t out_map_stride, void* stream) {
+iec_status iec_ops_group_norm(iec_ops* ops, const iec_group_norm_args* args, void* stream) {
   return guard([&] {
     need_ops(ops);
-    NormSpec p = norm_spec(x, dtype, n, pixels, c, x_stride, x_map_stride, groups, gamma, beta, eps, act);
-    if (n && pixels) {
-      need_aligned(out, dtype_bytes(dtype), "out");
-      check_stride(out_stride, c, pixels, "out_stride");
-      check_stride(out_map_stride, c, n, "out_map_stride");
+    NormSpec p = norm_spec(args);
+    if (p.n && p.pixels) {
+      need_aligned(args->out, dtype_bytes(p.dtype), "out");
+      check_stride(args->out_stride, args->c, args->pixels, "out_stride");
+      check_stride(args->out_map_stride, args->c, args->n, "out_map_stride");
     }
-    p.out = out;
-    p.out_stride = (long long)out_stride;
-    p.out_map_stride = (long long)out_map_stride;
+    p.out = args->out;
+    p.out_stride = (long long)args->out_stride;
+    p.out_map_stride = (long long)args->out_map_stride;
     DeviceScope scope(*ops->device);
     group_norm(*ops->device, p, ops_stream(*ops->device, stream));
   });
 }
 
-iec_status iec_ops_group_norm_fp8(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
-                                  size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
-                                  const float* beta, float eps, int act, uint8_t* codes, size_t code_stride,
-                                  float* scales, size_t scale_stride, void* stream) {
+iec_status iec_ops_group_norm_fp8(iec_ops* ops, const iec_group_norm_args* args, void* stream) {
   return guard([&] {
     need_ops(ops);
-    NormSpec p = norm_spec(x, dtype, n, pixels, c, x_stride, x_map_stride, groups, gamma, beta, eps, act);
-    p.q = fp8_out(codes, code_stride, scales, scale_stride, n * pixels, c, 1);
+    NormSpec p = norm_spec(args);
+    p.q = fp8_out(args->codes, args->code_stride, args->scales, args->scale_stride, args->n * args->pixels, args->c, 1);
     DeviceScope scope(*ops->device);
     group_norm(*ops->device, p, ops_stream(*ops->device, stream));
   });
 }
 
-iec_status iec_ops_quantize_fp8(iec_ops* ops, const void* x, int dtype, size_t rows, size_t k, size_t x_stride,
-                                size_t block_rows, uint8_t* codes, size_t code_stride, float* scales,
-                                size_t scale_stride, void* stream) {
+iec_status iec_ops_quantize_fp8(iec_ops* ops, const iec_quantize_fp8_args* args, void* stream) {
   return guard([&] {
     need_ops(ops);
-    check_dtype(dtype);
-    check_count(rows, MAX_ROWS, "rows");
-    check_count(k, MAX_COLS, "values a row");
-    if (block_rows != 1 && block_rows != 128)
-      throw Error(ERR_INPUT, "blocks of " + std::to_string(block_rows) + " rows: 1 or 128 are");
-    if (rows && k) {
-      need_aligned(x, dtype_bytes(dtype), "x");
-      check_stride(x_stride, k, rows, "x_stride");
+    need(args, "args");
+    const iec_quantize_fp8_args& a = *args;
+    check_dtype(a.dtype);
+    check_count(a.rows, MAX_ROWS, "rows");
+    check_count(a.k, MAX_COLS, "values a row");
+    if (a.block_rows != 1 && a.block_rows != 128)
+      throw Error(ERR_INPUT, "blocks of " + std::to_string(a.block_rows) + " rows: 1 or 128 are taken");
+    if (a.rows && a.k) {
+      need_aligned(a.x, dtype_bytes(a.dtype), "x");
+      check_stride(a.x_stride, a.k, a.rows, "x_stride");
     }
     QuantSpec p;
-    p.x = x;
-    p.dtype = dtype;
-    p.rows = (long long)rows;
-    p.k = (int)k;
-    p.x_stride = (long long)x_stride;
-    p.block_rows = (int)block_rows;
-    p.q = fp8_out(codes, code_stride, scales, scale_stride, rows, k, block_rows);
+    p.x = a.x;
+    p.dtype = a.dtype;
+    p.rows = (long long)a.rows;
+    p.k = (int)a.k;
+    p.x_stride = (long long)a.x_stride;
+    p.block_rows = (int)a.block_rows;
+    p.q = fp8_out(a.codes, a.code_stride, a.scales, a.scale_stride, a.rows, a.k, a.block_rows);
     DeviceScope scope(*ops->device);
     quantize_fp8(*ops->device, p, ops_stream(*ops->device, stream));
   });
 }
 
-iec_status iec_ops_matmul_fp8(iec_ops* ops, const uint8_t* a, size_t a_stride, const float* a_scales,
-                              size_t a_scale_stride, const uint8_t* w, size_t w_stride, const float* w_scales,
-                              size_t w_scale_stride, const float* bias, const void* residual,
-                              size_t residual_stride, size_t m, size_t n, size_t k, int act, int dtype, void* out,
-                              size_t out_stride, void* stream) {
+iec_status iec_ops_matmul_fp8(iec_ops* ops, const iec_matmul_fp8_args* args, void* stream) {
   return guard([&] {
     need_ops(ops);
-    check_dtype(dtype);
-    check_act(act);
-    check_count(m, MAX_ROWS, "rows");
-    check_count(n, MAX_COLS, "columns");
-    check_count(k, MAX_COLS, "values a row");
-    if (m && n) {
-      need_aligned(out, dtype_bytes(dtype), "out");
-      check_stride(out_stride, n, m, "out_stride");
-      if (residual) {
-        need_aligned(residual, dtype_bytes(dtype), "residual");
-        check_stride(residual_stride, n, m, "residual_stride");
+    need(args, "args");
+    const iec_matmul_fp8_args& a = *args;
+    check_dtype(a.dtype);
+    check_act(a.act);
+    check_count(a.m, MAX_ROWS, "rows");
+    check_count(a.n, MAX_COLS, "columns");
+    check_count(a.k, MAX_COLS, "values a row");
+    if (a.m && a.n) {
+      need_aligned(a.out, dtype_bytes(a.dtype), "out");
+      check_stride(a.out_stride, a.n, a.m, "out_stride");
+      if (a.residual) {
+        need_aligned(a.residual, dtype_bytes(a.dtype), "residual");
+        check_stride(a.residual_stride, a.n, a.m, "residual_stride");
       }
-      if (bias) need_aligned(bias, 4, "bias");
+      if (a.bias) need_aligned(a.bias, 4, "bias");
     }
-    if (m && n && k) {
-      need_aligned(a, 16, "a");
-      need_aligned(w, 16, "w");
-      need_aligned(a_scales, 4, "a_scales");
-      need_aligned(w_scales, 4, "w_scales");
-      check_stride(a_stride, k, m, "a_stride");
-      check_stride(w_stride, k, n, "w_stride");
-      check_stride(a_scale_stride, m, (k + 127) / 128, "a_scale_stride");
-      check_stride(w_scale_stride, (n + 127) / 128, (k + 127) / 128, "w_scale_stride");
-      if ((m > 1 && a_stride % 16) || (n > 1 && w_stride % 16))
+    if (a.m && a.n && a.k) {
+      const size_t blocks = (a.k + 127) / 128;
+      need_aligned(a.a, 16, "a");
+      need_aligned(a.w, 16, "w");
+      need_aligned(a.a_scales, 4, "a_scales");
+      need_aligned(a.w_scales, 4, "w_scales");
+      check_stride(a.a_stride, a.k, a.m, "a_stride");
+      check_stride(a.w_stride, a.k, a.n, "w_stride");
+      check_stride(a.a_scale_stride, a.m, blocks, "a_scale_stride");
+      check_stride(a.w_scale_stride, (a.n + 127) / 128, blocks, "w_scale_stride");
+      if ((a.m > 1 && a.a_stride % 16) || (a.n > 1 && a.w_stride % 16))
         throw Error(ERR_INPUT, "a_stride and w_stride must be multiples of 16 bytes");
     }
     Fp8MatmulSpec p;
-    p.a = a;
-    p.w = w;
-    p.a_scales = a_scales;
-    p.w_scales = w_scales;
-    p.a_stride = (long long)a_stride;
-    p.w_stride = (long long)w_stride;
-    p.a_scale_stride = (long long)a_scale_stride;
-    p.w_scale_stride = (long long)w_scale_stride;
-    p.bias = bias;
-    p.residual = residual;
-    p.residual_stride = (long long)residual_stride;
-    p.out = out;
-    p.out_stride = (long long)out_stride;
-    p.m = (int)m;
-    p.n = (int)n;
-    p.k = (int)k;
-    p.act = act;
-    p.dtype = dtype;
+    p.a = a.a;
+    p.w = a.w;
+    p.a_scales = a.a_scales;
+    p.w_scales = a.w_scales;
+    p.a_stride = (long long)a.a_stride;
+    p.w_stride = (long long)a.w_stride;
+    p.a_scale_stride = (long long)a.a_scale_stride;
+    p.w_scale_stride = (long long)a.w_scale_stride;
+    p.bias = a.bias;
+    p.residual = a.residual;
+    p.residual_stride = (long long)a.residual_stride;
+    p.out = a.out;
+    p.out_stride = (long long)a.out_stride;
+    p.m = (int)a.m;
+    p.n = (int)a.n;
+    p.k = (int)a.k;
+    p.act = a.act;
+    p.dtype = a.dtype;
     DeviceScope scope(*ops->device);
     matmul_fp8(*ops->device, p, ops_stream(*ops->device, stream));
   });

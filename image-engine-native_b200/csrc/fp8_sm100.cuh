@@ -10,12 +10,22 @@
 // lane quarter holds row t, so the scale of a is one register and that of w
 // is the same for all its columns.
 //
-// Persistent CTAs of 320 threads walk the tiles: warp 0 loads (TMA, 128-byte
-// swizzle), warp 1 issues the MMAs, warps 2..9 (two per TMEM lane quarter,
-// half the columns each) scale and add the blocks and write the tile. All
-// waits are bounded.
+// fp8_gemm_sm100<T, PAIR>: PAIR = 1 takes tiles of 256 x 256 by two CTAs of a
+// cluster (cta_group::2: each loads its 128 rows of a and half the rows of w
+// and holds its rows' accumulators), 0 tiles of 128 x 128 by one. Persistent
+// CTAs of 12 warps walk the tiles: warp 0 loads (TMA, 128-byte swizzle), warp
+// 1 issues the MMAs, warps 4..11 (two per TMEM lane quarter, half the columns
+// each) scale and add the blocks and write the tile; they take the registers
+// that the others give up (setmaxnreg), 128 of them for the sums of a row's
+// 128 columns. A tile is written through shared memory by TMA, each warp its
+// own 32 rows, and the residual comes in the same way while the tile's MMAs
+// run; where the rows of out or residual do not start on 16 bytes, they are
+// written through shared memory with plain accesses. All waits are bounded.
 #pragma once
 
+#include <type_traits>
+
+#include "igemm_sm100.cuh"
 #include "ops_sm100.cuh"
 #include "sm100.cuh"
 
@@ -31,23 +41,23 @@ struct Fp8Params {
   const void* residual;
   void* out;
   long long residual_stride, out_stride;
-  int wide;  // rows of out (and residual) start on 32 bytes
+  int tma_out;  // out and residual have tensor maps
   int* dev_err;
 };
 
-constexpr int FP8_THREADS = 320;
+constexpr int FP8_THREADS = 384;
+constexpr int FP8_EPI_WARPS = 8;
 constexpr int FP8_GROUP = 8;  // M tiles walked together, so that L2 serves their w tiles
 
-template <int BN>
 struct Fp8Smem {
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int NSTAGE = BN == 256 ? 4 : 6;
-  static constexpr int STG_PITCH = 33;  // a warp's 32 x 32 patch of the output, one float of padding a row
-  static constexpr int STG_OFF = NSTAGE * STAGE, STG_BYTES = 8 * 32 * STG_PITCH * 4;
-  static constexpr int BAR_OFF = STG_OFF + STG_BYTES;
-  static constexpr int MISC_OFF = BAR_OFF + (2 * NSTAGE + 4) * 8;
-  static constexpr int BYTES = MISC_OFF + 16;
-  static constexpr int DYN_BYTES = BYTES + 1024;
+  static constexpr int HALF_BYTES = 128 * 128, STAGE = 2 * HALF_BYTES;  // a's rows, w's rows
+  static constexpr int NSTAGE = 4;
+  static constexpr int OUT_OFF = NSTAGE * STAGE, OUT_WARP = 8192;  // a warp's patch of the output
+  static constexpr int BIAS_OFF = OUT_OFF + FP8_EPI_WARPS * OUT_WARP;
+  static constexpr int BAR_OFF = BIAS_OFF + FP8_EPI_WARPS * 128 * 4;
+  static constexpr int MISC_OFF = BAR_OFF + (2 * NSTAGE + 8 + FP8_EPI_WARPS) * 8;
+  static constexpr int DYN_BYTES = MISC_OFF + 16 + 1024;
+  static_assert(DYN_BYTES <= 232448, "shared memory of a CTA");
 };
 
 // Tile -> (M tile, N tile), in groups of FP8_GROUP M tiles.
@@ -58,106 +68,137 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, int tile, int* mt, 
   *mt = g * FP8_GROUP + r - *nt * rows;
 }
 
-// 32 bytes to or from global memory, 32-byte aligned.
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-__device__ __forceinline__ void ld_global_32(const void* p, uint32_t* v) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "l"(p)
-               : "memory");
+template <class T>
+__device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
+  const T a = from_f32<T>(lo), b = from_f32<T>(hi);
+  return (uint32_t) reinterpret_cast<const uint16_t&>(a) | (uint32_t) reinterpret_cast<const uint16_t&>(b) << 16;
 }
 
-// 32 bytes of T to f32 and back.
+// 16 bytes of T: add to f32, or make from f32.
 template <class T>
-__device__ __forceinline__ void unpack_32(const uint32_t* v, float* f) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void add_16(float* f, uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = __uint_as_float(v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      T lo, hi;
-      reinterpret_cast<uint16_t&>(lo) = (uint16_t)(v[i] & 0xffffu);
-      reinterpret_cast<uint16_t&>(hi) = (uint16_t)(v[i] >> 16);
-      f[2 * i] = to_f32(lo);
-      f[2 * i + 1] = to_f32(hi);
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] += __uint_as_float(w[i]);
+    } else {
+      const uint16_t lo = (uint16_t)(w[i] & 0xffffu), hi = (uint16_t)(w[i] >> 16);
+      f[2 * i] += to_f32(reinterpret_cast<const T&>(lo));
+      f[2 * i + 1] += to_f32(reinterpret_cast<const T&>(hi));
     }
   }
 }
 template <class T>
-__device__ __forceinline__ void pack_32(const float* f, uint32_t* v) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __float_as_uint(f[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const T lo = from_f32<T>(f[2 * i]), hi = from_f32<T>(f[2 * i + 1]);
-      v[i] = (uint32_t) reinterpret_cast<const uint16_t&>(lo) | (uint32_t) reinterpret_cast<const uint16_t&>(hi) << 16;
-    }
-  }
+__device__ __forceinline__ uint4 make_16(const float* f) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else
+    return make_uint4(pack_2<T>(f[0], f[1]), pack_2<T>(f[2], f[3]), pack_2<T>(f[4], f[5]), pack_2<T>(f[6], f[7]));
 }
 
-template <class T, int BN>
+// The activation in an unrolled epilogue: op_act, but GELU by the form of
+// igemm_sm100.cuh, a third of erff's instructions (|error| <= 1.5e-7 |v|).
+template <int ACT>
+__device__ __forceinline__ float fp8_act(float v) {
+  if (ACT == OP_GELU) return gemm_gelu(v);
+  return op_act<ACT>(v);
+}
+
+template <int REGS>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+#ifndef FP8_NPART
+#define FP8_NPART 1
+#endif
+template <class T, int PAIR>
 __global__ void __launch_bounds__(FP8_THREADS, 1)
     fp8_gemm_sm100(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap w_map,
+                   const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
                    const Fp8Params p) {
-  using L = Fp8Smem<BN>;
+  using L = Fp8Smem;
+  constexpr int BM = PAIR ? 256 : 128, BN = BM, CW = BN / 2;  // CW: columns of a thread
+  constexpr int NPART = FP8_NPART;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // of a pair, only the first CTA's is used
   uint64_t* empty = full + L::NSTAGE;
-  uint64_t* acc_full = empty + L::NSTAGE;
-  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* acc_full = empty + L::NSTAGE;  // [part][accumulator]
+  uint64_t* acc_empty = acc_full + 4;      // of a pair, only the first CTA's is used
+  uint64_t* res_full = acc_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::NSTAGE; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < 2; a++) {
+    for (int a = 0; a < 4; a++) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], FP8_EPI_WARPS / NPART * (PAIR ? 2 : 1));
     }
+    for (int w = 0; w < FP8_EPI_WARPS; w++) mbar_init(&res_full[w], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * BN);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, 2 * BN);
+    } else {
+      tmem_alloc(tmem_slot, 2 * BN);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  __syncwarp();
+  if (PAIR) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   griddep_launch_dependents();
   griddep_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    regs_dec<104>();
+    if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ producer
       int s = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+      for (int tile = first; tile < p.tiles && ok; tile += step) {
         int mt, nt;
         fp8_tile(p, tile, &mt, &nt);
+        const int row = mt * BM + (int)rank * 128, col = nt * BN + (int)rank * (BN / NPART / 2);
         for (int kb = 0; kb < p.kblocks; kb++) {
           if (!mbar_wait(&empty[s], phase ^ 1, abort_flag, p.dev_err, DEV_ERR_WAIT_EMPTY)) {
             ok = false;
             break;
           }
           uint8_t* st = smem + s * L::STAGE;
-          mbar_arrive_expect_tx(&full[s], L::STAGE);
-          tma_load_2d(st, &a_map, &full[s], kb * FP8_BLOCK, mt * 128);
-          tma_load_2d(st + L::A_BYTES, &w_map, &full[s], kb * FP8_BLOCK, nt * BN);
+          if (PAIR) {
+            // both CTAs' bytes complete on the first one's barrier
+            const uint32_t bar = cluster_map(&full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
+            tma_load_2d_pair(st, &a_map, bar, kb * FP8_BLOCK, row);
+            // half of the rows of w of each part
+            tma_load_2d_pair(st + L::HALF_BYTES, &w_map, bar, kb * FP8_BLOCK, col);
+            tma_load_2d_pair(st + L::HALF_BYTES + L::HALF_BYTES / 2, &w_map, bar, kb * FP8_BLOCK, NPART == 2 ? col + CW : col + 64);
+          } else {
+            mbar_arrive_expect_tx(&full[s], L::STAGE);
+            tma_load_2d(st, &a_map, &full[s], kb * FP8_BLOCK, row);
+            tma_load_2d(st + L::HALF_BYTES, &w_map, &full[s], kb * FP8_BLOCK, col);
+            tma_load_2d(st + L::HALF_BYTES + L::HALF_BYTES / 2, &w_map, &full[s], kb * FP8_BLOCK, col + 64);
+          }
           issued++;
           if (++s == L::NSTAGE) {
             s = 0;
@@ -165,33 +206,52 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
           }
         }
       }
-      // the copies in flight land before the CTA's shared memory goes
+      // the stages in flight are consumed before this CTA's memory goes
       for (int i = max(0, issued - L::NSTAGE); i < issued; i++)
-        mbar_wait(&full[i % L::NSTAGE], (uint32_t)(i / L::NSTAGE) & 1, abort_flag, p.dev_err, 0);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+        mbar_wait(&empty[i % L::NSTAGE], (uint32_t)(i / L::NSTAGE) & 1, abort_flag, p.dev_err, 0);
+    } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc = idesc_e4m3_f32(128, BN);
+      // (the whole warp walks the loop, one lane issues: see elect_one)
+      constexpr uint32_t idesc = idesc_e4m3_f32(BM, BN / NPART);
+      const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
       int s = 0, i = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
+      for (int tile = first; tile < p.tiles && ok; tile += step)
         for (int kb = 0; kb < p.kblocks; kb++, i++) {
-          const int a = i & 1;
-          if (!mbar_wait(&acc_empty[a], ((uint32_t)(i >> 1) & 1) ^ 1, abort_flag, p.dev_err, DEV_ERR_WAIT_ACC_EMPTY) ||
-              !mbar_wait(&full[s], phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t adesc = smem_desc_sw128(smem_u32(smem + s * L::STAGE));
-          const uint64_t bdesc = smem_desc_sw128(smem_u32(smem + s * L::STAGE + L::A_BYTES));
+          ok = __all_sync(~0u, mbar_wait(&full[s], phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL));
+          if (!ok) break;
+          const uint64_t adesc = desc0 + (uint32_t)(s * (L::STAGE >> 4));
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            umma_f8(tmem_base + (uint32_t)(a * BN), adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
-          umma_commit(&empty[s]);
-          umma_commit(&acc_full[a]);
+          for (int part = 0; part < NPART; part++) {
+            const int a = part * 2 + (i & 1);
+            ok = __all_sync(~0u, mbar_wait(&acc_empty[a], ((uint32_t)(i >> 1) & 1) ^ 1, abort_flag, p.dev_err,
+                                           DEV_ERR_WAIT_ACC_EMPTY));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t bdesc = adesc + (uint32_t)((L::HALF_BYTES + part * (L::HALF_BYTES / 2)) >> 4);
+            const uint32_t d = tmem_base + (uint32_t)(a * (BN / NPART));
+            if (elect_one()) {
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                if (PAIR)
+                  umma_f8_pair(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
+                else
+                  umma_f8(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
+              }
+              if (PAIR)
+                umma_commit_pair(&acc_full[a]);
+              else
+                umma_commit(&acc_full[a]);
+              if (part == NPART - 1) {
+                if (PAIR)
+                  umma_commit_pair(&empty[s]);
+                else
+                  umma_commit(&empty[s]);
+              }
+            }
+          }
+          if (!ok) break;
           if (++s == L::NSTAGE) {
             s = 0;
             phase ^= 1;
@@ -199,33 +259,69 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         }
       // the MMAs in flight end before TMEM is freed
       for (int q = max(0, i - 2); q < i; q++)
-        mbar_wait(&acc_full[q & 1], (uint32_t)(q >> 1) & 1, abort_flag, p.dev_err, 0);
+        for (int part = 0; part < NPART; part++)
+          mbar_wait(&acc_full[part * 2 + (q & 1)], (uint32_t)(q >> 1) & 1, abort_flag, p.dev_err, 0);
     }
   } else {
     // ------------------------------------------- scaling, sums and epilogue
-    constexpr int CW = BN / 2;  // columns of a thread
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    float* stg = reinterpret_cast<float*>(smem + L::STG_OFF) + (warp - 2) * 32 * L::STG_PITCH;
-    const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * CW);
+    regs_inc<200>();
+    // The output patch in shared memory: boxes of 32 rows x 128 bytes,
+    // 128-byte swizzled, BOXES at a time, ROUNDS times.
+    constexpr int BOX_COLS = 128 / (int)sizeof(T), BOXES = CW * (int)sizeof(T) / 128 < 2 ? 1 : 2;
+    constexpr int ROUNDS = CW / (BOXES * BOX_COLS), V = 16 / (int)sizeof(T);
+    const int e = warp - 4, quarter = warp & 3, part = e >> 2;
+    uint8_t* patch = smem + L::OUT_OFF + e * L::OUT_WARP;
+    float* sbias = reinterpret_cast<float*>(smem + L::BIAS_OFF) + e * 128;
+    const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(NPART == 2 ? part * 2 * CW : part * CW);
+    uint64_t* const part_full = acc_full + (NPART == 2 ? part * 2 : 0);
+    uint64_t* const part_empty = acc_empty + (NPART == 2 ? part * 2 : 0);
+    const uint32_t acc_bar = PAIR ? cluster_map(part_empty, 0) : 0;
     int i = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+    uint32_t res_phase = 0;
+    bool ok = true, res_flying = false;
+
+    // Round `r` of a tile's residual into the patch (lane 0; the patch free).
+    auto load_residual = [&](int row, int col, int r) __attribute__((noinline)) {
+      res_flying = true;
+      mbar_arrive_expect_tx(&res_full[e], BOXES * 4096);
+      for (int b = 0; b < BOXES; b++)
+        tma_load_2d(patch + b * 4096, &res_map, &res_full[e], col + (r * BOXES + b) * BOX_COLS, row);
+    };
+
+    // A tile's first row and column of this warp, and its first scales.
+    int row0 = 0, col0 = 0;
+    const float* sa = p.a_scales;
+    const float* sw = p.w_scales;
+    float sa_next = 0.0f, sw_next = 0.0f;
+    auto enter_tile = [&](int tile) {
       int mt, nt;
       fp8_tile(p, tile, &mt, &nt);
-      const int row0 = mt * 128 + quarter * 32, row = row0 + lane, col0 = nt * BN + half * CW;
-      const float* sa = p.a_scales + min(row, p.m - 1);
-      const float* sw = p.w_scales + min(col0, p.n - 1) / FP8_BLOCK;
-      float2 acc[CW / 2];
-#pragma unroll
-      for (int c = 0; c < CW / 2; c++) acc[c] = make_float2(0.0f, 0.0f);
-      float sa_next = 0.0f, sw_next = 0.0f;
+      row0 = mt * BM + (int)rank * 128 + quarter * 32;
+      col0 = nt * BN + part * CW;
+      sa = p.a_scales + min(row0 + lane, p.m - 1);
+      sw = p.w_scales + min(col0, p.n - 1) / FP8_BLOCK;
       if (p.kblocks) {
-        sa_next = sa[0];
-        sw_next = sw[0];
+        sa_next = *sa;
+        sw_next = *sw;
       }
+    };
+    if (first < p.tiles) enter_tile(first);
+
+    for (int tile = first; tile < p.tiles && ok; tile += step) {
+      const int row_t = row0, col_t = col0;
+      const bool any = row_t < p.m && col_t < p.n;
+      float bias_r[CW / 32];
+#pragma unroll
+      for (int c = 0; c < CW / 32; c++) {
+        const int col = col_t + c * 32 + lane;
+        bias_r[c] = p.bias && col < p.n ? p.bias[col] : 0.0f;
+      }
+      uint64_t acc[CW / 2];  // f32 pairs
+#pragma unroll
+      for (int c = 0; c < CW / 2; c++) acc[c] = 0;
       for (int kb = 0; kb < p.kblocks; kb++, i++) {
         const float s1 = sa_next * sw_next;
-        const float2 s2 = make_float2(s1, s1);
+        const uint64_t s2 = pack_f32x2(s1, s1);
         if (kb + 1 < p.kblocks) {
           sa += p.a_scale_stride;
           sw += p.w_scale_stride;
@@ -233,13 +329,13 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
           sw_next = *sw;
         }
         const int a = i & 1;
-        if (!mbar_wait(&acc_full[a], (uint32_t)(i >> 1) & 1, abort_flag, p.dev_err, DEV_ERR_WAIT_ACC_FULL)) ok = false;
+        if (!mbar_wait(&part_full[a], (uint32_t)(i >> 1) & 1, abort_flag, p.dev_err, DEV_ERR_WAIT_ACC_FULL)) ok = false;
         if (__any_sync(~0u, !ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t t = lanes + (uint32_t)(a * BN);
+        const uint32_t t = lanes + (uint32_t)(a * (BN / NPART));
         uint32_t r[2][16];
         tmem_ld16(t, r[0]);
 #pragma unroll
@@ -249,76 +345,140 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
             tmem_ld16(t + (uint32_t)(16 * (c + 1)), r[(c + 1) & 1]);
           } else {
             tc_fence_before();
-            if (lane == 0) mbar_arrive(&acc_empty[a]);
+            if (lane == 0) {
+              if (PAIR)
+                mbar_arrive_cluster(acc_bar + (uint32_t)(a * 8));
+              else
+                mbar_arrive(&part_empty[a]);
+            }
           }
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            acc[c * 8 + e] = ffma2(make_float2(__uint_as_float(r[c & 1][2 * e]), __uint_as_float(r[c & 1][2 * e + 1])), s2,
-                                   acc[c * 8 + e]);
+          for (int q = 0; q < 8; q++) ffma2_acc(acc[c * 8 + q], r[c & 1][2 * q], r[c & 1][2 * q + 1], s2);
+        }
+        // The residual, once the last tile has left the patch: behind the
+        // first block, so that the wait for the patch delays nothing.
+        if (kb == 0 && p.tma_out && p.residual && any && lane == 0) {
+          bulk_wait_read();
+          load_residual(row_t, col_t, 0);
         }
       }
       if (!ok) break;
-      // ---- bias, activation, residual, rounding
-      constexpr int V = 32 / (int)sizeof(T);
-      const bool whole = p.wide && col0 + CW <= p.n;
-      if (whole) {
-        if (row < p.m) {
-          T* out = static_cast<T*>(p.out) + row * p.out_stride + col0;
-          const T* res = static_cast<const T*>(p.residual) + (p.residual ? row * p.residual_stride + col0 : 0);
-#pragma unroll
-          for (int c = 0; c < CW / V; c++) {
-            float v[V];
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-              const float2 pr = acc[(c * V + e) / 2];
-              v[e] = e & 1 ? pr.y : pr.x;
-            }
-            if (p.bias)
-#pragma unroll
-              for (int e = 0; e < V; e++) v[e] += p.bias[col0 + c * V + e];
-            op_act_n<V>(v, p.act);
-            uint32_t w[8];
-            if (p.residual) {
-              float f[V];
-              ld_global_32(res + c * V, w);
-              unpack_32<T>(w, f);
-#pragma unroll
-              for (int e = 0; e < V; e++) v[e] += f[e];
-            }
-            pack_32<T>(v, w);
-            st_global_32(out + c * V, w);
-          }
-        }
-      } else {
-        // Through shared memory, 32 x 32 at a time, so that a warp's accesses
-        // are runs of a row wherever the rows start.
-#pragma unroll
-        for (int c = 0; c < CW / 32; c++) {
-          if (col0 + c * 32 >= p.n) break;
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            stg[lane * L::STG_PITCH + 2 * e] = acc[c * 16 + e].x;
-            stg[lane * L::STG_PITCH + 2 * e + 1] = acc[c * 16 + e].y;
-          }
-          __syncwarp();
-          const int col = col0 + c * 32 + lane;
-          if (col < p.n) {
-            const float b = p.bias ? p.bias[col] : 0.0f;
-            const int rows = min(32, p.m - row0);
-            for (int r = 0; r < rows; r++) {
-              float v = op_act_any(stg[r * L::STG_PITCH + lane] + b, p.act);
-              if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[(row0 + r) * p.residual_stride + col]);
-              static_cast<T*>(p.out)[(row0 + r) * p.out_stride + col] = from_f32<T>(v);
-            }
-          }
-        }
+      if (tile + step < p.tiles) enter_tile(tile + step);  // its first scales are on their way
+      if (!any) continue;
+      if (lane == 0) {
+        bulk_wait_read();  // the last tile has left the patch
+        if (p.kblocks == 0 && p.tma_out && p.residual) load_residual(row_t, col_t, 0);
       }
+#pragma unroll
+      for (int c = 0; c < CW / 32; c++) sbias[c * 32 + lane] = bias_r[c];
+      __syncwarp();
+      // ---- bias, activation, residual, rounding
+      // One copy of the code per activation, chosen once a tile: with the
+      // choice made per chunk, the unrolled code of all activations spread
+      // the executed part over more than the instruction cache (2048 values
+      // along k: 341 us a product against 280).
+      auto write_tile = [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
+        if (p.tma_out) {
+#pragma unroll
+          for (int h = 0; h < ROUNDS; h++) {
+            if (h) {
+              if (lane == 0) {
+                bulk_wait_read();
+                if (p.residual) load_residual(row_t, col_t, h);
+              }
+              __syncwarp();
+            }
+            if (p.residual) {
+              if (!mbar_wait(&res_full[e], res_phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL)) ok = false;
+              res_phase ^= 1;
+              res_flying = false;
+            }
+#pragma unroll
+            for (int j = 0; j < BOXES * 8; j++) {
+              const int at = h * BOXES * BOX_COLS + j * V;  // the chunk's first column
+              float v[V];
+#pragma unroll
+              for (int q = 0; q < V; q += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(sbias + at + q);
+                const float2 x = unpack_f32x2(acc[(at + q) / 2]), y = unpack_f32x2(acc[(at + q) / 2 + 1]);
+                v[q] = fp8_act<ACT>(x.x + b.x);
+                v[q + 1] = fp8_act<ACT>(x.y + b.y);
+                v[q + 2] = fp8_act<ACT>(y.x + b.z);
+                v[q + 3] = fp8_act<ACT>(y.y + b.w);
+              }
+              uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
+              if (p.residual) add_16<T>(v, *chunk);
+              *chunk = make_16<T>(v);
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+              for (int b = 0; b < BOXES; b++) {
+                const int col = col_t + (h * BOXES + b) * BOX_COLS;
+                if (col < p.n) tma_store_2d(&out_map, patch + b * 4096, col, row_t);
+              }
+              bulk_commit();
+            }
+          }
+        } else {
+          // 32 rows x 64 columns at a time through the patch, so that a
+          // warp's accesses are runs of a row wherever the rows start.
+          float* stg = reinterpret_cast<float*>(patch);
+          const int rows = min(32, p.m - row_t);
+#pragma unroll
+          for (int h = 0; h < CW / 64; h++) {
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 32; q++) {
+              const float2 pr = unpack_f32x2(acc[h * 32 + q]);
+              stg[lane * 64 + ((2 * q) ^ lane)] = pr.x;
+              stg[lane * 64 + ((2 * q + 1) ^ lane)] = pr.y;
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int g = 0; g < 2; g++) {
+              const int at = h * 64 + g * 32 + lane, col = col_t + at;
+              if (col >= p.n) break;
+              const float b = sbias[at];
+              const T* res = static_cast<const T*>(p.residual) + (long long)row_t * p.residual_stride + col;
+              T* out = static_cast<T*>(p.out) + (long long)row_t * p.out_stride + col;
+#pragma unroll 4
+              for (int r = 0; r < rows; r++) {
+                float v = fp8_act<ACT>(stg[r * 64 + ((g * 32 + lane) ^ r)] + b);
+                if (p.residual) v += to_f32(res[r * p.residual_stride]);
+                out[r * p.out_stride] = from_f32<T>(v);
+              }
+            }
+          }
+        }
+      };
+      switch (p.act) {
+        case OP_RELU: write_tile(std::integral_constant<int, OP_RELU>()); break;
+        case OP_GELU: write_tile(std::integral_constant<int, OP_GELU>()); break;
+        case OP_SIGMOID: write_tile(std::integral_constant<int, OP_SIGMOID>()); break;
+        case OP_SILU: write_tile(std::integral_constant<int, OP_SILU>()); break;
+        default: write_tile(std::integral_constant<int, OP_NONE>());
+      }
+      __syncwarp();  // sbias and the patch are read
+    }
+    if (lane == 0) {
+      bulk_wait();
+      // after an abort: a residual still on its way lands first
+      if (res_flying) mbar_wait(&res_full[e], res_phase, abort_flag, p.dev_err, 0);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, 2 * BN);
+  __syncwarp();
+  if (PAIR) cluster_sync();  // nothing of the other CTA is in flight to this one
+  if (warp == 1) {
+    if (PAIR)
+      tmem_dealloc_pair(tmem_base, 2 * BN);
+    else
+      tmem_dealloc(tmem_base, 2 * BN);
+  }
 }
 
 }  // namespace iec

@@ -1,6 +1,7 @@
 // Host side of the block-scaled e4m3 product (fp8_sm100.cuh): tile choice,
 // tensor maps and launches.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_sm100.cuh"
 
@@ -19,6 +20,27 @@ CUtensorMap code_map(const uint8_t* codes, long long stride, int rows, int k, in
   return map;
 }
 
+// out (or residual) as boxes of 32 rows x 128 bytes, 128-byte swizzled.
+template <class T>
+CUtensorMap value_map(const void* values, long long stride, int rows, int cols) {
+  CUtensorMap map;
+  const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
+  const uint64_t bytes = rows > 1 ? (uint64_t)stride * sizeof(T) : ((uint64_t)cols * sizeof(T) + 15) / 16 * 16;
+  const uint64_t strides[1] = {bytes};
+  const uint32_t box[2] = {128 / sizeof(T), 32};
+  const CUtensorMapDataType type = std::is_same<T, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  encode_tensor_map(&map, type, 2, values, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return map;
+}
+
+// The rows of a matrix start on 16 bytes, as tensor maps need.
+template <class T>
+bool on_16(const void* values, long long stride, int rows) {
+  return reinterpret_cast<uintptr_t>(values) % 16 == 0 && (rows == 1 || stride * (long long)sizeof(T) % 16 == 0);
+}
+
 template <auto Kernel>
 void allow_smem(Device& dev, int bytes) {
   static bool done[64] = {};
@@ -27,21 +49,74 @@ void allow_smem(Device& dev, int bytes) {
   d = true;
 }
 
-template <class T, int BN>
+// CTAs of `Kernel` in clusters of `cluster` that the device holds at once.
+template <auto Kernel>
+int resident(Device& dev, int threads, int smem, int cluster) {
+  static int found[64] = {};
+  int& f = found[dev.ordinal() & 63];
+  if (f == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(dev.sms() / cluster * cluster));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    IEC_CUDA(cudaOccupancyMaxActiveClusters(&clusters, Kernel, &cfg));
+    if (clusters < 1) throw Error(ERR_GPU, "no room for a cluster of CTAs");
+    f = std::min(clusters * cluster, dev.sms());
+  }
+  return f;
+}
+
+// launch_pdl in clusters of `cluster` CTAs along x.
+template <class... KArgs, class... Args>
+void launch_clusters(void (*kernel)(KArgs...), int grid, int threads, size_t smem, int cluster, cudaStream_t s,
+                     Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  IEC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+template <class T, int PAIR>
 void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s) {
-  using L = Fp8Smem<BN>;
-  constexpr auto kernel = fp8_gemm_sm100<T, BN>;
+  using L = Fp8Smem;
+  constexpr auto kernel = fp8_gemm_sm100<T, PAIR>;
+  constexpr int edge = PAIR ? 256 : 128, cluster = PAIR ? 2 : 1;
   allow_smem<kernel>(dev, L::DYN_BYTES);
-  CUtensorMap a_map = {}, w_map = {};
+  CUtensorMap a_map = {}, w_map = {}, out_map = {}, res_map = {};
   if (q.k) {
     a_map = code_map(q.a, q.a_stride, q.m, q.k, 128);
-    w_map = code_map(q.w, q.w_stride, q.n, q.k, BN);
+    w_map = code_map(q.w, q.w_stride, q.n, q.k, 64);
   }
-  p.tiles_m = (q.m + 127) / 128;
-  p.tiles_n = (q.n + BN - 1) / BN;
+  p.tma_out = on_16<T>(q.out, q.out_stride, q.m) && (!q.residual || on_16<T>(q.residual, q.residual_stride, q.m));
+  if (p.tma_out) {
+    out_map = value_map<T>(q.out, q.out_stride, q.m, q.n);
+    if (q.residual) res_map = value_map<T>(q.residual, q.residual_stride, q.m, q.n);
+  }
+  p.tiles_m = (q.m + edge - 1) / edge;
+  p.tiles_n = (q.n + edge - 1) / edge;
   if ((long long)p.tiles_m * p.tiles_n > INT32_MAX / 2) throw Error(ERR_INPUT, "product too large for one launch");
   p.tiles = p.tiles_m * p.tiles_n;
-  launch_pdl(kernel, dim3(std::min(p.tiles, dev.sms())), dim3(FP8_THREADS), (size_t)L::DYN_BYTES, s, a_map, w_map, p);
+  const int most = PAIR ? resident<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster) : dev.sms();
+  const int grid = std::min(p.tiles * cluster, most);
+  if (PAIR)
+    launch_clusters(kernel, grid, FP8_THREADS, (size_t)L::DYN_BYTES, cluster, s, a_map, w_map, out_map, res_map, p);
+  else
+    launch_pdl(kernel, dim3(grid), dim3(FP8_THREADS), (size_t)L::DYN_BYTES, s, a_map, w_map, out_map, res_map, p);
 }
 
 template <class T>
@@ -60,21 +135,17 @@ void run(Device& dev, const Fp8MatmulSpec& q, cudaStream_t s) {
   p.out = q.out;
   p.residual_stride = q.residual_stride;
   p.out_stride = q.out_stride;
-  auto rows_on_32 = [](const void* ptr, long long stride) {
-    return reinterpret_cast<uintptr_t>(ptr) % 32 == 0 && stride * (long long)sizeof(T) % 32 == 0;
-  };
-  p.wide = rows_on_32(q.out, q.out_stride) && (!q.residual || rows_on_32(q.residual, q.residual_stride));
   p.dev_err = dev.dev_err();
   const double m = q.m, n = q.n, k = q.k;
-  char name[96];
-  const long long wide = (long long)((q.m + 127) / 128) * ((q.n + 255) / 256);
-  const int bn = wide >= dev.sms() ? 256 : 128;
-  snprintf(name, sizeof name, "fp8_gemm_sm100<%d> %dx%dx%d", bn, q.m, q.n, q.k);
+  const long long pairs = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256);
+  const bool pair = pairs * 2 >= dev.sms();
+  char name[96] = "";
+  if (dev.timing()) snprintf(name, sizeof name, "fp8_gemm_sm100<%d> %dx%dx%d", pair ? 1 : 0, q.m, q.n, q.k);
   timed_launch(name, 2 * m * n * k, m * k + n * k + m * n * sizeof(T) * (q.residual ? 2 : 1), s, [&] {
-    if (bn == 256)
-      run_tiles<T, 256>(dev, q, p, s);
+    if (pair)
+      run_tiles<T, 1>(dev, q, p, s);
     else
-      run_tiles<T, 128>(dev, q, p, s);
+      run_tiles<T, 0>(dev, q, p, s);
   });
 }
 

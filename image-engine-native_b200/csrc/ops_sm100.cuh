@@ -29,12 +29,14 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 // reciprocal is the limit 0.
 __device__ __forceinline__ float op_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
+// The products that end an activation are not contracted with what is added
+// to them, so that every kernel and path rounds the same.
 template <int ACT>
 __device__ __forceinline__ float op_act(float v) {
   if (ACT == OP_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays
-  if (ACT == OP_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+  if (ACT == OP_GELU) return __fmul_rn(0.5f * v, 1.0f + erff(v * 0.70710678118654752f));
   if (ACT == OP_SIGMOID) return op_sigmoid(v);
-  if (ACT == OP_SILU) return v * op_sigmoid(v);
+  if (ACT == OP_SILU) return __fmul_rn(v, op_sigmoid(v));
   return v;
 }
 

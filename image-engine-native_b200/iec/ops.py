@@ -15,15 +15,22 @@ and the calls return without waiting. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+from struct import Struct
 
 import torch
 
-from . import IecError, ERR_INPUT, Options, _check, lib
+from . import ERR_INPUT, IecError, Options, _check, lib
 
 NONE, RELU, GELU, SIGMOID, SILU = range(5)
 BLOCK = 128  # values along a row that share a scale
 
+# The argument structs of iec_cuda.h, field by field.
+GROUP_NORM = Struct("@P6n3P2nPnPnfii0P")
+QUANTIZE = Struct("@P4nPnPni0P")
+MATMUL = Struct("@PnPnPnPnPPnP4nii0P")
+
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_F32, _FP8 = torch.float32, torch.float8_e4m3fn
 _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream has the handle 0
 
 
@@ -38,49 +45,67 @@ def _dtype(t, what: str) -> int:
     return code
 
 
-def _f32_vector(t, n: int, what: str):
+def _f32_vector(t, n: int, what: str) -> int:
+    """The address of n contiguous floats, 0 for None."""
     if t is None:
-        return None
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        return 0
+    if t.dtype is not _F32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         _bad(f"{what} must be {n} contiguous float32 values")
     return t.data_ptr()
 
 
-def _rows(t, rows: int, k: int, dtype, what: str) -> int:
-    """The row stride of a rows x k matrix whose rows are contiguous."""
-    if t.dtype is not dtype:
-        _bad(f"{what} is {t.dtype}, not {dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != k:
-        _bad(f"{what} is {tuple(t.shape)}, not {(rows, k)}")
-    if k > 1 and t.stride(1) != 1:
+def _rows(t, shape, dtype, what: str) -> int:
+    """The row stride of a matrix of `shape` whose rows are contiguous."""
+    if t.dtype is dtype and t.shape == shape:
+        step, one = t.stride()
+        if one == 1 or shape[1] <= 1:
+            return step if shape[0] > 1 else max(shape[1], 1)
         _bad(f"{what} must have contiguous rows")
-    return t.stride(0) if rows > 1 else max(k, 1)
+    _bad(f"{what} is {tuple(t.shape)} of {t.dtype}, not {tuple(shape)} of {dtype}")
 
 
 def _maps(t, what: str):
     """(maps, pixels, channels, pixel stride, map stride) of n x ... x c."""
-    if t.dim() < 2:
-        _bad(f"{what} must be maps x pixels (or height x width) x channels")
     shape, stride = t.shape, t.stride()
+    if len(shape) < 2:
+        _bad(f"{what} must be maps x pixels (or height x width) x channels")
     n, c = shape[0], shape[-1]
     if c > 1 and stride[-1] != 1:
         _bad(f"{what} must have contiguous channels")
-    pixels, step = 1, 0
-    for size, s in zip(shape[-2:0:-1], stride[-2:0:-1]):
+    pixels, step = 1, c
+    for at in range(len(shape) - 2, 0, -1):
+        size = shape[at]
         if size == 1:
             continue
-        if pixels > 1 and s != step * pixels:
-            _bad(f"{what} must have its pixels at one stride")
         if pixels == 1:
-            step = s
+            step = stride[at]
+        elif stride[at] != step * pixels:
+            _bad(f"{what} must have its pixels at one stride")
         pixels *= size
-    return n, pixels, c, step if pixels > 1 else c, stride[0] if n > 1 else c
+    return n, pixels, c, step, stride[0] if n > 1 else c
+
+
+def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device):
+    if codes is None:
+        codes = empty_codes(rows, k, device)
+    code_step = _rows(codes, (rows, k), _FP8, "codes")
+    blocks = -(-k // BLOCK)
+    if scales is None:
+        scales = torch.empty((blocks, scale_rows), dtype=_F32, device=device)
+    return codes, code_step, scales, _rows(scales, (blocks, scale_rows), _F32, "scales")
+
+
+def _stream(stream, device: int) -> int:
+    """`stream`, or torch's current one of the device."""
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(device)
+    return stream or _LEGACY_STREAM
 
 
 def empty_codes(rows: int, k: int, device):
     """Codes of a rows x k matrix as matmul_fp8 reads them: rows a multiple
     of 16 bytes apart."""
-    return torch.empty((rows, -(-max(k, 1) // 16) * 16), dtype=torch.float8_e4m3fn, device=device)[:, :k]
+    return torch.empty((rows, -(-max(k, 1) // 16) * 16), dtype=_FP8, device=device)[:, :k]
 
 
 class Ops:
@@ -88,24 +113,21 @@ class Ops:
 
     def __init__(self, device: int = -1, timeout_ms: int = 0):
         L = lib()
-        vp, sz, i32, f32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
-        norm = [vp, vp, i32, sz, sz, sz, sz, sz, sz, vp, vp, f32, i32]
+        vp = ctypes.c_void_p
         L.iec_ops_device_name.restype = ctypes.c_char_p
         L.iec_ops_device_name.argtypes = [vp]
         L.iec_ops_free.argtypes = [vp]
         L.iec_ops_sync.argtypes = [vp, vp]
-        L.iec_ops_group_norm.argtypes = norm + [vp, sz, sz, vp]
-        L.iec_ops_group_norm_fp8.argtypes = norm + [vp, sz, vp, sz, vp]
-        L.iec_ops_quantize_fp8.argtypes = [vp, vp, i32, sz, sz, sz, sz, vp, sz, vp, sz, vp]
-        L.iec_ops_matmul_fp8.argtypes = [vp, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, sz, sz, sz, i32, i32, vp, sz, vp]
-        self._h = ctypes.c_void_p()
+        for f in (L.iec_ops_group_norm, L.iec_ops_group_norm_fp8, L.iec_ops_quantize_fp8, L.iec_ops_matmul_fp8):
+            f.argtypes = [vp, ctypes.c_char_p, vp]
+        self._lib = L
+        self._h = vp()
         opt = Options(device, timeout_ms, 0)
         _check(L.iec_ops_open(ctypes.byref(opt), ctypes.byref(self._h)))
-        self._lib = L
 
     def close(self):
         if getattr(self, "_h", None):
-            lib().iec_ops_free(self._h)
+            self._lib.iec_ops_free(self._h)
             self._h = None
 
     __del__ = close
@@ -116,13 +138,7 @@ class Ops:
 
     def sync(self, stream=None):
         """Wait (bounded) for the stream's work and raise what went wrong."""
-        _check(self._lib.iec_ops_sync(self._h, self._stream(stream)))
-
-    @staticmethod
-    def _stream(stream, device=None):
-        if stream is None:
-            stream = torch.cuda.current_stream(device).cuda_stream
-        return stream or _LEGACY_STREAM
+        _check(self._lib.iec_ops_sync(self._h, _stream(stream, torch.cuda.current_device())))
 
     def group_norm(self, x, groups: int, gamma=None, beta=None, eps: float = 1e-5, act: int = NONE, out=None,
                    stream=None):
@@ -132,13 +148,15 @@ class Ops:
         n, pixels, c, step, map_step = _maps(x, "x")
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if out.dtype is not x.dtype or out.shape != x.shape:
+        elif out.dtype is not x.dtype or out.shape != x.shape:
             _bad("out must have the shape and type of x")
         _, _, _, out_step, out_map_step = _maps(out, "out")
-        _check(self._lib.iec_ops_group_norm(
-            self._h, x.data_ptr(), dtype, n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
-            _f32_vector(beta, c, "beta"), eps, act, out.data_ptr(), out_step, out_map_step,
-            self._stream(stream, x.device)))
+        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
+                               _f32_vector(beta, c, "beta"), out.data_ptr(), out_step, out_map_step, 0, 0, 0, 0, eps,
+                               dtype, act)
+        status = self._lib.iec_ops_group_norm(self._h, args, _stream(stream, x.get_device()))
+        if status:
+            _check(status)
         return out
 
     def group_norm_fp8(self, x, groups: int, gamma=None, beta=None, eps: float = 1e-5, act: int = NONE, codes=None,
@@ -147,11 +165,13 @@ class Ops:
         n*pixels x c, scales ceil(c / 128) x n*pixels)."""
         dtype = _dtype(x, "x")
         n, pixels, c, step, map_step = _maps(x, "x")
-        codes, code_step, scales, scale_step = self._fp8_out(codes, scales, n * pixels, c, n * pixels, x.device)
-        _check(self._lib.iec_ops_group_norm_fp8(
-            self._h, x.data_ptr(), dtype, n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
-            _f32_vector(beta, c, "beta"), eps, act, codes.data_ptr(), code_step, scales.data_ptr(), scale_step,
-            self._stream(stream, x.device)))
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, x.device)
+        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
+                               _f32_vector(beta, c, "beta"), 0, 0, 0, codes.data_ptr(), code_step, scales.data_ptr(),
+                               scale_step, eps, dtype, act)
+        status = self._lib.iec_ops_group_norm_fp8(self._h, args, _stream(stream, x.get_device()))
+        if status:
+            _check(status)
         return codes, scales
 
     def quantize_fp8(self, x, block_rows: int = 1, codes=None, scales=None, stream=None):
@@ -159,49 +179,44 @@ class Ops:
         ceil(k / 128) x rows), with block_rows 128 (weights) scales
         ceil(k / 128) x ceil(rows / 128)."""
         dtype = _dtype(x, "x")
-        if x.dim() != 2:
+        shape = x.shape
+        if len(shape) != 2:
             _bad("x must be rows x values")
-        rows, k = x.shape
-        step = _rows(x, rows, k, x.dtype, "x")
+        rows, k = shape
+        step = _rows(x, shape, x.dtype, "x")
         scale_rows = rows if block_rows != BLOCK else -(-rows // BLOCK)
-        codes, code_step, scales, scale_step = self._fp8_out(codes, scales, rows, k, scale_rows, x.device)
-        _check(self._lib.iec_ops_quantize_fp8(self._h, x.data_ptr(), dtype, rows, k, step, block_rows,
-                                              codes.data_ptr(), code_step, scales.data_ptr(), scale_step,
-                                              self._stream(stream, x.device)))
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, x.device)
+        args = QUANTIZE.pack(x.data_ptr(), rows, k, step, block_rows, codes.data_ptr(), code_step, scales.data_ptr(),
+                             scale_step, dtype)
+        status = self._lib.iec_ops_quantize_fp8(self._h, args, _stream(stream, x.get_device()))
+        if status:
+            _check(status)
         return codes, scales
-
-    @staticmethod
-    def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device):
-        if codes is None:
-            codes = empty_codes(rows, k, device)
-        code_step = _rows(codes, rows, k, torch.float8_e4m3fn, "codes")
-        blocks = -(-k // BLOCK)
-        if scales is None:
-            scales = torch.empty((blocks, scale_rows), dtype=torch.float32, device=device)
-        return codes, code_step, scales, _rows(scales, blocks, scale_rows, torch.float32, "scales")
 
     def matmul_fp8(self, a, a_scales, w, w_scales, bias=None, act: int = NONE, residual=None, out=None,
                    dtype=torch.float16, stream=None):
         """act(a w^T + bias) + residual for 8-bit rows a (m x k) and w (n x
         k, quantised with block_rows 128); `out` (default: a new tensor of
         `dtype`) may be `residual`."""
-        if a.dim() != 2 or w.dim() != 2:
+        a_shape, w_shape = a.shape, w.shape
+        if len(a_shape) != 2 or len(w_shape) != 2:
             _bad("a and w must be matrices")
-        m, k = a.shape
-        n = w.shape[0]
-        fp8, blocks = torch.float8_e4m3fn, -(-k // BLOCK)
-        a_step, w_step = _rows(a, m, k, fp8, "a"), _rows(w, n, k, fp8, "w")
-        a_scale_step = _rows(a_scales, blocks, m, torch.float32, "a_scales")
-        w_scale_step = _rows(w_scales, blocks, -(-n // BLOCK), torch.float32, "w_scales")
+        m, k = a_shape
+        n = w_shape[0]
+        blocks = -(-k // BLOCK)
         if out is None:
             out = torch.empty((m, n), dtype=dtype, device=a.device)
         code = _dtype(out, "out")
-        out_step = _rows(out, m, n, out.dtype, "out")
-        res, res_step = None, 0
+        res, res_step = 0, 0
         if residual is not None:
-            res, res_step = residual.data_ptr(), _rows(residual, m, n, out.dtype, "residual")
-        _check(self._lib.iec_ops_matmul_fp8(
-            self._h, a.data_ptr(), a_step, a_scales.data_ptr(), a_scale_step, w.data_ptr(), w_step,
-            w_scales.data_ptr(), w_scale_step, _f32_vector(bias, n, "bias"), res, res_step, m, n, k, act, code,
-            out.data_ptr(), out_step, self._stream(stream, a.device)))
+            res, res_step = residual.data_ptr(), _rows(residual, (m, n), out.dtype, "residual")
+        args = MATMUL.pack(a.data_ptr(), _rows(a, a_shape, _FP8, "a"),
+                           a_scales.data_ptr(), _rows(a_scales, (blocks, m), _F32, "a_scales"),
+                           w.data_ptr(), _rows(w, (n, k), _FP8, "w"),
+                           w_scales.data_ptr(), _rows(w_scales, (blocks, -(-n // BLOCK)), _F32, "w_scales"),
+                           _f32_vector(bias, n, "bias"), res, res_step,
+                           out.data_ptr(), _rows(out, (m, n), out.dtype, "out"), m, n, k, act, code)
+        status = self._lib.iec_ops_matmul_fp8(self._h, args, _stream(stream, a.get_device()))
+        if status:
+            _check(status)
         return out

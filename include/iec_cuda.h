@@ -360,19 +360,29 @@ iec_status iec_ops_sync(iec_ops* ops, void* stream);
  *   out = act((x - mean) / sqrt(variance + eps) * gamma[channel] + beta[channel]),
  * the variance without Bessel's correction; `gamma`, `beta` (c floats) may
  * be NULL (1 and 0). Sums are f32; the result is rounded once to `dtype`,
- * the type of `x` and `out`. `out` may be `x` itself with its strides. */
-iec_status iec_ops_group_norm(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
-                              size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
-                              const float* beta, float eps, int act, void* out, size_t out_stride,
-                              size_t out_map_stride, void* stream);
+ * the type of `x` and `out`. `out` may be `x` itself with its strides. The
+ * fields codes .. scale_stride are not read. */
+typedef struct iec_group_norm_args {
+  const void* x;
+  size_t n, pixels, c, x_stride, x_map_stride, groups;
+  const float* gamma;
+  const float* beta;
+  void* out;
+  size_t out_stride, out_map_stride;
+  uint8_t* codes;
+  size_t code_stride;
+  float* scales;
+  size_t scale_stride;
+  float eps;
+  int dtype, act;
+} iec_group_norm_args;
+iec_status iec_ops_group_norm(iec_ops* ops, const iec_group_norm_args* args, void* stream);
 
 /* iec_ops_group_norm with its result, in f32, stored as 8-bit rows of c
- * values (block_rows 1), one per pixel, map after map: what
- * iec_ops_matmul_fp8 takes as `a`. */
-iec_status iec_ops_group_norm_fp8(iec_ops* ops, const void* x, int dtype, size_t n, size_t pixels, size_t c,
-                                  size_t x_stride, size_t x_map_stride, size_t groups, const float* gamma,
-                                  const float* beta, float eps, int act, uint8_t* codes, size_t code_stride,
-                                  float* scales, size_t scale_stride, void* stream);
+ * values (block_rows 1) at `codes` and `scales`, one per pixel, map after
+ * map: what iec_ops_matmul_fp8 takes as `a`. The fields out ..
+ * out_map_stride are not read. */
+iec_status iec_ops_group_norm_fp8(iec_ops* ops, const iec_group_norm_args* args, void* stream);
 
 /* `rows` x `k` values of `dtype` as 8-bit rows: over each block (of
  * `block_rows` 1 or 128 rows and 128 values along k, fewer at the edges)
@@ -380,9 +390,16 @@ iec_status iec_ops_group_norm_fp8(iec_ops* ops, const void* x, int dtype, size_t
  * rounded to nearest even. A block whose amax is below 2^-100 gets scale 1
  * and zero codes. A NaN or an infinity in a block makes its scale NaN or
  * infinite, and all its values read back as NaN. */
-iec_status iec_ops_quantize_fp8(iec_ops* ops, const void* x, int dtype, size_t rows, size_t k, size_t x_stride,
-                                size_t block_rows, uint8_t* codes, size_t code_stride, float* scales,
-                                size_t scale_stride, void* stream);
+typedef struct iec_quantize_fp8_args {
+  const void* x;
+  size_t rows, k, x_stride, block_rows;
+  uint8_t* codes;
+  size_t code_stride;
+  float* scales;
+  size_t scale_stride;
+  int dtype;
+} iec_quantize_fp8_args;
+iec_status iec_ops_quantize_fp8(iec_ops* ops, const iec_quantize_fp8_args* args, void* stream);
 
 /* out (m x n of `dtype`) = act(a w^T + bias) + residual for 8-bit rows `a`
  * (m x k, block_rows 1) and `w` (n x k, block_rows 128): a linear layer, or
@@ -391,11 +408,23 @@ iec_status iec_ops_quantize_fp8(iec_ops* ops, const void* x, int dtype, size_t r
  * the result is rounded once. `bias` (n floats) and `residual` (m x n of
  * `dtype`, may be `out` itself with its stride) may be NULL. `a` and `w`
  * must start on 16 bytes, with strides a multiple of 16. */
-iec_status iec_ops_matmul_fp8(iec_ops* ops, const uint8_t* a, size_t a_stride, const float* a_scales,
-                              size_t a_scale_stride, const uint8_t* w, size_t w_stride, const float* w_scales,
-                              size_t w_scale_stride, const float* bias, const void* residual,
-                              size_t residual_stride, size_t m, size_t n, size_t k, int act, int dtype, void* out,
-                              size_t out_stride, void* stream);
+typedef struct iec_matmul_fp8_args {
+  const uint8_t* a;
+  size_t a_stride;
+  const float* a_scales;
+  size_t a_scale_stride;
+  const uint8_t* w;
+  size_t w_stride;
+  const float* w_scales;
+  size_t w_scale_stride;
+  const float* bias;
+  const void* residual;
+  size_t residual_stride;
+  void* out;
+  size_t out_stride, m, n, k;
+  int act, dtype;
+} iec_matmul_fp8_args;
+iec_status iec_ops_matmul_fp8(iec_ops* ops, const iec_matmul_fp8_args* args, void* stream);
 
 /* Launch timing (measurement hooks, no counterpart in the reference).
  * iec_set_launch_timing(model, 1) on any model handle (SCUNet, LaMa,

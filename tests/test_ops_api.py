@@ -50,6 +50,6 @@ def test_tensor_views():
             ops._maps(bad, "t")
     codes = ops.empty_codes(3, 50, "cpu")
     assert codes.shape == (3, 50) and codes.stride(0) == 64
-    assert ops._rows(codes, 3, 50, torch.float8_e4m3fn, "codes") == 64
+    assert ops._rows(codes, (3, 50), torch.float8_e4m3fn, "codes") == 64
     with pytest.raises(iec.IecError):
-        ops._rows(codes.t(), 50, 3, torch.float8_e4m3fn, "codes")
+        ops._rows(codes.t(), (50, 3), torch.float8_e4m3fn, "codes")

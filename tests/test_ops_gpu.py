@@ -451,11 +451,17 @@ def test_refusals(ops):
     refused(lambda: ops.matmul_fp8(a, sa, w, sw, dtype=torch.float64), "float64")
     L = iec.lib()
     f = np.zeros(1, np.float32).ctypes.data
-    assert L.iec_ops_quantize_fp8(ops._h, x.data_ptr() + 1, 0, 2, 16, 16, 1, f, 16, f, 2, None) == iec.ERR_INPUT
+
+    def raw(x=x.data_ptr(), rows=2, step=16, dtype=0):
+        args = iec.ops.QUANTIZE.pack(x or 0, rows, 16, step, 1, f, 16, f, 2, dtype)
+        return L.iec_ops_quantize_fp8(ops._h, args, None)
+
+    assert raw(x=x.data_ptr() + 1) == iec.ERR_INPUT
     assert b"aligned" in L.iec_last_error()
-    assert L.iec_ops_quantize_fp8(ops._h, x.data_ptr(), 7, 2, 16, 16, 1, f, 16, f, 2, None) == iec.ERR_INPUT
-    assert L.iec_ops_quantize_fp8(ops._h, x.data_ptr(), 0, 2, 16, 15, 1, f, 16, f, 2, None) == iec.ERR_INPUT
-    assert L.iec_ops_quantize_fp8(ops._h, None, 0, 2, 16, 16, 1, f, 16, f, 2, None) == iec.ERR_INPUT
-    assert L.iec_ops_quantize_fp8(ops._h, x.data_ptr(), 0, 1 << 40, 16, 16, 1, f, 16, f, 2, None) == iec.ERR_INPUT
+    assert raw(dtype=7) == iec.ERR_INPUT
+    assert raw(step=15) == iec.ERR_INPUT
+    assert raw(x=None) == iec.ERR_INPUT
+    assert raw(rows=1 << 40) == iec.ERR_INPUT
+    assert L.iec_ops_quantize_fp8(ops._h, None, None) == iec.ERR_INPUT
     # the handle works on after a refusal
     assert torch.isfinite(ops.group_norm(x, 4)).all()
