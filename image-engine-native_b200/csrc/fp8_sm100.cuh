@@ -34,6 +34,7 @@ namespace iec {
 struct Fp8Params {
   int m, n, kblocks, act;
   int tiles_m, tiles_n, tiles;
+  FastDiv div_group, div_rest;  // by the tiles of a group of M tiles, and by the M tiles of the last one
   const float* a_scales;
   const float* w_scales;
   long long a_scale_stride, w_scale_stride;
@@ -55,23 +56,30 @@ struct Fp8Smem {
   static constexpr int OUT_OFF = NSTAGE * STAGE, OUT_WARP = 8192;  // a warp's patch of the output
   static constexpr int BIAS_OFF = OUT_OFF + FP8_EPI_WARPS * OUT_WARP;
   static constexpr int BAR_OFF = BIAS_OFF + FP8_EPI_WARPS * 128 * 4;
-  static constexpr int MISC_OFF = BAR_OFF + (2 * NSTAGE + 8 + FP8_EPI_WARPS) * 8;
+  static constexpr int MISC_OFF = BAR_OFF + (2 * NSTAGE + 4 + FP8_EPI_WARPS) * 8;
   static constexpr int DYN_BYTES = MISC_OFF + 16 + 1024;
   static_assert(DYN_BYTES <= 232448, "shared memory of a CTA");
 };
 
 // Tile -> (M tile, N tile), in groups of FP8_GROUP M tiles.
 __device__ __forceinline__ void fp8_tile(const Fp8Params& p, int tile, int* mt, int* nt) {
-  const int per = FP8_GROUP * p.tiles_n, g = tile / per, r = tile - g * per;
-  const int rows = min(FP8_GROUP, p.tiles_m - g * FP8_GROUP);
-  *nt = r / rows;
+  const int g = (int)p.div_group.div((uint32_t)tile), r = tile - g * FP8_GROUP * p.tiles_n;
+  const bool last = (g + 1) * FP8_GROUP > p.tiles_m;
+  const int rows = last ? p.tiles_m - g * FP8_GROUP : FP8_GROUP;
+  *nt = last ? (int)p.div_rest.div((uint32_t)r) : r / FP8_GROUP;
   *mt = g * FP8_GROUP + r - *nt * rows;
 }
 
+// Two values rounded to T in one instruction (single conversions go through
+// a unit with an eighth of the rate).
 template <class T>
 __device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
-  const T a = from_f32<T>(lo), b = from_f32<T>(hi);
-  return (uint32_t) reinterpret_cast<const uint16_t&>(a) | (uint32_t) reinterpret_cast<const uint16_t&>(b) << 16;
+  uint32_t v;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
 }
 
 // 16 bytes of T: add to f32, or make from f32.
@@ -114,9 +122,15 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-#ifndef FP8_NPART
-#define FP8_NPART 1
-#endif
+// `BOXES` boxes of 4 KB next to each other in a row. (Out of line: inlined
+// where it is used, it took registers from the sums.)
+template <int BOXES, int BOX_COLS>
+__device__ __noinline__ void fp8_load_boxes(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row) {
+  mbar_arrive_expect_tx(bar, BOXES * 4096);
+#pragma unroll
+  for (int b = 0; b < BOXES; b++) tma_load_2d(dst + b * 4096, map, bar, col + b * BOX_COLS, row);
+}
+
 template <class T, int PAIR>
 __global__ void __launch_bounds__(FP8_THREADS, 1)
     fp8_gemm_sm100(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap w_map,
@@ -124,14 +138,13 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
                    const Fp8Params p) {
   using L = Fp8Smem;
   constexpr int BM = PAIR ? 256 : 128, BN = BM, CW = BN / 2;  // CW: columns of a thread
-  constexpr int NPART = FP8_NPART;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // of a pair, only the first CTA's is used
   uint64_t* empty = full + L::NSTAGE;
-  uint64_t* acc_full = empty + L::NSTAGE;  // [part][accumulator]
-  uint64_t* acc_empty = acc_full + 4;      // of a pair, only the first CTA's is used
-  uint64_t* res_full = acc_empty + 4;
+  uint64_t* acc_full = empty + L::NSTAGE;
+  uint64_t* acc_empty = acc_full + 2;  // of a pair, only the first CTA's is used
+  uint64_t* res_full = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -143,9 +156,9 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < 4; a++) {
+    for (int a = 0; a < 2; a++) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], FP8_EPI_WARPS / NPART * (PAIR ? 2 : 1));
+      mbar_init(&acc_empty[a], FP8_EPI_WARPS * (PAIR ? 2 : 1));
     }
     for (int w = 0; w < FP8_EPI_WARPS; w++) mbar_init(&res_full[w], 1);
     *abort_flag = 0;
@@ -178,7 +191,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       for (int tile = first; tile < p.tiles && ok; tile += step) {
         int mt, nt;
         fp8_tile(p, tile, &mt, &nt);
-        const int row = mt * BM + (int)rank * 128, col = nt * BN + (int)rank * (BN / NPART / 2);
+        const int row = mt * BM + (int)rank * 128, col = nt * BN + (int)rank * 128;
         for (int kb = 0; kb < p.kblocks; kb++) {
           if (!mbar_wait(&empty[s], phase ^ 1, abort_flag, p.dev_err, DEV_ERR_WAIT_EMPTY)) {
             ok = false;
@@ -190,14 +203,11 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
             const uint32_t bar = cluster_map(&full[s], 0);
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
             tma_load_2d_pair(st, &a_map, bar, kb * FP8_BLOCK, row);
-            // half of the rows of w of each part
             tma_load_2d_pair(st + L::HALF_BYTES, &w_map, bar, kb * FP8_BLOCK, col);
-            tma_load_2d_pair(st + L::HALF_BYTES + L::HALF_BYTES / 2, &w_map, bar, kb * FP8_BLOCK, NPART == 2 ? col + CW : col + 64);
           } else {
             mbar_arrive_expect_tx(&full[s], L::STAGE);
             tma_load_2d(st, &a_map, &full[s], kb * FP8_BLOCK, row);
             tma_load_2d(st + L::HALF_BYTES, &w_map, &full[s], kb * FP8_BLOCK, col);
-            tma_load_2d(st + L::HALF_BYTES + L::HALF_BYTES / 2, &w_map, &full[s], kb * FP8_BLOCK, col + 64);
           }
           issued++;
           if (++s == L::NSTAGE) {
@@ -212,7 +222,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       // (the whole warp walks the loop, one lane issues: see elect_one)
-      constexpr uint32_t idesc = idesc_e4m3_f32(BM, BN / NPART);
+      constexpr uint32_t idesc = idesc_e4m3_f32(BM, BN);
       const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
       int s = 0, i = 0;
       uint32_t phase = 0;
@@ -221,37 +231,29 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         for (int kb = 0; kb < p.kblocks; kb++, i++) {
           ok = __all_sync(~0u, mbar_wait(&full[s], phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL));
           if (!ok) break;
-          const uint64_t adesc = desc0 + (uint32_t)(s * (L::STAGE >> 4));
+          const int a = i & 1;
+          ok = __all_sync(~0u, mbar_wait(&acc_empty[a], ((uint32_t)(i >> 1) & 1) ^ 1, abort_flag, p.dev_err,
+                                         DEV_ERR_WAIT_ACC_EMPTY));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t adesc = desc0 + (uint32_t)(s * (L::STAGE >> 4)), bdesc = adesc + (L::HALF_BYTES >> 4);
+          const uint32_t d = tmem_base + (uint32_t)(a * BN);
+          if (elect_one()) {
 #pragma unroll
-          for (int part = 0; part < NPART; part++) {
-            const int a = part * 2 + (i & 1);
-            ok = __all_sync(~0u, mbar_wait(&acc_empty[a], ((uint32_t)(i >> 1) & 1) ^ 1, abort_flag, p.dev_err,
-                                           DEV_ERR_WAIT_ACC_EMPTY));
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t bdesc = adesc + (uint32_t)((L::HALF_BYTES + part * (L::HALF_BYTES / 2)) >> 4);
-            const uint32_t d = tmem_base + (uint32_t)(a * (BN / NPART));
-            if (elect_one()) {
-#pragma unroll
-              for (int j = 0; j < 4; j++) {
-                if (PAIR)
-                  umma_f8_pair(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
-                else
-                  umma_f8(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
-              }
+            for (int j = 0; j < 4; j++) {
               if (PAIR)
-                umma_commit_pair(&acc_full[a]);
+                umma_f8_pair(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
               else
-                umma_commit(&acc_full[a]);
-              if (part == NPART - 1) {
-                if (PAIR)
-                  umma_commit_pair(&empty[s]);
-                else
-                  umma_commit(&empty[s]);
-              }
+                umma_f8(d, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0);
+            }
+            if (PAIR) {
+              umma_commit_pair(&empty[s]);
+              umma_commit_pair(&acc_full[a]);
+            } else {
+              umma_commit(&empty[s]);
+              umma_commit(&acc_full[a]);
             }
           }
-          if (!ok) break;
           if (++s == L::NSTAGE) {
             s = 0;
             phase ^= 1;
@@ -259,8 +261,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         }
       // the MMAs in flight end before TMEM is freed
       for (int q = max(0, i - 2); q < i; q++)
-        for (int part = 0; part < NPART; part++)
-          mbar_wait(&acc_full[part * 2 + (q & 1)], (uint32_t)(q >> 1) & 1, abort_flag, p.dev_err, 0);
+        mbar_wait(&acc_full[q & 1], (uint32_t)(q >> 1) & 1, abort_flag, p.dev_err, 0);
     }
   } else {
     // ------------------------------------------- scaling, sums and epilogue
@@ -272,27 +273,23 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
     const int e = warp - 4, quarter = warp & 3, part = e >> 2;
     uint8_t* patch = smem + L::OUT_OFF + e * L::OUT_WARP;
     float* sbias = reinterpret_cast<float*>(smem + L::BIAS_OFF) + e * 128;
-    const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(NPART == 2 ? part * 2 * CW : part * CW);
-    uint64_t* const part_full = acc_full + (NPART == 2 ? part * 2 : 0);
-    uint64_t* const part_empty = acc_empty + (NPART == 2 ? part * 2 : 0);
-    const uint32_t acc_bar = PAIR ? cluster_map(part_empty, 0) : 0;
+    const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * CW);
+    const uint32_t acc_bar = PAIR ? cluster_map(acc_empty, 0) : 0;
     int i = 0;
     uint32_t res_phase = 0;
     bool ok = true, res_flying = false;
 
     // Round `r` of a tile's residual into the patch (lane 0; the patch free).
-    auto load_residual = [&](int row, int col, int r) __attribute__((noinline)) {
+    auto load_residual = [&](int row, int col, int r) {
       res_flying = true;
-      mbar_arrive_expect_tx(&res_full[e], BOXES * 4096);
-      for (int b = 0; b < BOXES; b++)
-        tma_load_2d(patch + b * 4096, &res_map, &res_full[e], col + (r * BOXES + b) * BOX_COLS, row);
+      fp8_load_boxes<BOXES, BOX_COLS>(patch, &res_map, &res_full[e], col + r * BOXES * BOX_COLS, row);
     };
 
-    // A tile's first row and column of this warp, and its first scales.
+    // A tile's first row and column of this warp, its first scales and bias.
     int row0 = 0, col0 = 0;
     const float* sa = p.a_scales;
     const float* sw = p.w_scales;
-    float sa_next = 0.0f, sw_next = 0.0f;
+    float sa_next = 0.0f, sw_next = 0.0f, bias_r[CW / 32];
     auto enter_tile = [&](int tile) {
       int mt, nt;
       fp8_tile(p, tile, &mt, &nt);
@@ -304,18 +301,20 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         sa_next = *sa;
         sw_next = *sw;
       }
+#pragma unroll
+      for (int c = 0; c < CW / 32; c++) {
+        const int col = col0 + c * 32 + lane;
+        bias_r[c] = p.bias && col < p.n ? p.bias[col] : 0.0f;
+      }
     };
     if (first < p.tiles) enter_tile(first);
 
     for (int tile = first; tile < p.tiles && ok; tile += step) {
       const int row_t = row0, col_t = col0;
       const bool any = row_t < p.m && col_t < p.n;
-      float bias_r[CW / 32];
+      __syncwarp();
 #pragma unroll
-      for (int c = 0; c < CW / 32; c++) {
-        const int col = col_t + c * 32 + lane;
-        bias_r[c] = p.bias && col < p.n ? p.bias[col] : 0.0f;
-      }
+      for (int c = 0; c < CW / 32; c++) sbias[c * 32 + lane] = bias_r[c];
       uint64_t acc[CW / 2];  // f32 pairs
 #pragma unroll
       for (int c = 0; c < CW / 2; c++) acc[c] = 0;
@@ -329,18 +328,18 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
           sw_next = *sw;
         }
         const int a = i & 1;
-        if (!mbar_wait(&part_full[a], (uint32_t)(i >> 1) & 1, abort_flag, p.dev_err, DEV_ERR_WAIT_ACC_FULL)) ok = false;
+        if (!mbar_wait(&acc_full[a], (uint32_t)(i >> 1) & 1, abort_flag, p.dev_err, DEV_ERR_WAIT_ACC_FULL)) ok = false;
         if (__any_sync(~0u, !ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t t = lanes + (uint32_t)(a * (BN / NPART));
+        const uint32_t t = lanes + (uint32_t)(a * BN);
         uint32_t r[2][16];
         tmem_ld16(t, r[0]);
 #pragma unroll
         for (int c = 0; c < CW / 16; c++) {
-          tmem_wait_ld16(r[c & 1]);
+          tmem_wait_ld();
           if (c + 1 < CW / 16) {
             tmem_ld16(t + (uint32_t)(16 * (c + 1)), r[(c + 1) & 1]);
           } else {
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               if (PAIR)
                 mbar_arrive_cluster(acc_bar + (uint32_t)(a * 8));
               else
-                mbar_arrive(&part_empty[a]);
+                mbar_arrive(&acc_empty[a]);
             }
           }
 #pragma unroll
@@ -363,33 +362,33 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         }
       }
       if (!ok) break;
-      if (tile + step < p.tiles) enter_tile(tile + step);  // its first scales are on their way
+      if (tile + step < p.tiles) enter_tile(tile + step);  // its first scales and bias are on their way
       if (!any) continue;
       if (lane == 0) {
         bulk_wait_read();  // the last tile has left the patch
         if (p.kblocks == 0 && p.tma_out && p.residual) load_residual(row_t, col_t, 0);
       }
-#pragma unroll
-      for (int c = 0; c < CW / 32; c++) sbias[c * 32 + lane] = bias_r[c];
       __syncwarp();
       // ---- bias, activation, residual, rounding
-      // One copy of the code per activation, chosen once a tile: with the
-      // choice made per chunk, the unrolled code of all activations spread
-      // the executed part over more than the instruction cache (2048 values
-      // along k: 341 us a product against 280).
-      auto write_tile = [&](auto act_c) {
+      // One copy of the code per activation, with and without a residual,
+      // chosen once a tile: with the choices made per chunk, the unrolled
+      // code of all of them put the executed part out of the instruction
+      // cache's reach and kept chunks from overlapping (a 128-column row
+      // took 9,000 cycles, against 1,500).
+      auto write_tile = [&](auto act_c, auto res_c) {
         constexpr int ACT = decltype(act_c)::value;
+        constexpr bool RES = decltype(res_c)::value;
         if (p.tma_out) {
 #pragma unroll
           for (int h = 0; h < ROUNDS; h++) {
             if (h) {
               if (lane == 0) {
                 bulk_wait_read();
-                if (p.residual) load_residual(row_t, col_t, h);
+                if (RES) load_residual(row_t, col_t, h);
               }
               __syncwarp();
             }
-            if (p.residual) {
+            if (RES) {
               if (!mbar_wait(&res_full[e], res_phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL)) ok = false;
               res_phase ^= 1;
               res_flying = false;
@@ -400,15 +399,16 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               float v[V];
 #pragma unroll
               for (int q = 0; q < V; q += 4) {
-                const float4 b = *reinterpret_cast<const float4*>(sbias + at + q);
-                const float2 x = unpack_f32x2(acc[(at + q) / 2]), y = unpack_f32x2(acc[(at + q) / 2 + 1]);
-                v[q] = fp8_act<ACT>(x.x + b.x);
-                v[q + 1] = fp8_act<ACT>(x.y + b.y);
-                v[q + 2] = fp8_act<ACT>(y.x + b.z);
-                v[q + 3] = fp8_act<ACT>(y.y + b.w);
+                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sbias + at + q);
+                const float2 x = unpack_f32x2(fadd2_pair(acc[(at + q) / 2], b.x));
+                const float2 y = unpack_f32x2(fadd2_pair(acc[(at + q) / 2 + 1], b.y));
+                v[q] = fp8_act<ACT>(x.x);
+                v[q + 1] = fp8_act<ACT>(x.y);
+                v[q + 2] = fp8_act<ACT>(y.x);
+                v[q + 3] = fp8_act<ACT>(y.y);
               }
               uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
-              if (p.residual) add_16<T>(v, *chunk);
+              if (RES) add_16<T>(v, *chunk);
               *chunk = make_16<T>(v);
             }
             fence_proxy_async_shared();
@@ -447,21 +447,27 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
 #pragma unroll 4
               for (int r = 0; r < rows; r++) {
                 float v = fp8_act<ACT>(stg[r * 64 + ((g * 32 + lane) ^ r)] + b);
-                if (p.residual) v += to_f32(res[r * p.residual_stride]);
+                if (RES) v += to_f32(res[r * p.residual_stride]);
                 out[r * p.out_stride] = from_f32<T>(v);
               }
             }
           }
         }
       };
+      auto write_act = [&](auto act_c) {
+        if (p.residual)
+          write_tile(act_c, std::true_type());
+        else
+          write_tile(act_c, std::false_type());
+      };
       switch (p.act) {
-        case OP_RELU: write_tile(std::integral_constant<int, OP_RELU>()); break;
-        case OP_GELU: write_tile(std::integral_constant<int, OP_GELU>()); break;
-        case OP_SIGMOID: write_tile(std::integral_constant<int, OP_SIGMOID>()); break;
-        case OP_SILU: write_tile(std::integral_constant<int, OP_SILU>()); break;
-        default: write_tile(std::integral_constant<int, OP_NONE>());
+        case OP_RELU: write_act(std::integral_constant<int, OP_RELU>()); break;
+        case OP_GELU: write_act(std::integral_constant<int, OP_GELU>()); break;
+        case OP_SIGMOID: write_act(std::integral_constant<int, OP_SIGMOID>()); break;
+        case OP_SILU: write_act(std::integral_constant<int, OP_SILU>()); break;
+        default: write_act(std::integral_constant<int, OP_NONE>());
       }
-      __syncwarp();  // sbias and the patch are read
+      __syncwarp();  // the patch is read
     }
     if (lane == 0) {
       bulk_wait();

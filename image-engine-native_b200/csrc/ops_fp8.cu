@@ -100,7 +100,7 @@ void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s)
   CUtensorMap a_map = {}, w_map = {}, out_map = {}, res_map = {};
   if (q.k) {
     a_map = code_map(q.a, q.a_stride, q.m, q.k, 128);
-    w_map = code_map(q.w, q.w_stride, q.n, q.k, 64);
+    w_map = code_map(q.w, q.w_stride, q.n, q.k, 128);
   }
   p.tma_out = on_16<T>(q.out, q.out_stride, q.m) && (!q.residual || on_16<T>(q.residual, q.residual_stride, q.m));
   if (p.tma_out) {
@@ -109,8 +109,11 @@ void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s)
   }
   p.tiles_m = (q.m + edge - 1) / edge;
   p.tiles_n = (q.n + edge - 1) / edge;
-  if ((long long)p.tiles_m * p.tiles_n > INT32_MAX / 2) throw Error(ERR_INPUT, "product too large for one launch");
+  if ((long long)p.tiles_m * p.tiles_n >= 1 << 24 || FP8_GROUP * p.tiles_n >= 1 << 16)
+    throw Error(ERR_INPUT, "product too large for one launch");
   p.tiles = p.tiles_m * p.tiles_n;
+  p.div_group = FastDiv((uint32_t)(FP8_GROUP * p.tiles_n));
+  p.div_rest = FastDiv((uint32_t)std::max(1, p.tiles_m % FP8_GROUP));
   const int most = PAIR ? resident<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster) : dev.sms();
   const int grid = std::min(p.tiles * cluster, most);
   if (PAIR)
