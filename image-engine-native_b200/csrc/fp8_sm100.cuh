@@ -23,9 +23,6 @@
 // written through shared memory with plain accesses. All waits are bounded.
 #pragma once
 
-#include <type_traits>
-
-#include "igemm_sm100.cuh"
 #include "ops_sm100.cuh"
 #include "sm100.cuh"
 
@@ -70,18 +67,6 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, int tile, int* mt, 
   *mt = g * FP8_GROUP + r - *nt * rows;
 }
 
-// Two values rounded to T in one instruction (single conversions go through
-// a unit with an eighth of the rate).
-template <class T>
-__device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
-  uint32_t v;
-  if constexpr (std::is_same<T, __half>::value)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
-  return v;
-}
-
 // 16 bytes of T: add to f32, or make from f32.
 template <class T>
 __device__ __forceinline__ void add_16(float* f, uint4 v) {
@@ -103,14 +88,6 @@ __device__ __forceinline__ uint4 make_16(const float* f) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   else
     return make_uint4(pack_2<T>(f[0], f[1]), pack_2<T>(f[2], f[3]), pack_2<T>(f[4], f[5]), pack_2<T>(f[6], f[7]));
-}
-
-// The activation in an unrolled epilogue: op_act, but GELU by the form of
-// igemm_sm100.cuh, a third of erff's instructions (|error| <= 1.5e-7 |v|).
-template <int ACT>
-__device__ __forceinline__ float fp8_act(float v) {
-  if (ACT == OP_GELU) return gemm_gelu(v);
-  return op_act<ACT>(v);
 }
 
 template <int REGS>
@@ -174,7 +151,6 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
-  __syncwarp();
   if (PAIR) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
@@ -402,11 +378,12 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
                 const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sbias + at + q);
                 const float2 x = unpack_f32x2(fadd2_pair(acc[(at + q) / 2], b.x));
                 const float2 y = unpack_f32x2(fadd2_pair(acc[(at + q) / 2 + 1], b.y));
-                v[q] = fp8_act<ACT>(x.x);
-                v[q + 1] = fp8_act<ACT>(x.y);
-                v[q + 2] = fp8_act<ACT>(y.x);
-                v[q + 3] = fp8_act<ACT>(y.y);
+                v[q] = x.x;
+                v[q + 1] = x.y;
+                v[q + 2] = y.x;
+                v[q + 3] = y.y;
               }
+              op_act_vec<ACT, true, V>(v);
               uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
               if (RES) add_16<T>(v, *chunk);
               *chunk = make_16<T>(v);
@@ -437,36 +414,34 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               stg[lane * 64 + ((2 * q + 1) ^ lane)] = pr.y;
             }
             __syncwarp();
-#pragma unroll 1
-            for (int g = 0; g < 2; g++) {
-              const int at = h * 64 + g * 32 + lane, col = col_t + at;
-              if (col >= p.n) break;
-              const float b = sbias[at];
+            // two columns a lane: the pairs whose activations go together
+            const int at = h * 64 + 2 * lane, col = col_t + at;
+            if (col < p.n) {
+              const float2 b = *reinterpret_cast<const float2*>(sbias + at);
               const T* res = static_cast<const T*>(p.residual) + (long long)row_t * p.residual_stride + col;
               T* out = static_cast<T*>(p.out) + (long long)row_t * p.out_stride + col;
-#pragma unroll 4
+              const bool two = col + 1 < p.n;
+#pragma unroll 1
               for (int r = 0; r < rows; r++) {
-                float v = fp8_act<ACT>(stg[r * 64 + ((g * 32 + lane) ^ r)] + b);
-                if (RES) v += to_f32(res[r * p.residual_stride]);
-                out[r * p.out_stride] = from_f32<T>(v);
+                float v[2] = {stg[r * 64 + ((2 * lane) ^ r)] + b.x, stg[r * 64 + ((2 * lane + 1) ^ r)] + b.y};
+                op_act_vec<ACT, true, 2>(v);
+                if (RES) {
+                  v[0] += to_f32(res[r * p.residual_stride]);
+                  if (two) v[1] += to_f32(res[r * p.residual_stride + 1]);
+                }
+                out[r * p.out_stride] = from_f32<T>(v[0]);
+                if (two) out[r * p.out_stride + 1] = from_f32<T>(v[1]);
               }
             }
           }
         }
       };
-      auto write_act = [&](auto act_c) {
+      op_act_switch(p.act, [&](auto act_c) {
         if (p.residual)
           write_tile(act_c, std::true_type());
         else
           write_tile(act_c, std::false_type());
-      };
-      switch (p.act) {
-        case OP_RELU: write_act(std::integral_constant<int, OP_RELU>()); break;
-        case OP_GELU: write_act(std::integral_constant<int, OP_GELU>()); break;
-        case OP_SIGMOID: write_act(std::integral_constant<int, OP_SIGMOID>()); break;
-        case OP_SILU: write_act(std::integral_constant<int, OP_SILU>()); break;
-        default: write_act(std::integral_constant<int, OP_NONE>());
-      }
+      });
       __syncwarp();  // the patch is read
     }
     if (lane == 0) {
@@ -477,7 +452,6 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
-  __syncwarp();
   if (PAIR) cluster_sync();  // nothing of the other CTA is in flight to this one
   if (warp == 1) {
     if (PAIR)

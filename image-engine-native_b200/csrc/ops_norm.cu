@@ -1,105 +1,158 @@
-// Group normalisation with an activation over channels-last maps.
-//
-//   mean = sum x / N, variance = sum (x - mean)^2 / N over the N = pixels *
-//   c / groups values of a group, out = act((x - mean) rstd gamma + beta)
-//
-// One CTA per map and group computes the statistics (two passes, so that a
-// mean far from zero costs no digits), a second kernel applies them.
-#include "ops_sm100.cuh"
+// Host side of the group normalisation (norm_sm100.cuh): which kernels a
+// shape takes, and their launches.
+#include <algorithm>
+#include <numeric>
+
+#include "norm_sm100.cuh"
 
 namespace iec {
 
 namespace {
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.0f;
-  for (int i = 0; i < (int)blockDim.x / 32; i++) t += red[i];
-  return t;
+constexpr int RESIDENT_BYTES = 180 * 1024;  // of a CTA's values in shared memory
+constexpr int CLUSTER = 8;
+
+template <auto Kernel>
+void allow_smem(Device& dev, int bytes) {
+  static int most[64] = {};
+  int& m = most[dev.ordinal() & 63];
+  if (bytes > m) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  m = std::max(m, bytes);
 }
 
+template <class... KArgs, class... Args>
+void launch(void (*kernel)(KArgs...), dim3 grid, size_t smem, int cluster, cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(NORM_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  IEC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// The resident kernel's shape, or false where a segment outgrows a cluster.
+// A segment is the smallest run of whole groups, vectors (and with fp8 whole
+// blocks) that has at least 128 bytes, so that segments read whole lines and
+// there are as many clusters as possible.
 template <class T>
-__global__ void __launch_bounds__(512) norm_stats(NormSpec p, float2* stats) {
-  __shared__ float red[16];
-  const int g = blockIdx.x, i = blockIdx.y, cg = p.c / p.groups;
-  const T* x = static_cast<const T*>(p.x) + i * p.x_map_stride + g * cg;
-  const long long count = p.pixels * cg;
-  float s = 0.0f;
-  for (long long e = threadIdx.x; e < count; e += blockDim.x) s += to_f32(x[e / cg * p.x_stride + e % cg]);
-  const float mean = block_sum(s, red) / (float)count;
-  float q = 0.0f;
-  for (long long e = threadIdx.x; e < count; e += blockDim.x) {
-    const float d = to_f32(x[e / cg * p.x_stride + e % cg]) - mean;
-    q = fmaf(d, d, q);
+bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, int* cluster, size_t* smem) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  const int cg = p.c / p.groups;
+  long long unit = std::lcm<long long>(cg, VE);
+  if (fp8) unit = std::lcm<long long>(unit, FP8_BLOCK);
+  long long seg = p.c;
+  if (unit < p.c && p.c % unit == 0) {
+    seg = unit;
+    while (seg < p.c && (seg * (long long)sizeof(T) < 128 || p.c % seg)) seg += unit;
   }
-  const float var = block_sum(q, red) / (float)count;
-  if (threadIdx.x == 0) stats[i * p.groups + g] = make_float2(mean, 1.0f / sqrtf(var + p.eps));
+  q->seg_c = (int)seg;
+  q->vecs = (int)seg / VE;
+  const int lanes = fp8 ? FP8_BLOCK / VE : 1;
+  q->slots = (q->vecs + lanes - 1) / lanes * lanes;
+  if (q->slots > NORM_THREADS || p.pixels > (1 << 24)) return false;
+  q->rows = NORM_THREADS / q->slots;
+  const int segs = p.c / q->seg_c, most_steps = RESIDENT_BYTES / (NORM_THREADS * 16);
+  const long long need = (p.pixels + (long long)most_steps * q->rows - 1) / ((long long)most_steps * q->rows);
+  if (need > CLUSTER || segs > 65535) return false;
+  // as many CTAs as fill the GPU, but at least two steps each
+  const long long spread = dev.sms() / std::max<long long>(1, (long long)segs * p.n);
+  const long long fill = (p.pixels + 2LL * q->rows - 1) / (2LL * q->rows);
+  int n = (int)std::max(need, std::min({spread, fill, (long long)CLUSTER}));
+  n = std::max(n, 1);
+  q->pixels = (int)((p.pixels + n - 1) / n);
+  *cluster = n;
+  const int steps = (q->pixels + q->rows - 1) / q->rows;
+  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 4 + (size_t)(q->seg_c / cg) * 16;
+  return *smem <= 220 * 1024;
 }
 
-template <class T>
-__device__ __forceinline__ float normed(const NormSpec& p, const float2* stats, long long row, int ch) {
-  const int i = (int)(row / p.pixels);
-  const long long px = row - i * p.pixels;
-  const float2 st = stats[i * p.groups + ch / (p.c / p.groups)];
-  const float v = to_f32(static_cast<const T*>(p.x)[i * p.x_map_stride + px * p.x_stride + ch]);
-  const float y = (v - st.x) * st.y * (p.gamma ? p.gamma[ch] : 1.0f) + (p.beta ? p.beta[ch] : 0.0f);
-  return op_act_any(y, p.act);
-}
-
-template <class T>
-__global__ void __launch_bounds__(256) norm_apply(NormSpec p, const float2* stats) {
-  const long long total = p.n * p.pixels * p.c;
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-    const long long row = e / p.c;
-    const int ch = (int)(e - row * p.c), i = (int)(row / p.pixels);
-    const float y = normed<T>(p, stats, row, ch);
-    static_cast<T*>(p.out)[i * p.out_map_stride + (row - i * p.pixels) * p.out_stride + ch] = from_f32<T>(y);
-  }
-}
-
-// One warp per pixel and block of 128 channels.
-template <class T>
-__global__ void __launch_bounds__(256) norm_apply_fp8(NormSpec p, const float2* stats) {
-  const int kb = (p.c + FP8_BLOCK - 1) / FP8_BLOCK, lane = threadIdx.x & 31;
-  const long long total = p.n * p.pixels * kb;
-  for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < total; t += (long long)gridDim.x * 8) {
-    const long long row = t / kb;
-    const int b = (int)(t - row * kb);
-    float v[4];
-    uint32_t top = 0;
-    for (int j = 0; j < 4; j++) {
-      const int ch = b * FP8_BLOCK + j * 32 + lane;
-      v[j] = ch < p.c ? normed<T>(p, stats, row, ch) : 0.0f;
-      top = max(top, abs_bits(v[j]));
-    }
-    top = __reduce_max_sync(~0u, top);
-    float factor, scale;
-    fp8_scale(top, &factor, &scale);
-    for (int j = 0; j < 4; j++) {
-      const int ch = b * FP8_BLOCK + j * 32 + lane;
-      if (ch < p.c) p.q.codes[row * p.q.code_stride + ch] = (uint8_t)e4m3x2(v[j] * factor, 0.0f);
-    }
-    if (lane == 0) p.q.scales[b * p.q.scale_stride + row] = scale;
+template <class T, int VE>
+void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
+  const int cg = p.c / p.groups;
+  NormChunks q = {};
+  q.tile_c = std::min(p.c, NORM_THREADS * VE);
+  q.tiles = (p.c + q.tile_c - 1) / q.tile_c;
+  q.slots = std::min(p.groups, (q.tile_c + cg - 2) / cg + 1);
+  if (q.tiles > 65535) throw Error(ERR_INPUT, "too many channels");
+  // Maps at a time: as many as their pairs take a few MB for.
+  const int rows = std::max(1, NORM_THREADS / (std::min(q.tile_c, p.c) / VE));
+  const long long ctas = dev.sms();
+  auto chunks_of = [&](long long maps) {
+    const long long want = std::max<long long>(1, ctas / (maps * q.tiles));
+    return std::max<long long>(1, std::min(want, (p.pixels + 8LL * rows - 1) / (8LL * rows)));
+  };
+  long long maps = p.n;
+  while (maps > 1 && maps * chunks_of(maps) * q.tiles * q.slots > (8 << 20)) maps = (maps + 1) / 2;
+  q.chunk = (p.pixels + chunks_of(maps) - 1) / chunks_of(maps);
+  q.chunks = (int)((p.pixels + q.chunk - 1) / q.chunk);
+  q.part = static_cast<float2*>(dev.scratch((size_t)maps * q.chunks * q.tiles * q.slots * sizeof(float2), s));
+  const size_t stats_smem = (size_t)NORM_THREADS * VE * 8;
+  const double values = (double)p.pixels * p.c;
+  for (q.map0 = 0; q.map0 < p.n; q.map0 += (int)maps) {
+    const int now = (int)std::min<long long>(maps, p.n - q.map0);
+    timed_launch("norm_stats", 4 * values * now, values * now * sizeof(T), s, [&] {
+      constexpr auto kernel = norm_stats<T, VE>;
+      launch(kernel, dim3(q.chunks, q.tiles, now), stats_smem, 1, s, p, q);
+    });
+    timed_launch("norm_apply", 10 * values * now, values * now * (sizeof(T) + (p.out ? sizeof(T) : 1)), s, [&] {
+      // two CTAs an SM, of at least eight steps
+      const long long per = std::max<long long>(1, 2LL * ctas / ((long long)now * q.tiles));
+      const dim3 grid((unsigned)std::min(per, (p.pixels + 8LL * rows - 1) / (8LL * rows)), q.tiles, now);
+      const size_t smem = (size_t)q.slots * sizeof(float2);
+      if (p.out) {
+        constexpr auto kernel = norm_apply<T, VE, false>;
+        allow_smem<kernel>(dev, (int)smem);
+        launch(kernel, grid, smem, 1, s, p, q);
+      } else if constexpr (VE > 1) {
+        constexpr auto kernel = norm_apply<T, VE, true>;
+        allow_smem<kernel>(dev, (int)smem);
+        launch(kernel, grid, smem, 1, s, p, q);
+      } else {
+        constexpr auto kernel = norm_apply_fp8_odd<T>;
+        const int blocks = (p.c + FP8_BLOCK - 1) / FP8_BLOCK;
+        const long long want = std::max<long long>(1, 4LL * ctas / ((long long)now * blocks));
+        const long long px = (p.pixels + NORM_THREADS / 32 - 1) / (NORM_THREADS / 32);
+        launch(kernel, dim3((unsigned)std::min(want, px), blocks, now), FP8_BLOCK * sizeof(float2), 1, s, p, q);
+      }
+    });
   }
 }
 
 template <class T>
 void run(Device& dev, const NormSpec& p, cudaStream_t s) {
-  float2* stats = static_cast<float2*>(dev.scratch((size_t)p.n * p.groups * sizeof(float2), s));
+  constexpr int VE = 16 / (int)sizeof(T);
+  const bool fp8 = p.out == nullptr;
+  // 16-byte vectors of x (and of out), 8 or 4 bytes of codes.
+  auto even = [](const void* ptr, long long a, long long b, int c, int bytes, int values) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && a % values == 0 && b % values == 0 && c % values == 0;
+  };
+  const bool wide = even(p.x, p.x_stride, p.x_map_stride, p.c, 16, VE) &&
+                    (fp8 ? even(p.q.codes, (long long)p.q.code_stride, 0, p.c, VE, VE)
+                         : even(p.out, p.out_stride, p.out_map_stride, p.c, 16, VE));
+  if (!wide) return run_chunks<T, 1>(dev, p, s);
+  NormResident q;
+  int cluster = 1;
+  size_t smem = 0;
+  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE>(dev, p, s);
   const double values = (double)p.n * p.pixels * p.c;
-  timed_launch("norm_stats", 3 * values, values * sizeof(T), s, [&] {
-    norm_stats<T><<<dim3(p.groups, p.n), 512, 0, s>>>(p, stats);
-    IEC_CUDA(cudaGetLastError());
-  });
-  timed_launch("norm_apply", 8 * values, values * (sizeof(T) + (p.out ? sizeof(T) : 1)), s, [&] {
-    if (p.out)
-      norm_apply<T><<<dev.sms() * 8, 256, 0, s>>>(p, stats);
-    else
-      norm_apply_fp8<T><<<dev.sms() * 8, 256, 0, s>>>(p, stats);
-    IEC_CUDA(cudaGetLastError());
+  timed_launch("norm_resident", 12 * values, values * (sizeof(T) + (fp8 ? 1 : sizeof(T))), s, [&] {
+    const dim3 grid(cluster, p.c / q.seg_c, p.n);
+    if (fp8) {
+      constexpr auto kernel = norm_resident<T, true>;
+      allow_smem<kernel>(dev, (int)smem);
+      launch(kernel, grid, smem, cluster, s, p, q);
+    } else {
+      constexpr auto kernel = norm_resident<T, false>;
+      allow_smem<kernel>(dev, (int)smem);
+      launch(kernel, grid, smem, cluster, s, p, q);
+    }
   });
 }
 

@@ -7,6 +7,7 @@
 #include <cuda_fp8.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "ops.h"
 
@@ -25,41 +26,113 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-// 1 / (1 + e^-v). e^-v overflows to infinity for v below about -88, whose
-// reciprocal is the limit 0.
-__device__ __forceinline__ float op_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-
-// The products that end an activation are not contracted with what is added
-// to them, so that every kernel and path rounds the same.
-template <int ACT>
-__device__ __forceinline__ float op_act(float v) {
-  if (ACT == OP_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays
-  if (ACT == OP_GELU) return __fmul_rn(0.5f * v, 1.0f + erff(v * 0.70710678118654752f));
-  if (ACT == OP_SIGMOID) return op_sigmoid(v);
-  if (ACT == OP_SILU) return __fmul_rn(v, op_sigmoid(v));
+// Two values rounded to T in one instruction (single conversions go through
+// a unit with an eighth of the rate).
+template <class T>
+__device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
+  uint32_t v;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
   return v;
 }
 
-__device__ __forceinline__ float op_act_any(float v, int act) {
-  if (act == OP_RELU) return op_act<OP_RELU>(v);
-  if (act == OP_GELU) return op_act<OP_GELU>(v);
-  if (act == OP_SIGMOID) return op_act<OP_SIGMOID>(v);
-  if (act == OP_SILU) return op_act<OP_SILU>(v);
-  return v;
+// Activations. Two kinds of accuracy: FAST for results that are rounded to 16
+// bits (a few units of f32), exact to about one unit for f32 results and for
+// values that are quantised (where every unit moves more of them across a
+// rounding boundary).
+//
+// e^-v for -43.6 <= v: t = -v log2(e), 2^t by the special-function unit, and
+// for the exact kind the rounding of t put back: 2^(t + d) = 2^t (1 + d ln 2).
+// Arguments outside [-43.6, 87] are clamped: below, v / (1 + e^-v) is less
+// than 1e-17 either way, and two denominators still multiply without
+// overflow (op_sigmoid_pair); above, 1 + e^-v is 1.
+template <bool FAST>
+__device__ __forceinline__ float op_exp_neg(float v) {
+  v = fminf(fmaxf(v, -43.6f), 87.0f);
+  constexpr float L = -1.4426950408889634f, L_LO = -1.925963033500e-8f;  // log2(e) = -(L + L_LO)
+  const float t = v * L;
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  if (!FAST) e = fmaf(e * 0.6931471805599453f, fmaf(v, L_LO, fmaf(v, L, -t)), e);
+  return e;
 }
 
-// The activation of N values, one branch for all of them.
-template <int N>
-__device__ __forceinline__ void op_act_n(float* v, int act) {
-#define IEC_OP_ACT(A_)                                  \
-  if (act == A_) {                                      \
-    _Pragma("unroll") for (int e = 0; e < N; e++) v[e] = op_act<A_>(v[e]); \
+// 1 / d; one Newton step for the exact kind.
+template <bool FAST>
+__device__ __forceinline__ float op_rcp(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  if (!FAST) r = fmaf(r, fmaf(-d, r, 1.0f), r);
+  return r;
+}
+
+template <bool FAST>
+__device__ __forceinline__ float op_sigmoid(float v) { return op_rcp<FAST>(1.0f + op_exp_neg<FAST>(v)); }
+
+// Two sigmoids by one reciprocal, of the denominators' product: the unit for
+// exponentials and reciprocals has an eighth of the multiplies' rate and
+// bounds these activations.
+template <bool FAST>
+__device__ __forceinline__ void op_sigmoid_pair(float v, float w, float* sv, float* sw) {
+  const float a = 1.0f + op_exp_neg<FAST>(v), b = 1.0f + op_exp_neg<FAST>(w), r = op_rcp<FAST>(a * b);
+  *sv = r * b;
+  *sw = r * a;
+}
+
+// GELU for FAST, as max(v, 0) - |v| / (2 P^16) (igemm_sm100.cuh); |error| at
+// most 1.5e-7 |v|.
+__device__ __forceinline__ float op_gelu_fast(float v) {
+  const float av = fabsf(v), a = av * 0.70710678118654752f;
+  float q = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(4.30638e-5f, a, 2.765672e-4f), a, 1.520143e-4f), a, 9.2705272e-3f), a,
+                          4.22820123e-2f),
+                     a, 7.05230784e-2f),
+                a, 1.0f);
+  q *= q;
+  q *= q;
+  q *= q;
+  q *= q;
+  return fmaf(-0.5f * av, op_rcp<true>(q), fmaxf(v, 0.0f));
+}
+
+// The activation of N values. The products that end an activation are not
+// contracted with what is added to them, so that every kernel and path
+// rounds the same. NaN stays NaN.
+template <int ACT, bool FAST, int N>
+__device__ __forceinline__ void op_act_vec(float* v) {
+  if constexpr (ACT == OP_RELU) {
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = v[e] < 0.0f ? 0.0f : v[e];
+  } else if constexpr (ACT == OP_GELU) {
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      v[e] = FAST ? op_gelu_fast(v[e]) : __fmul_rn(0.5f * v[e], 1.0f + erff(v[e] * 0.70710678118654752f));
+  } else if constexpr (ACT == OP_SIGMOID || ACT == OP_SILU) {
+    float s[N];
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < N; e += 2) op_sigmoid_pair<FAST>(v[e], v[e + 1], &s[e], &s[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++) s[e] = op_sigmoid<FAST>(v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = ACT == OP_SILU ? __fmul_rn(v[e], s[e]) : v[e] != v[e] ? v[e] : s[e];
   }
-  IEC_OP_ACT(OP_RELU)
-  else IEC_OP_ACT(OP_GELU)
-  else IEC_OP_ACT(OP_SIGMOID)
-  else IEC_OP_ACT(OP_SILU)
-#undef IEC_OP_ACT
+}
+
+// Calls f(std::integral_constant<int, ACT>()) for the activation `act`: the
+// choice is made once, outside the loops over values.
+template <class F>
+__device__ __forceinline__ void op_act_switch(int act, F&& f) {
+  switch (act) {
+    case OP_RELU: f(std::integral_constant<int, OP_RELU>()); break;
+    case OP_GELU: f(std::integral_constant<int, OP_GELU>()); break;
+    case OP_SIGMOID: f(std::integral_constant<int, OP_SIGMOID>()); break;
+    case OP_SILU: f(std::integral_constant<int, OP_SILU>()); break;
+    default: f(std::integral_constant<int, OP_NONE>());
+  }
 }
 
 constexpr int FP8_BLOCK = 128;  // values along k that share a scale
