@@ -8,17 +8,22 @@
 //
 // norm_resident: maps whose values fit into the shared memory of a cluster
 // per channel segment (a run of whole groups). Each thread copies its own
-// vectors there (cp.async), and sums, squared deviations and results are
-// computed from there, so a value crosses HBM once each way, in one launch,
-// and the variance is the exact two-pass one. The CTAs of a cluster split the
-// pixels and add their group sums over distributed shared memory, in a fixed
-// order.
+// vectors there (cp.async) and takes statistics as they arrive, so a value
+// crosses HBM once each way, in one launch; the CTAs of a cluster split the
+// pixels and join their statistics over distributed shared memory.
 //
 // norm_stats + norm_apply: larger maps. The first kernel reduces chunks of
-// pixels, per channel around the channel's first value (so that a mean far
-// from zero costs no digits), to (mean, sum of squared deviations) per
-// group; the second joins the chunks' pairs and applies them, walking the
-// pixels backwards, since the last ones are the likeliest to be in L2 still.
+// pixels to (mean, sum of squared deviations) per group; the second joins the
+// chunks' pairs and applies them, walking the pixels backwards, since the
+// last ones are the likeliest to be in L2 still.
+//
+// Statistics: each thread takes a few pixels at a time from registers, their
+// mean and the squared deviations around it, and joins that to what it has
+//   mean' = mean + d k / (n + k),  dev' = dev + dev_k + d^2 n k / (n + k)
+// (k values of mean mean_k after n, d = mean_k - mean), as threads, CTAs and
+// chunks are joined after it (means as one of them plus weighted differences
+// from it): no difference of large sums anywhere, so a mean far from zero
+// costs no digits, and equal values have variance 0. The order is fixed.
 #pragma once
 
 #include "ops_sm100.cuh"
@@ -26,19 +31,40 @@
 
 namespace iec {
 
-// VE values of T next to each other as f32: 16 bytes where the map's
-// channels, strides and base allow, else one at a time.
-template <class T, int VE>
+constexpr int NORM_THREADS = 512;
+
+// VE values of T next to each other: 16 bytes where the map has a multiple
+// of them as channels (AL: its base and strides let them be read at once),
+// else one value.
+template <class T, int VE, bool AL>
 struct Vec {
   using Raw = std::conditional_t<VE == 1, T, uint4>;
+  static constexpr int WORD = VE == 8 ? 2 : 1;  // values of a 32-bit word
   static __device__ __forceinline__ Raw zero() {
     if constexpr (VE == 1)
       return from_f32<T>(0.0f);
     else
       return make_uint4(0, 0, 0, 0);
   }
-  static __device__ __forceinline__ Raw fetch(const T* p) { return *reinterpret_cast<const Raw*>(p); }
-  static __device__ __forceinline__ void load(const T* p, float* v) { expand(fetch(p), v); }
+  static __device__ __forceinline__ Raw fetch(const T* p) {
+    if constexpr (VE == 1 || AL) {
+      return *reinterpret_cast<const Raw*>(p);
+    } else {
+      T v[VE];
+#pragma unroll
+      for (int e = 0; e < VE; e++) v[e] = p[e];
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4)
+          w[i] = __float_as_uint(v[i]);
+        else
+          w[i] = (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i]) |
+                 (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i + 1]) << 16;
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
   static __device__ __forceinline__ void expand(Raw q, float* v) {
     if constexpr (VE == 1) {
       v[0] = to_f32(q);
@@ -46,22 +72,29 @@ struct Vec {
       expand_16(q, v);
     }
   }
-  static __device__ __forceinline__ void expand_16(uint4 q, float* v) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
+  // The values of the i-th 32-bit word (VE 1: the one value).
+  static __device__ __forceinline__ void word(Raw q, int i, float* v) {
+    if constexpr (VE == 1) {
+      v[0] = to_f32(q);
+    } else {
+      const uint32_t w = i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w;
       if constexpr (sizeof(T) == 4) {
-        v[i] = __uint_as_float(w[i]);
+        v[0] = __uint_as_float(w);
       } else {
-        const uint16_t lo = (uint16_t)(w[i] & 0xffffu), hi = (uint16_t)(w[i] >> 16);
-        v[2 * i] = to_f32(reinterpret_cast<const T&>(lo));
-        v[2 * i + 1] = to_f32(reinterpret_cast<const T&>(hi));
+        const uint16_t lo = (uint16_t)(w & 0xffffu), hi = (uint16_t)(w >> 16);
+        v[0] = to_f32(reinterpret_cast<const T&>(lo));
+        v[1] = to_f32(reinterpret_cast<const T&>(hi));
       }
     }
   }
+  static __device__ __forceinline__ void expand_16(uint4 q, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) word(q, i, v + i * (VE / 4));
+  }
   static __device__ __forceinline__ void store(T* p, const float* v) {
-    if constexpr (VE == 1) {
-      *p = from_f32<T>(v[0]);
+    if constexpr (VE == 1 || !AL) {
+#pragma unroll
+      for (int e = 0; e < VE; e++) p[e] = from_f32<T>(v[e]);
     } else if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -74,7 +107,7 @@ struct Vec {
 // A thread's VE values of a pixel as e4m3 codes with the scale of their block
 // of 128: the block's threads are 128 / VE consecutive lanes. `live`: the
 // thread's channels exist.
-template <int VE>
+template <int VE, bool AL>
 __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch, bool live, const float* v) {
   constexpr int LANES = FP8_BLOCK / VE;
   uint32_t top = 0;
@@ -92,10 +125,14 @@ __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch
     w[e / 4] = (uint32_t)e4m3x2(v[e] * factor, v[e + 1] * factor) |
                (uint32_t)e4m3x2(v[e + 2] * factor, v[e + 3] * factor) << 16;
   uint8_t* out = q.codes + row * (long long)q.code_stride + ch;
-  if constexpr (VE == 8)
+  if constexpr (!AL) {
+#pragma unroll
+    for (int e = 0; e < VE; e++) out[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+  } else if constexpr (VE == 8) {
     *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-  else
+  } else {
     *reinterpret_cast<uint32_t*>(out) = w[0];
+  }
   if (ch % FP8_BLOCK == 0) q.scales[(long long)(ch / FP8_BLOCK) * (long long)q.scale_stride + row] = scale;
 }
 
@@ -105,6 +142,102 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// The running statistics of a thread's VE channels.
+template <int VE>
+struct Running {
+  float mean[VE], dev[VE];
+  int n = 0;
+  __device__ __forceinline__ Running() {
+#pragma unroll
+    for (int e = 0; e < VE; e++) mean[e] = dev[e] = 0.0f;
+  }
+  // U pixels, two channels at a time, so that few are held as f32.
+  template <class V, int U>
+  __device__ __forceinline__ void add(const typename V::Raw* raw) {
+    const float share = (float)U / (float)(n + U), both = (float)n * share;
+    constexpr int W = V::WORD;
+#pragma unroll
+    for (int e0 = 0; e0 < VE; e0 += W) {
+      float v[U][W];
+#pragma unroll
+      for (int u = 0; u < U; u++) V::word(raw[u], e0 / W, v[u]);
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        const int e = e0 + w;
+        // pairs of pairs: the mean of equal values is that value
+        float m[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) m[u] = v[u][w];
+#pragma unroll
+        for (int k = U / 2; k; k /= 2)
+#pragma unroll
+          for (int u = 0; u < k; u++) m[u] += m[u + k];
+        m[0] *= 1.0f / (float)U;
+        const float d = m[0] - mean[e];
+        float q = dev[e];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const float x = v[u][w] - m[0];
+          q = fmaf(x, x, q);
+        }
+        mean[e] = fmaf(d, share, mean[e]);
+        dev[e] = fmaf(d * both, d, q);
+      }
+    }
+    n += U;
+  }
+};
+
+// Joins the statistics of a CTA's threads per group: mean[r * c + ch] and
+// dev[] of channel ch over the pixels r, r + rows, ... of `px` (both arrays
+// are overwritten). Calls put(group, mean, dev) in one lane for each group of
+// cg channels that has some of the channels c0 .. c0 + c - 1.
+template <class F>
+__device__ __forceinline__ void join_threads(float* mean, float* dev, int c, int rows, int px, int c0, int cg, F&& put) {
+  __syncthreads();
+  const int full = min(rows, px), parts = max(1, min(NORM_THREADS / c, full));
+  const int q = px / rows, rem = px - q * rows;  // row r has q + (r < rem) pixels
+  auto count = [&](int part) {
+    const int k = (full - part + parts - 1) / parts, more = part < rem ? (rem - part + parts - 1) / parts : 0;
+    return (float)(k * q + more);
+  };
+  for (int i = threadIdx.x; i < c * parts; i += NORM_THREADS) {
+    const int part = i / c, ch = i - part * c;
+    const float inv = 1.0f / count(part);
+    const float m0 = mean[i];
+    float m = 0.0f, d = 0.0f;
+    for (int r = part; r < full; r += parts) m = fmaf((float)(q + (r < rem)) * inv, mean[r * c + ch] - m0, m);
+    m += m0;
+    for (int r = part; r < full; r += parts) {
+      const float x = mean[r * c + ch] - m;
+      d += fmaf((float)(q + (r < rem)) * x, x, dev[r * c + ch]);
+    }
+    mean[i] = m;  // row `part`, which only this thread has read
+    dev[i] = d;
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
+  for (int g = g0 + warp; g <= g1; g += NORM_THREADS / 32) {
+    const int a = max(g * cg, c0) - c0, w = min((g + 1) * cg, c0 + c) - c0 - a;
+    const float inv = 1.0f / ((float)px * (float)w);
+    const float m0 = mean[a];
+    float m = 0.0f, d = 0.0f;
+    for (int i = lane; i < w * parts; i += 32) {
+      const int part = i / w;
+      m = fmaf(count(part) * inv, mean[part * c + a + i - part * w] - m0, m);
+    }
+    m = m0 + warp_sum(m);
+    for (int i = lane; i < w * parts; i += 32) {
+      const int part = i / w, at = part * c + a + i - part * w;
+      const float x = mean[at] - m;
+      d += fmaf(count(part) * x, x, dev[at]);
+    }
+    d = warp_sum(d);
+    if (lane == 0) put(g, m, d);
+  }
+}
+
 // ---------------------------------------------------------------- resident
 struct NormResident {
   int seg_c, vecs, rows;  // channels of a segment, their vectors, pixels a CTA takes per step
@@ -112,18 +245,20 @@ struct NormResident {
   int pixels;             // of a CTA
 };
 
-constexpr int NORM_THREADS = 512;
-
 __device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(p, rank)) : "memory");
+template <int LEFT>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(const float2* p, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(p, rank)) : "memory");
   return v;
 }
 
-template <class T, bool FP8>
+template <class T, bool FP8, bool AL>
 __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec p, const NormResident q) {
   constexpr bool FAST = !FP8 && sizeof(T) == 2;
   constexpr int VE = 16 / (int)sizeof(T);
@@ -131,113 +266,114 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   const int rank = blockIdx.x, ctas = gridDim.x, seg = blockIdx.y, map = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cg = p.c / p.groups, groups = q.seg_c / cg;
-  // [step][thread] vectors, then per-channel sums of the rows of threads,
-  // then the group sums of the two reductions and the group's results.
-  uint4* data = reinterpret_cast<uint4*>(smem);
   const int steps = (q.pixels + q.rows - 1) / q.rows;
-  float* red = reinterpret_cast<float*>(smem + (size_t)steps * NORM_THREADS * 16);
-  float* sums = red + NORM_THREADS * VE;  // [2][groups]
-  float* stat = sums + 2 * groups;        // [2][groups]: mean, rstd
-  const int slot = threadIdx.x % q.slots, r = threadIdx.x / q.slots;
+  // [step][thread] vectors, the threads' statistics, the groups' statistics
+  // over this CTA and their mean and rstd over the cluster.
+  uint4* data = reinterpret_cast<uint4*>(smem) + threadIdx.x;
+  float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * NORM_THREADS * 16);
+  float* tdev = tmean + NORM_THREADS * VE;
+  float2* own = reinterpret_cast<float2*>(tdev + NORM_THREADS * VE);
+  float2* stat = own + groups;
+  const int r = threadIdx.x / q.slots, slot = threadIdx.x - r * q.slots;
   const bool live = r < q.rows && slot < q.vecs;
-  const int first = rank * q.pixels, last = (int)min((long long)first + q.pixels, p.pixels);
-  const int ch0 = seg * q.seg_c, ch = ch0 + slot * VE;
+  const int first = rank * q.pixels, px = max(0, (int)min((long long)q.pixels, p.pixels - first));
+  const int ch = seg * q.seg_c + slot * VE;
+  const int n = live && r < px ? (px - r + q.rows - 1) / q.rows : 0;  // this thread's vectors
   griddep_launch_dependents();
   griddep_wait();
 
-  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + ch;
-  for (int s = 0; s < steps; s++) {
-    const int px = first + s * q.rows + r;
-    if (live && px < last) cp_async_16(&data[s * NORM_THREADS + threadIdx.x], x + px * p.x_stride);
+  // The copies, in four groups; the first groups are added up while the
+  // others are on their way.
+  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + (first + r) * p.x_stride + ch;
+  const long long step = q.rows * p.x_stride;
+  const int batch = (steps + 15) / 16 * 4;  // whole fours
+  int s = 0;
+#pragma unroll 1
+  for (int b = 0; b < 4; b++) {
+    for (const int end = min(n, (b + 1) * batch); s < end; s++)
+      if constexpr (AL)
+        cp_async_16(data + s * NORM_THREADS, x + s * step);
+      else
+        data[s * NORM_THREADS] = Vec<T, VE, AL>::fetch(x + s * step);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-
-  // A group's total over this CTA of each thread's per-channel sums, the
-  // whole cluster's totals being ready when it returns.
-  auto group_total = [&](const float* v, float* own) {
-    if (live)
+  float scale[VE], beta[VE];
 #pragma unroll
-      for (int e = 0; e < VE; e++) red[r * q.seg_c + slot * VE + e] = v[e];
-    __syncthreads();
-    for (int ch_ = threadIdx.x; ch_ < q.seg_c; ch_ += NORM_THREADS) {
-      float t = 0.0f;
-      for (int k = 0; k < q.rows; k++) t += red[k * q.seg_c + ch_];
-      red[ch_] = t;  // its first row, which only this thread has read
+  for (int e = 0; e < VE; e++) {
+    scale[e] = live && p.gamma ? p.gamma[ch + e] : 1.0f;
+    beta[e] = live && p.beta ? p.beta[ch + e] : 0.0f;
+  }
+  using V = Vec<T, VE, AL>;
+  Running<VE> run;
+  auto add_until = [&](int end) {
+    int i = run.n;
+    for (; i + 4 <= end; i += 4) {
+      uint4 raw[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) raw[u] = data[(i + u) * NORM_THREADS];
+      run.template add<V, 4>(raw);
     }
-    __syncthreads();
-    for (int g = warp; g < groups; g += NORM_THREADS / 32) {
-      float t = 0.0f;
-      for (int k = lane; k < cg; k += 32) t += red[g * cg + k];
-      t = warp_sum(t);
-      if (lane == 0) own[g] = t;
+    if (end == n)
+      for (; i < end; i++) run.template add<V, 1>(data + i * NORM_THREADS);
+  };
+  cp_async_wait<3>();
+  add_until(min(n, batch));
+  cp_async_wait<2>();
+  add_until(min(n, 2 * batch));
+  cp_async_wait<1>();
+  add_until(min(n, 3 * batch));
+  cp_async_wait<0>();
+  add_until(n);
+  if (live)
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+      tmean[r * q.seg_c + slot * VE + e] = run.mean[e];
+      tdev[r * q.seg_c + slot * VE + e] = run.dev[e];
     }
-    cluster_sync();
-  };
-  auto joined = [&](const float* own, int g) {
-    float t = 0.0f;
-    for (int k = 0; k < ctas; k++) t += ld_cluster_f32(own + g, (uint32_t)k);
-    return t;
-  };
+  if (px > 0)
+    join_threads(tmean, tdev, q.seg_c, q.rows, px, 0, cg, [&](int g, float m, float d) { own[g] = make_float2(m, d); });
+  cluster_sync();
   const float count = (float)p.pixels * (float)cg;
-
-  float acc[VE];
-#pragma unroll
-  for (int e = 0; e < VE; e++) acc[e] = 0.0f;
-  for (int s = 0; s < steps; s++)
-    if (live && first + s * q.rows + r < last) {
-      float v[VE];
-      Vec<T, VE>::expand(data[s * NORM_THREADS + threadIdx.x], v);
-#pragma unroll
-      for (int e = 0; e < VE; e++) acc[e] += v[e];
+  for (int g = warp; g < groups; g += NORM_THREADS / 32) {
+    float2 v = make_float2(0.0f, 0.0f);
+    float k = 0.0f;
+    if (lane < ctas) {
+      k = (float)max(0, (int)min((long long)q.pixels, p.pixels - lane * q.pixels)) * (float)cg;
+      if (k > 0.0f) v = ld_cluster_f32x2(own + g, (uint32_t)lane);
     }
-  group_total(acc, sums);
-  for (int g = threadIdx.x; g < groups; g += NORM_THREADS) stat[g] = joined(sums, g) / count;
+    const float m0 = __shfl_sync(~0u, v.x, 0);  // the first CTA always has pixels
+    const float m = m0 + warp_sum(k * (v.x - m0)) / count, d = v.x - m;
+    const float dev = warp_sum(fmaf(k * d, d, v.y));
+    if (lane == 0) stat[g] = make_float2(m, 1.0f / sqrtf(dev / count + p.eps));
+  }
   __syncthreads();
   float mean[VE];
 #pragma unroll
   for (int e = 0; e < VE; e++) {
-    mean[e] = live ? stat[(slot * VE + e) / cg] : 0.0f;
-    acc[e] = 0.0f;
-  }
-  for (int s = 0; s < steps; s++)
-    if (live && first + s * q.rows + r < last) {
-      float v[VE];
-      Vec<T, VE>::expand(data[s * NORM_THREADS + threadIdx.x], v);
-#pragma unroll
-      for (int e = 0; e < VE; e++) {
-        const float d = v[e] - mean[e];
-        acc[e] = fmaf(d, d, acc[e]);
-      }
-    }
-  group_total(acc, sums + groups);
-  for (int g = threadIdx.x; g < groups; g += NORM_THREADS)
-    stat[groups + g] = 1.0f / sqrtf(joined(sums + groups, g) / count + p.eps);
-  __syncthreads();
-  float scale[VE], beta[VE];
-#pragma unroll
-  for (int e = 0; e < VE; e++) {
-    scale[e] = live ? stat[groups + (slot * VE + e) / cg] * (p.gamma ? p.gamma[ch + e] : 1.0f) : 0.0f;
-    beta[e] = live && p.beta ? p.beta[ch + e] : 0.0f;
+    const float2 st = live ? stat[(slot * VE + e) / cg] : make_float2(0.0f, 0.0f);
+    mean[e] = st.x;
+    scale[e] *= st.y;
   }
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    for (int s = 0; s < steps; s++) {
-      const int px = first + s * q.rows + r;
-      const bool here = live && px < last;
-      // with fp8 the lanes of a block go through the shuffles together
-      if (!FP8 && !here) continue;
+    // with fp8 the lanes of a block go through the shuffles together
+    const int end = FP8 ? steps : n;
+    const long long row0 = map * p.pixels + first + r;
+    T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + (first + r) * p.out_stride + ch;
+    const long long out_step = q.rows * p.out_stride;
+    for (int i = 0; i < end; i++) {
       float v[VE];
-      Vec<T, VE>::expand(here ? data[s * NORM_THREADS + threadIdx.x] : make_uint4(0, 0, 0, 0), v);
+      Vec<T, VE, AL>::expand(i < n ? data[i * NORM_THREADS] : make_uint4(0, 0, 0, 0), v);
 #pragma unroll
       for (int e = 0; e < VE; e++) v[e] = fmaf(v[e] - mean[e], scale[e], beta[e]);
       op_act_vec<ACT, FAST, VE>(v);
       if (FP8)
-        store_fp8<VE>(p.q, map * p.pixels + px, ch, here, v);
+        store_fp8<VE, AL>(p.q, row0 + (long long)i * q.rows, ch, i < n, v);
       else
-        Vec<T, VE>::store(static_cast<T*>(p.out) + map * p.out_map_stride + px * p.out_stride + ch, v);
+        Vec<T, VE, AL>::store(out + i * out_step, v);
     }
   });
-  cluster_sync();  // the others have read this CTA's sums
+  cluster_sync();  // the others have read this CTA's statistics
 }
 
 // ------------------------------------------------------------- two kernels
@@ -251,93 +387,45 @@ struct NormChunks {
   float2* part;
 };
 
-template <class T, int VE>
-__global__ void __launch_bounds__(NORM_THREADS) norm_stats(const NormSpec p, const NormChunks q) {
-  extern __shared__ __align__(16) float red[];  // [3][rows][channels of the tile]: value, mean, deviations
+template <class T, int VE, bool AL>
+__global__ void __launch_bounds__(NORM_THREADS, 2) norm_stats(const NormSpec p, const NormChunks q) {
+  extern __shared__ __align__(16) float tmean[];  // [2][rows][channels of the tile]
   const int tile = blockIdx.y, map = q.map0 + blockIdx.z;
   const int c0 = tile * q.tile_c, c = min(q.tile_c, p.c - c0), vecs = c / VE, cg = p.c / p.groups;
-  const int slot = threadIdx.x % vecs, r = threadIdx.x / vecs, rows = NORM_THREADS / vecs;
-  const bool live = r < rows;
-  const long long first = blockIdx.x * q.chunk, last = min(first + q.chunk, p.pixels);
+  const int r = threadIdx.x / vecs, slot = threadIdx.x - r * vecs, rows = NORM_THREADS / vecs;
+  const long long first = blockIdx.x * q.chunk;
+  const int px = (int)(min(first + q.chunk, p.pixels) - first);
   griddep_launch_dependents();
   griddep_wait();
-  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + c0 + slot * VE;
-  // Sums of the distances to this thread's first value of the channel.
-  float k[VE], s[VE], d2[VE];
-  int n = 0;
-#pragma unroll
-  for (int e = 0; e < VE; e++) k[e] = s[e] = d2[e] = 0.0f;
-  if (live && first + r < last) {
-    const T* at = x + (first + r) * p.x_stride;
+  using V = Vec<T, VE, AL>;
+  Running<VE> run;
+  if (r < rows) {
+    const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + c0 + slot * VE + (first + r) * p.x_stride;
     const long long step = (long long)rows * p.x_stride;
-    Vec<T, VE>::load(at, k);
-    n = (int)((last - first - r + rows - 1) / rows);
-    auto add = [&](typename Vec<T, VE>::Raw raw) {
-      float v[VE];
-      Vec<T, VE>::expand(raw, v);
-#pragma unroll
-      for (int e = 0; e < VE; e++) {
-        const float d = v[e] - k[e];
-        s[e] += d;
-        d2[e] = fmaf(d, d, d2[e]);
-      }
-    };
-    constexpr int U = 8;
+    const int n = r < px ? (px - r + rows - 1) / rows : 0;
+    constexpr int U = VE == 1 ? 8 : 4;
     int i = 0;
-    for (; i + U <= n; i += U, at += U * step) {
-      typename Vec<T, VE>::Raw raw[U];
+    for (; i + U <= n; i += U, x += U * step) {
+      typename Vec<T, VE, AL>::Raw raw[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) raw[u] = Vec<T, VE>::fetch(at + u * step);
-#pragma unroll
-      for (int u = 0; u < U; u++) add(raw[u]);
+      for (int u = 0; u < U; u++) raw[u] = Vec<T, VE, AL>::fetch(x + u * step);
+      run.template add<V, U>(raw);
     }
-    for (; i < n; i++, at += step) add(Vec<T, VE>::fetch(at));
+    for (; i < n; i++, x += step) {
+      const typename Vec<T, VE, AL>::Raw raw = Vec<T, VE, AL>::fetch(x);
+      run.template add<V, 1>(&raw);
+    }
   }
-  // (mean, deviations) of each thread's channels, joined over the rows of
-  // threads (each of its own count), then over a group's channels.
-  float* smean = red;
-  float* sdev = red + NORM_THREADS * VE;
-  if (live) {
-    const float inv = n ? 1.0f / (float)n : 0.0f;
+  float* tdev = tmean + NORM_THREADS * VE;
+  if (r < rows)
 #pragma unroll
     for (int e = 0; e < VE; e++) {
-      smean[r * c + slot * VE + e] = fmaf(s[e], inv, k[e]);
-      // not below zero; NaN stays
-      const float dev = fmaf(-s[e] * inv, s[e], d2[e]);
-      sdev[r * c + slot * VE + e] = dev < 0.0f ? 0.0f : dev;
+      tmean[r * c + slot * VE + e] = run.mean[e];
+      tdev[r * c + slot * VE + e] = run.dev[e];
     }
-  }
-  __syncthreads();
-  const int px = (int)(last - first), full = min(rows, px);
-  const float inv_px = 1.0f / (float)px;
-  for (int ch = threadIdx.x; ch < c; ch += NORM_THREADS) {
-    float mean = 0.0f, dev = 0.0f;
-    for (int k_ = 0; k_ < full; k_++)
-      mean = fmaf((float)((px - k_ + rows - 1) / rows) * inv_px, smean[k_ * c + ch], mean);
-    for (int k_ = 0; k_ < full; k_++) {
-      const float d = smean[k_ * c + ch] - mean;
-      dev += fmaf((float)((px - k_ + rows - 1) / rows) * d, d, sdev[k_ * c + ch]);
-    }
-    smean[ch] = mean;  // its first row, which only this thread has read
-    sdev[ch] = dev;
-  }
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
-  for (int g = g0 + warp; g <= g1; g += NORM_THREADS / 32) {
-    const int a = max(g * cg, c0) - c0, b = min((g + 1) * cg, c0 + c) - c0;
-    float t = 0.0f;
-    for (int ch = a + lane; ch < b; ch += 32) t += smean[ch];
-    const float mean = warp_sum(t) / (float)(b - a);
-    t = 0.0f;
-    for (int ch = a + lane; ch < b; ch += 32) {
-      const float d = smean[ch] - mean;
-      t += fmaf((float)px * d, d, sdev[ch]);
-    }
-    t = warp_sum(t);
-    if (lane == 0)
-      q.part[((blockIdx.z * (long long)q.chunks + blockIdx.x) * q.tiles + tile) * q.slots + g - g0] = make_float2(mean, t);
-  }
+  const int g0 = c0 / cg;
+  float2* part = q.part + ((blockIdx.z * (long long)q.chunks + blockIdx.x) * q.tiles + tile) * q.slots;
+  join_threads(tmean, tdev, c, rows, px, c0, cg, [&](int g, float m, float d) { part[g - g0] = make_float2(m, d); });
 }
 
 // Mean and rstd of group `g` of map `z` (of this launch) from the chunks'
@@ -352,22 +440,39 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
     return q.part[((z * (long long)q.chunks + chunk) * q.tiles + tile) * q.slots + g - c0 / cg];
   };
   const float count = (float)p.pixels * (float)cg;
-  float t = 0.0f, n;
-  for (int i = lane; i < q.chunks * span; i += 32) {
-    const float2 v = pair(i, &n);
-    t = fmaf(n, v.x, t);
+  const int all = q.chunks * span;
+  float m = 0.0f, d = 0.0f, n0;
+  const float m0 = pair(0, &n0).x;
+  if (all <= 8 * 32) {  // the usual case: all loads at once
+    float2 v[8];
+    float n[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      v[i] = make_float2(0.0f, 0.0f);
+      n[i] = 0.0f;
+      if (i * 32 + lane < all) v[i] = pair(i * 32 + lane, &n[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = fmaf(n[i], v[i].x - m0, m);
+    m = m0 + warp_sum(m) / count;
+#pragma unroll
+    for (int i = 0; i < 8; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
+  } else {
+    float n;
+    for (int i = lane; i < all; i += 32) {
+      const float2 v = pair(i, &n);
+      m = fmaf(n, v.x - m0, m);
+    }
+    m = m0 + warp_sum(m) / count;
+    for (int i = lane; i < all; i += 32) {
+      const float2 v = pair(i, &n);
+      d += fmaf(n * (v.x - m), v.x - m, v.y);
+    }
   }
-  const float mean = warp_sum(t) / count;
-  t = 0.0f;
-  for (int i = lane; i < q.chunks * span; i += 32) {
-    const float2 v = pair(i, &n);
-    const float d = v.x - mean;
-    t += fmaf(n * d, d, v.y);
-  }
-  return make_float2(mean, 1.0f / sqrtf(warp_sum(t) / count + p.eps));
+  return make_float2(m, 1.0f / sqrtf(warp_sum(d) / count + p.eps));
 }
 
-template <class T, int VE, bool FP8>
+template <class T, int VE, bool FP8, bool AL>
 __global__ void __launch_bounds__(NORM_THREADS, 2) norm_apply(const NormSpec p, const NormChunks q) {
   constexpr bool FAST = !FP8 && sizeof(T) == 2;
   extern __shared__ __align__(16) float2 stat[];  // of the tile's groups
@@ -404,26 +509,26 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) norm_apply(const NormSpec p, 
     constexpr int ACT = decltype(act_c)::value;
     constexpr int U = VE == 1 ? 8 : 4;
     for (int s = (steps - 1) / U * U; s >= 0 && steps; s -= U) {
-      typename Vec<T, VE>::Raw raw[U];
+      typename Vec<T, VE, AL>::Raw raw[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const long long px = first + (long long)(s + u) * rows + r;
-        raw[u] = Vec<T, VE>::zero();
-        if (live && px < last) raw[u] = Vec<T, VE>::fetch(x + px * p.x_stride);
+        raw[u] = Vec<T, VE, AL>::zero();
+        if (live && px < last) raw[u] = Vec<T, VE, AL>::fetch(x + px * p.x_stride);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const long long px = first + (long long)(s + u) * rows + r;
         const bool here = live && px < last;
         float v[VE];
-        Vec<T, VE>::expand(raw[u], v);
+        Vec<T, VE, AL>::expand(raw[u], v);
 #pragma unroll
         for (int e = 0; e < VE; e++) v[e] = fmaf(v[e] - mean[e], scale[e], beta[e]);
         op_act_vec<ACT, FAST, VE>(v);
         if constexpr (FP8)
-          store_fp8<VE>(p.q, map * p.pixels + px, ch, here, v);
+          store_fp8<VE, AL>(p.q, map * p.pixels + px, ch, here, v);
         else if (here)
-          Vec<T, VE>::store(out + px * p.out_stride, v);
+          Vec<T, VE, AL>::store(out + px * p.out_stride, v);
       }
     }
   });

@@ -10,12 +10,13 @@ namespace iec {
 namespace {
 
 constexpr int RESIDENT_BYTES = 180 * 1024;  // of a CTA's values in shared memory
-constexpr int CLUSTER = 8;
+constexpr int CLUSTER = 16;
 
 template <auto Kernel>
 void allow_smem(Device& dev, int bytes) {
   static int most[64] = {};
   int& m = most[dev.ordinal() & 63];
+  if (m == 0) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   if (bytes > m) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   m = std::max(m, bytes);
 }
@@ -69,11 +70,11 @@ bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, in
   q->pixels = (int)((p.pixels + n - 1) / n);
   *cluster = n;
   const int steps = (q->pixels + q->rows - 1) / q->rows;
-  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 4 + (size_t)(q->seg_c / cg) * 16;
+  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 8 + (size_t)(q->seg_c / cg) * 16;
   return *smem <= 220 * 1024;
 }
 
-template <class T, int VE>
+template <class T, int VE, bool AL>
 void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   const int cg = p.c / p.groups;
   NormChunks q = {};
@@ -83,7 +84,7 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   if (q.tiles > 65535) throw Error(ERR_INPUT, "too many channels");
   // Maps at a time: as many as their pairs take a few MB for.
   const int rows = std::max(1, NORM_THREADS / (std::min(q.tile_c, p.c) / VE));
-  const long long ctas = dev.sms();
+  const long long ctas = 2LL * dev.sms();  // two an SM
   auto chunks_of = [&](long long maps) {
     const long long want = std::max<long long>(1, ctas / (maps * q.tiles));
     return std::max<long long>(1, std::min(want, (p.pixels + 8LL * rows - 1) / (8LL * rows)));
@@ -98,26 +99,24 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   for (q.map0 = 0; q.map0 < p.n; q.map0 += (int)maps) {
     const int now = (int)std::min<long long>(maps, p.n - q.map0);
     timed_launch("norm_stats", 4 * values * now, values * now * sizeof(T), s, [&] {
-      constexpr auto kernel = norm_stats<T, VE>;
+      constexpr auto kernel = norm_stats<T, VE, AL>;
       launch(kernel, dim3(q.chunks, q.tiles, now), stats_smem, 1, s, p, q);
     });
     timed_launch("norm_apply", 10 * values * now, values * now * (sizeof(T) + (p.out ? sizeof(T) : 1)), s, [&] {
-      // two CTAs an SM, of at least eight steps
-      const long long per = std::max<long long>(1, 2LL * ctas / ((long long)now * q.tiles));
-      const dim3 grid((unsigned)std::min(per, (p.pixels + 8LL * rows - 1) / (8LL * rows)), q.tiles, now);
+      const dim3 grid(q.chunks, q.tiles, now);
       const size_t smem = (size_t)q.slots * sizeof(float2);
       if (p.out) {
-        constexpr auto kernel = norm_apply<T, VE, false>;
+        constexpr auto kernel = norm_apply<T, VE, false, AL>;
         allow_smem<kernel>(dev, (int)smem);
         launch(kernel, grid, smem, 1, s, p, q);
       } else if constexpr (VE > 1) {
-        constexpr auto kernel = norm_apply<T, VE, true>;
+        constexpr auto kernel = norm_apply<T, VE, true, AL>;
         allow_smem<kernel>(dev, (int)smem);
         launch(kernel, grid, smem, 1, s, p, q);
       } else {
         constexpr auto kernel = norm_apply_fp8_odd<T>;
         const int blocks = (p.c + FP8_BLOCK - 1) / FP8_BLOCK;
-        const long long want = std::max<long long>(1, 4LL * ctas / ((long long)now * blocks));
+        const long long want = std::max<long long>(1, 2LL * ctas / ((long long)now * blocks));
         const long long px = (p.pixels + NORM_THREADS / 32 - 1) / (NORM_THREADS / 32);
         launch(kernel, dim3((unsigned)std::min(want, px), blocks, now), FP8_BLOCK * sizeof(float2), 1, s, p, q);
       }
@@ -125,35 +124,42 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   }
 }
 
-template <class T>
-void run(Device& dev, const NormSpec& p, cudaStream_t s) {
+template <class T, bool AL>
+void run_vectors(Device& dev, const NormSpec& p, cudaStream_t s) {
   constexpr int VE = 16 / (int)sizeof(T);
   const bool fp8 = p.out == nullptr;
-  // 16-byte vectors of x (and of out), 8 or 4 bytes of codes.
-  auto even = [](const void* ptr, long long a, long long b, int c, int bytes, int values) {
-    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && a % values == 0 && b % values == 0 && c % values == 0;
-  };
-  const bool wide = even(p.x, p.x_stride, p.x_map_stride, p.c, 16, VE) &&
-                    (fp8 ? even(p.q.codes, (long long)p.q.code_stride, 0, p.c, VE, VE)
-                         : even(p.out, p.out_stride, p.out_map_stride, p.c, 16, VE));
-  if (!wide) return run_chunks<T, 1>(dev, p, s);
   NormResident q;
   int cluster = 1;
   size_t smem = 0;
-  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE>(dev, p, s);
+  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE, AL>(dev, p, s);
   const double values = (double)p.n * p.pixels * p.c;
   timed_launch("norm_resident", 12 * values, values * (sizeof(T) + (fp8 ? 1 : sizeof(T))), s, [&] {
     const dim3 grid(cluster, p.c / q.seg_c, p.n);
     if (fp8) {
-      constexpr auto kernel = norm_resident<T, true>;
+      constexpr auto kernel = norm_resident<T, true, AL>;
       allow_smem<kernel>(dev, (int)smem);
       launch(kernel, grid, smem, cluster, s, p, q);
     } else {
-      constexpr auto kernel = norm_resident<T, false>;
+      constexpr auto kernel = norm_resident<T, false, AL>;
       allow_smem<kernel>(dev, (int)smem);
       launch(kernel, grid, smem, cluster, s, p, q);
     }
   });
+}
+
+template <class T>
+void run(Device& dev, const NormSpec& p, cudaStream_t s) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  if (p.c % VE) return run_chunks<T, 1, true>(dev, p, s);
+  // 16-byte vectors of x and out, 8 or 4 bytes of codes
+  auto even = [](const void* ptr, long long a, long long b, int bytes) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && a % VE == 0 && b % VE == 0;
+  };
+  if (even(p.x, p.x_stride, p.x_map_stride, 16) && (p.out ? even(p.out, p.out_stride, p.out_map_stride, 16)
+                                                           : even(p.q.codes, (long long)p.q.code_stride, 0, VE)))
+    run_vectors<T, true>(dev, p, s);
+  else
+    run_vectors<T, false>(dev, p, s);
 }
 
 }  // namespace

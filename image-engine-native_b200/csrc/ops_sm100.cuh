@@ -45,12 +45,13 @@ __device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
 //
 // e^-v for -43.6 <= v: t = -v log2(e), 2^t by the special-function unit, and
 // for the exact kind the rounding of t put back: 2^(t + d) = 2^t (1 + d ln 2).
-// Arguments outside [-43.6, 87] are clamped: below, v / (1 + e^-v) is less
-// than 1e-17 either way, and two denominators still multiply without
-// overflow (op_sigmoid_pair); above, 1 + e^-v is 1.
+// Arguments are clamped from below, where v / (1 + e^-v) is less than 1e-17
+// either way, so that two denominators multiply without overflow
+// (op_sigmoid_pair), and for the exact kind from above, where 1 + e^-v is 1.
 template <bool FAST>
 __device__ __forceinline__ float op_exp_neg(float v) {
-  v = fminf(fmaxf(v, -43.6f), 87.0f);
+  v = fmaxf(v, -43.6f);
+  if (!FAST) v = fminf(v, 87.0f);
   constexpr float L = -1.4426950408889634f, L_LO = -1.925963033500e-8f;  // log2(e) = -(L + L_LO)
   const float t = v * L;
   float e;
