@@ -13,9 +13,9 @@
 // pixels and join their statistics over distributed shared memory.
 //
 // norm_stats + norm_apply: larger maps. The first kernel reduces chunks of
-// pixels to (mean, sum of squared deviations) per group; the second joins the
-// chunks' pairs and applies them, walking the pixels backwards, since the
-// last ones are the likeliest to be in L2 still.
+// pixels, a cluster of CTAs each, to (mean, sum of squared deviations) per
+// group; the second joins the chunks' pairs and applies them, walking the
+// pixels backwards, since the last ones are the likeliest to be in L2 still.
 //
 // Statistics: each thread takes a few pixels at a time from registers, their
 // mean and the squared deviations around it, and joins that to what it has
@@ -32,6 +32,8 @@
 namespace iec {
 
 constexpr int NORM_THREADS = 512;
+constexpr int NORM_RING = 3;
+constexpr int APPLY_THREADS = 256;
 
 // VE values of T next to each other: 16 bytes where the map has a multiple
 // of them as channels (AL: its base and strides let them be read at once),
@@ -39,7 +41,6 @@ constexpr int NORM_THREADS = 512;
 template <class T, int VE, bool AL>
 struct Vec {
   using Raw = std::conditional_t<VE == 1, T, uint4>;
-  static constexpr int WORD = VE == 8 ? 2 : 1;  // values of a 32-bit word
   static __device__ __forceinline__ Raw zero() {
     if constexpr (VE == 1)
       return from_f32<T>(0.0f);
@@ -87,6 +88,19 @@ struct Vec {
       }
     }
   }
+  // Channels 2 i and 2 i + 1 (VE 1: the one value, twice).
+  static __device__ __forceinline__ float2 pair(Raw q, int i) {
+    float v[2];
+    if constexpr (VE == 1) {
+      v[0] = v[1] = to_f32(q);
+    } else if constexpr (VE == 8) {
+      word(q, i, v);
+    } else {
+      word(q, 2 * i, v);
+      word(q, 2 * i + 1, v + 1);
+    }
+    return make_float2(v[0], v[1]);
+  }
   static __device__ __forceinline__ void expand_16(uint4 q, float* v) {
 #pragma unroll
     for (int i = 0; i < 4; i++) word(q, i, v + i * (VE / 4));
@@ -110,10 +124,10 @@ struct Vec {
 template <int VE, bool AL>
 __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch, bool live, const float* v) {
   constexpr int LANES = FP8_BLOCK / VE;
-  uint32_t top = 0;
+  float most = 0.0f;
 #pragma unroll
-  for (int e = 0; e < VE; e++) top = max(top, abs_bits(v[e]));
-  if (!live) top = 0;
+  for (int e = 0; e < VE; e++) most = max_abs(v[e], most);
+  uint32_t top = live ? abs_bits(most) : 0u;
 #pragma unroll
   for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
   float factor, scale;
@@ -121,9 +135,11 @@ __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch
   if (!live) return;
   uint32_t w[VE / 4];
 #pragma unroll
-  for (int e = 0; e < VE; e += 4)
-    w[e / 4] = (uint32_t)e4m3x2(v[e] * factor, v[e + 1] * factor) |
-               (uint32_t)e4m3x2(v[e + 2] * factor, v[e + 3] * factor) << 16;
+  for (int e = 0; e < VE; e += 4) {
+    const float2 a = fmul2(make_float2(v[e], v[e + 1]), both(factor));
+    const float2 b = fmul2(make_float2(v[e + 2], v[e + 3]), both(factor));
+    w[e / 4] = (uint32_t)e4m3x2(a.x, a.y) | (uint32_t)e4m3x2(b.x, b.y) << 16;
+  }
   uint8_t* out = q.codes + row * (long long)q.code_stride + ch;
   if constexpr (!AL) {
 #pragma unroll
@@ -134,6 +150,19 @@ __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch
     *reinterpret_cast<uint32_t*>(out) = w[0];
   }
   if (ch % FP8_BLOCK == 0) q.scales[(long long)(ch / FP8_BLOCK) * (long long)q.scale_stride + row] = scale;
+}
+
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(const float2* p, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(p, rank)) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -151,92 +180,177 @@ struct Running {
 #pragma unroll
     for (int e = 0; e < VE; e++) mean[e] = dev[e] = 0.0f;
   }
-  // U pixels, two channels at a time, so that few are held as f32.
+  // U pixels, two channels at a time: few are held as f32, on packed pairs.
   template <class V, int U>
   __device__ __forceinline__ void add(const typename V::Raw* raw) {
-    const float share = (float)U / (float)(n + U), both = (float)n * share;
-    constexpr int W = V::WORD;
+    const float share = (float)U * op_rcp((float)(n + U)), both_n = (float)n * share;
+    constexpr int P = VE == 1 ? 1 : 2;
 #pragma unroll
-    for (int e0 = 0; e0 < VE; e0 += W) {
-      float v[U][W];
+    for (int e = 0; e < VE; e += P) {
+      float2 v[U], m[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) V::word(raw[u], e0 / W, v[u]);
+      for (int u = 0; u < U; u++) m[u] = v[u] = V::pair(raw[u], e / P);
+      // pairs of pairs: the mean of equal values is that value
 #pragma unroll
-      for (int w = 0; w < W; w++) {
-        const int e = e0 + w;
-        // pairs of pairs: the mean of equal values is that value
-        float m[U];
+      for (int k = U / 2; k; k /= 2)
 #pragma unroll
-        for (int u = 0; u < U; u++) m[u] = v[u][w];
+        for (int u = 0; u < k; u++) m[u] = fadd2(m[u], m[u + k]);
+      m[0] = fmul2(m[0], both(1.0f / (float)U));
+      float2 q = make_float2(dev[e], dev[e + P - 1]);
+      const float2 old = make_float2(mean[e], mean[e + P - 1]);
+      const float2 neg = make_float2(-m[0].x, -m[0].y);
 #pragma unroll
-        for (int k = U / 2; k; k /= 2)
-#pragma unroll
-          for (int u = 0; u < k; u++) m[u] += m[u + k];
-        m[0] *= 1.0f / (float)U;
-        const float d = m[0] - mean[e];
-        float q = dev[e];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          const float x = v[u][w] - m[0];
-          q = fmaf(x, x, q);
-        }
-        mean[e] = fmaf(d, share, mean[e]);
-        dev[e] = fmaf(d * both, d, q);
+      for (int u = 0; u < U; u++) {
+        const float2 x = fadd2(v[u], neg);
+        q = ffma2(x, x, q);
       }
+      const float2 d = fadd2(old, neg);  // the other way round: its sign cancels below
+      const float2 now = ffma2(d, both(-share), old);
+      q = ffma2(fmul2(d, both(both_n)), d, q);
+      mean[e] = now.x;
+      dev[e] = q.x;
+      mean[e + P - 1] = P == 2 ? now.y : now.x;
+      dev[e + P - 1] = P == 2 ? q.y : q.x;
     }
     n += U;
   }
 };
 
-// Joins the statistics of a CTA's threads per group: mean[r * c + ch] and
-// dev[] of channel ch over the pixels r, r + rows, ... of `px` (both arrays
-// are overwritten). Calls put(group, mean, dev) in one lane for each group of
-// cg channels that has some of the channels c0 .. c0 + c - 1.
-template <class F>
-__device__ __forceinline__ void join_threads(float* mean, float* dev, int c, int rows, int px, int c0, int cg, F&& put) {
-  __syncthreads();
-  const int full = min(rows, px), parts = max(1, min(NORM_THREADS / c, full));
-  const int q = px / rows, rem = px - q * rows;  // row r has q + (r < rem) pixels
-  auto count = [&](int part) {
-    const int k = (full - part + parts - 1) / parts, more = part < rem ? (rem - part + parts - 1) / parts : 0;
-    return (float)(k * q + more);
-  };
-  for (int i = threadIdx.x; i < c * parts; i += NORM_THREADS) {
-    const int part = i / c, ch = i - part * c;
-    const float inv = 1.0f / count(part);
-    const float m0 = mean[i];
-    float m = 0.0f, d = 0.0f;
-    for (int r = part; r < full; r += parts) m = fmaf((float)(q + (r < rem)) * inv, mean[r * c + ch] - m0, m);
-    m += m0;
-    for (int r = part; r < full; r += parts) {
-      const float x = mean[r * c + ch] - m;
-      d += fmaf((float)(q + (r < rem)) * x, x, dev[r * c + ch]);
+// The largest power of two, at most VE, that divides a group's channels: so
+// many of a thread's channels next to each other are of one group.
+template <int VE>
+__host__ __device__ __forceinline__ int norm_run(int cg) {
+  return min(VE, cg & -cg);
+}
+
+// Joins a thread's channels (each of n pixels) in runs of `run`, and stores
+// the VE / run statistics at mean[] and dev[].
+template <int VE>
+__device__ __forceinline__ void store_runs(Running<VE>& s, int run, float* mean, float* dev) {
+  const float half = 0.5f * (float)s.n;
+#pragma unroll
+  for (int k = 1; k < VE; k *= 2)
+    if (k < run)
+#pragma unroll
+      for (int e = 0; e < VE; e += 2 * k) {
+        const float x = s.mean[e] - s.mean[e + k];
+        s.dev[e] = s.dev[e] + s.dev[e + k] + x * x * (half * (float)k);
+        s.mean[e] = fmaf(-0.5f, x, s.mean[e]);
+      }
+#pragma unroll
+  for (int e = 0; e < VE; e++)
+    if (e % run == 0) {
+      mean[e / run] = s.mean[e];
+      dev[e / run] = s.dev[e];
     }
-    mean[i] = m;  // row `part`, which only this thread has read
-    dev[i] = d;
-  }
+}
+
+// Joins the statistics of a CTA's threads per group: mean[r * c + ch] and
+// dev[] of the ch-th run of `run` channels over the pixels r, r + rows, ...
+// of `px` > 0 (both arrays are overwritten; c, c0 and cg count runs). Calls
+// put(group, mean, dev) in one lane for each group of cg runs that has some
+// of the runs c0 .. c0 + c - 1.
+template <class F>
+__device__ __forceinline__ void join_threads(float* mean, float* dev, int c, int rows, int px, int c0, int cg, int run,
+                                             F&& put) {
+  __shared__ float counts[NORM_THREADS];
   __syncthreads();
+  // First each run over the rows part, part + parts, ... ; row r has q +
+  // (r < rem) pixels.
+  const int full = min(rows, px), parts = max(1, min(NORM_THREADS / c, full));
+  const int q = px / rows, rem = px - q * rows;
+  const float k0 = (float)q, k1 = (float)(q + 1);
+  const int part = threadIdx.x / c, stride = c * parts;
+  if (part < parts)
+#pragma unroll 1
+    for (int i = threadIdx.x; i < (c > NORM_THREADS ? c : stride); i += NORM_THREADS) {
+      const float m0 = mean[i];
+      float m = 0.0f, d = 0.0f, n = 0.0f;
+#pragma unroll 1
+      for (int r = part, at = i; r < full; r += parts, at += stride) {
+        const float k = r < rem ? k1 : k0;
+        m = fmaf(k, mean[at] - m0, m);
+        n += k;
+      }
+      m = fmaf(m, op_rcp(n), m0);
+#pragma unroll 1
+      for (int r = part, at = i; r < full; r += parts, at += stride) {
+        const float x = mean[at] - m;
+        d += fmaf((r < rem ? k1 : k0) * (float)run * x, x, dev[at]);
+      }
+      mean[i] = m;  // row `part`, which only this thread has read
+      dev[i] = d;
+      counts[part] = n;
+    }
+  __syncthreads();
+  // Then a group's runs and parts, one warp a group: `per` parts of w runs
+  // at a time.
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
+#pragma unroll 1
   for (int g = g0 + warp; g <= g1; g += NORM_THREADS / 32) {
     const int a = max(g * cg, c0) - c0, w = min((g + 1) * cg, c0 + c) - c0 - a;
-    const float inv = 1.0f / ((float)px * (float)w);
+    const int per = w < 32 ? 32 / w : 1, first = w < 32 ? lane / w : 0, j0 = lane - first * w;
     const float m0 = mean[a];
     float m = 0.0f, d = 0.0f;
-    for (int i = lane; i < w * parts; i += 32) {
-      const int part = i / w;
-      m = fmaf(count(part) * inv, mean[part * c + a + i - part * w] - m0, m);
-    }
-    m = m0 + warp_sum(m);
-    for (int i = lane; i < w * parts; i += 32) {
-      const int part = i / w, at = part * c + a + i - part * w;
-      const float x = mean[at] - m;
-      d += fmaf(count(part) * x, x, dev[at]);
-    }
+    if (first < per)
+#pragma unroll 1
+      for (int k = first; k < parts; k += per)
+        for (int j = j0; j < w; j += 32) m = fmaf(counts[k], mean[k * c + a + j] - m0, m);
+    m = m0 + warp_sum(m) / ((float)px * (float)w);
+    if (first < per)
+#pragma unroll 1
+      for (int k = first; k < parts; k += per)
+        for (int j = j0; j < w; j += 32) {
+          const float x = mean[k * c + a + j] - m;
+          d += fmaf(counts[k] * (float)run * x, x, dev[k * c + a + j]);
+        }
     d = warp_sum(d);
     if (lane == 0) put(g, m, d);
   }
 }
+
+// The constants of a thread's VE channels from its groups' (mean, rstd):
+// act((v - mean) scale + shift). (v scale + (shift - mean scale) would be an
+// operation less, but rounds at the size of mean scale.)
+template <int VE>
+struct Affine {
+  float mean[VE], scale[VE], shift[VE];
+  __device__ __forceinline__ void fetch(const NormSpec& p, int ch, bool live) {
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+      scale[e] = live && p.gamma ? p.gamma[ch + e] : 1.0f;
+      shift[e] = live && p.beta ? p.beta[ch + e] : 0.0f;
+    }
+  }
+  // `ch`: the first channel; stat[0] is group `g0`'s.
+  __device__ __forceinline__ void set(const float2* stat, int ch, int g0, int cg) {
+    int g = ch / cg, left = (g + 1) * cg - ch;
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+      const float2 st = stat[g - g0];
+      mean[e] = st.x;
+      scale[e] *= st.y;
+      if (--left == 0) {
+        g++;
+        left = cg;
+      }
+    }
+  }
+  __device__ __forceinline__ void apply(float* v) const {
+    if constexpr (VE == 1) {
+      v[0] = fmaf(v[0] - mean[0], scale[0], shift[0]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) {
+        const float2 d = fadd2(make_float2(v[e], v[e + 1]), make_float2(-mean[e], -mean[e + 1]));
+        const float2 y = ffma2(d, make_float2(scale[e], scale[e + 1]), make_float2(shift[e], shift[e + 1]));
+        v[e] = y.x;
+        v[e + 1] = y.y;
+      }
+    }
+  }
+};
 
 // ---------------------------------------------------------------- resident
 struct NormResident {
@@ -244,19 +358,6 @@ struct NormResident {
   int slots;              // threads of a pixel: vecs, rounded up to whole blocks of 128 channels with fp8
   int pixels;             // of a CTA
 };
-
-__device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-template <int LEFT>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-__device__ __forceinline__ float2 ld_cluster_f32x2(const float2* p, uint32_t rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(p, rank)) : "memory");
-  return v;
-}
 
 template <class T, bool FP8, bool AL>
 __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec p, const NormResident q) {
@@ -297,12 +398,8 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
         data[s * NORM_THREADS] = Vec<T, VE, AL>::fetch(x + s * step);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  float scale[VE], beta[VE];
-#pragma unroll
-  for (int e = 0; e < VE; e++) {
-    scale[e] = live && p.gamma ? p.gamma[ch + e] : 1.0f;
-    beta[e] = live && p.beta ? p.beta[ch + e] : 0.0f;
-  }
+  Affine<VE> affine;
+  affine.fetch(p, ch, live);
   using V = Vec<T, VE, AL>;
   Running<VE> run;
   auto add_until = [&](int end) {
@@ -324,36 +421,29 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   add_until(min(n, 3 * batch));
   cp_async_wait<0>();
   add_until(n);
-  if (live)
-#pragma unroll
-    for (int e = 0; e < VE; e++) {
-      tmean[r * q.seg_c + slot * VE + e] = run.mean[e];
-      tdev[r * q.seg_c + slot * VE + e] = run.dev[e];
-    }
+  const int w = norm_run<VE>(cg), runs = q.seg_c / w;
+  if (live) store_runs<VE>(run, w, tmean + r * runs + slot * VE / w, tdev + r * runs + slot * VE / w);
   if (px > 0)
-    join_threads(tmean, tdev, q.seg_c, q.rows, px, 0, cg, [&](int g, float m, float d) { own[g] = make_float2(m, d); });
+    join_threads(tmean, tdev, runs, q.rows, px, 0, cg / w, w,
+                 [&](int g, float m, float d) { own[g] = make_float2(m, d); });
   cluster_sync();
-  const float count = (float)p.pixels * (float)cg;
+  const float inv = 1.0f / ((float)p.pixels * (float)cg);
+#pragma unroll 1
   for (int g = warp; g < groups; g += NORM_THREADS / 32) {
     float2 v = make_float2(0.0f, 0.0f);
     float k = 0.0f;
-    if (lane < ctas) {
-      k = (float)max(0, (int)min((long long)q.pixels, p.pixels - lane * q.pixels)) * (float)cg;
-      if (k > 0.0f) v = ld_cluster_f32x2(own + g, (uint32_t)lane);
+    const int theirs = min(q.pixels, (int)p.pixels - lane * q.pixels);
+    if (lane < ctas && theirs > 0) {
+      k = (float)theirs * (float)cg;
+      v = ld_cluster_f32x2(own + g, (uint32_t)lane);
     }
     const float m0 = __shfl_sync(~0u, v.x, 0);  // the first CTA always has pixels
-    const float m = m0 + warp_sum(k * (v.x - m0)) / count, d = v.x - m;
+    const float m = m0 + warp_sum(k * (v.x - m0)) * inv, d = v.x - m;
     const float dev = warp_sum(fmaf(k * d, d, v.y));
-    if (lane == 0) stat[g] = make_float2(m, 1.0f / sqrtf(dev / count + p.eps));
+    if (lane == 0) stat[g] = make_float2(m, 1.0f / sqrtf(dev * inv + p.eps));
   }
   __syncthreads();
-  float mean[VE];
-#pragma unroll
-  for (int e = 0; e < VE; e++) {
-    const float2 st = live ? stat[(slot * VE + e) / cg] : make_float2(0.0f, 0.0f);
-    mean[e] = st.x;
-    scale[e] *= st.y;
-  }
+  affine.set(stat, live ? slot * VE : 0, 0, cg);
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     // with fp8 the lanes of a block go through the shuffles together
@@ -361,11 +451,11 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     const long long row0 = map * p.pixels + first + r;
     T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + (first + r) * p.out_stride + ch;
     const long long out_step = q.rows * p.out_stride;
+#pragma unroll 1
     for (int i = 0; i < end; i++) {
       float v[VE];
       Vec<T, VE, AL>::expand(i < n ? data[i * NORM_THREADS] : make_uint4(0, 0, 0, 0), v);
-#pragma unroll
-      for (int e = 0; e < VE; e++) v[e] = fmaf(v[e] - mean[e], scale[e], beta[e]);
+      affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
       if (FP8)
         store_fp8<VE, AL>(p.q, row0 + (long long)i * q.rows, ch, i < n, v);
@@ -377,13 +467,15 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
 }
 
 // ------------------------------------------------------------- two kernels
-// A tile is a run of up to NORM_THREADS vectors of channels (tile_c
-// channels, the last one shorter), a chunk a run of pixels. part[map][chunk]
-// [tile][slot] is the pair of the tile's slot-th group over the chunk.
+// A tile is a run of up to APPLY_THREADS vectors of channels (tile_c
+// channels, the last one shorter), a chunk the pixels of one cluster: `span`
+// for each of its `cluster` CTAs. part[map][tile][slot][chunk] is the pair of
+// the tile's slot-th group over the chunk. (One pair a CTA, joined by every
+// CTA of norm_apply, cost that kernel 11 us of L2 reads at 296 CTAs.)
 struct NormChunks {
-  int tiles, tile_c, chunks, slots;
-  long long chunk;  // pixels
-  int map0;         // the first map of this launch
+  int tiles, tile_c, chunks, slots, cluster;
+  long long span;  // pixels of a CTA of norm_stats
+  int map0;        // the first map of this launch
   float2* part;
 };
 
@@ -393,39 +485,82 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) norm_stats(const NormSpec p, 
   const int tile = blockIdx.y, map = q.map0 + blockIdx.z;
   const int c0 = tile * q.tile_c, c = min(q.tile_c, p.c - c0), vecs = c / VE, cg = p.c / p.groups;
   const int r = threadIdx.x / vecs, slot = threadIdx.x - r * vecs, rows = NORM_THREADS / vecs;
-  const long long first = blockIdx.x * q.chunk;
-  const int px = (int)(min(first + q.chunk, p.pixels) - first);
+  const long long first = blockIdx.x * q.span;
+  const int px = (int)max(0ll, min(q.span, p.pixels - first));
   griddep_launch_dependents();
   griddep_wait();
   using V = Vec<T, VE, AL>;
   Running<VE> run;
-  if (r < rows) {
-    const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + c0 + slot * VE + (first + r) * p.x_stride;
-    const long long step = (long long)rows * p.x_stride;
-    const int n = r < px ? (px - r + rows - 1) / rows : 0;
-    constexpr int U = VE == 1 ? 8 : 4;
-    int i = 0;
-    for (; i + U <= n; i += U, x += U * step) {
-      typename Vec<T, VE, AL>::Raw raw[U];
+  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + c0 + slot * VE + (first + r) * p.x_stride;
+  const long long step = (long long)rows * p.x_stride;
+  const int n = r < rows && r < px ? (px - r + rows - 1) / rows : 0;
+  int i = 0;
+  if constexpr (VE > 1 && AL) {
+    // Through a ring of shared memory, NORM_RING fours of pixels deep, so
+    // that copies are on their way all the time.
+    uint4* ring = reinterpret_cast<uint4*>(tmean) + threadIdx.x;
+    const int fours = n / 4;
+    auto copy = [&](int f) {
+      if (f < fours) {
+        const T* at = x + 4 * f * step;
+        uint4* to = ring + f % NORM_RING * 4 * NORM_THREADS;
 #pragma unroll
-      for (int u = 0; u < U; u++) raw[u] = Vec<T, VE, AL>::fetch(x + u * step);
+        for (int u = 0; u < 4; u++) cp_async_16(to + u * NORM_THREADS, at + u * step);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int f = 0; f < NORM_RING - 1; f++) copy(f);
+    for (int f = 0; f < fours; f++) {
+      copy(f + NORM_RING - 1);
+      cp_async_wait<NORM_RING - 1>();
+      uint4 raw[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) raw[u] = ring[(f % NORM_RING * 4 + u) * NORM_THREADS];
+      run.template add<V, 4>(raw);
+    }
+    i = 4 * fours;
+    cp_async_wait<0>();
+    __syncthreads();  // the ring becomes the threads' statistics
+  } else {
+    constexpr int U = VE == 1 ? 8 : 4;
+    for (; i + U <= n; i += U) {
+      typename V::Raw raw[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) raw[u] = V::fetch(x + (i + u) * step);
       run.template add<V, U>(raw);
     }
-    for (; i < n; i++, x += step) {
-      const typename Vec<T, VE, AL>::Raw raw = Vec<T, VE, AL>::fetch(x);
-      run.template add<V, 1>(&raw);
-    }
+  }
+  for (; i < n; i++) {
+    const typename V::Raw raw = V::fetch(x + i * step);
+    run.template add<V, 1>(&raw);
   }
   float* tdev = tmean + NORM_THREADS * VE;
-  if (r < rows)
-#pragma unroll
-    for (int e = 0; e < VE; e++) {
-      tmean[r * c + slot * VE + e] = run.mean[e];
-      tdev[r * c + slot * VE + e] = run.dev[e];
-    }
-  const int g0 = c0 / cg;
-  float2* part = q.part + ((blockIdx.z * (long long)q.chunks + blockIdx.x) * q.tiles + tile) * q.slots;
-  join_threads(tmean, tdev, c, rows, px, c0, cg, [&](int g, float m, float d) { part[g - g0] = make_float2(m, d); });
+  const int w = norm_run<VE>(cg), runs = c / w;
+  if (r < rows) store_runs<VE>(run, w, tmean + r * runs + slot * VE / w, tdev + r * runs + slot * VE / w);
+  const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
+  __shared__ float2 own[NORM_THREADS];
+  float2* const pairs = q.slots <= NORM_THREADS ? own : reinterpret_cast<float2*>(tdev + NORM_THREADS * VE);
+  if (px > 0)
+    join_threads(tmean, tdev, runs, rows, px, c0 / w, cg / w, w,
+                 [&](int g, float m, float d) { pairs[g - g0] = make_float2(m, d); });
+  cluster_sync();
+  const int rank = blockIdx.x % q.cluster, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long base = first - rank * q.span;  // the cluster's first pixel
+#pragma unroll 1
+  for (int g = g0 + rank * (NORM_THREADS / 32) + warp; g <= g1; g += q.cluster * (NORM_THREADS / 32)) {
+    const int width = min((g + 1) * cg, c0 + c) - max(g * cg, c0);
+    const float k = (float)max(0ll, min(q.span, p.pixels - base - lane * q.span)) * (float)width;
+    const bool some = lane < q.cluster && k > 0.0f;
+    const float2 v = some ? ld_cluster_f32x2(pairs + g - g0, (uint32_t)lane) : make_float2(0.0f, 0.0f);
+    const float n = warp_sum(some ? k : 0.0f), m0 = __shfl_sync(~0u, v.x, 0);
+    const float m = m0 + warp_sum(some ? k * (v.x - m0) : 0.0f) / fmaxf(n, 1.0f), d = v.x - m;
+    const float dev = warp_sum(some ? fmaf(k * d, d, v.y) : 0.0f);
+    if (lane == 0)
+      q.part[((blockIdx.z * (long long)q.tiles + tile) * q.slots + g - g0) * q.chunks + blockIdx.x / q.cluster] =
+          make_float2(m, dev);
+  }
+  cluster_sync();  // the others have read this CTA's pairs
 }
 
 // Mean and rstd of group `g` of map `z` (of this launch) from the chunks'
@@ -433,30 +568,31 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) norm_stats(const NormSpec p, 
 __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks& q, int z, int g) {
   const int cg = p.c / p.groups, lane = threadIdx.x & 31;
   const int t0 = g * cg / q.tile_c, t1 = (g * cg + cg - 1) / q.tile_c, span = t1 - t0 + 1;
+  const long long chunk = q.span * q.cluster;
   auto pair = [&](int i, float* n) {
-    const int chunk = i / span, tile = t0 + i % span, c0 = tile * q.tile_c;
+    const int s = span == 1 ? 0 : i / q.chunks, tile = t0 + s, k = i - s * q.chunks, c0 = tile * q.tile_c;
     const int w = min((g + 1) * cg, c0 + q.tile_c) - max(g * cg, c0);
-    *n = (float)(min((chunk + 1) * q.chunk, p.pixels) - chunk * q.chunk) * (float)w;
-    return q.part[((z * (long long)q.chunks + chunk) * q.tiles + tile) * q.slots + g - c0 / cg];
+    *n = (float)max(0ll, min(chunk, p.pixels - k * chunk)) * (float)w;
+    return q.part[((z * (long long)q.tiles + tile) * q.slots + g - c0 / cg) * q.chunks + k];
   };
   const float count = (float)p.pixels * (float)cg;
   const int all = q.chunks * span;
   float m = 0.0f, d = 0.0f, n0;
   const float m0 = pair(0, &n0).x;
-  if (all <= 8 * 32) {  // the usual case: all loads at once
-    float2 v[8];
-    float n[8];
+  if (all <= 2 * 32) {  // the usual case: all loads at once
+    float2 v[2];
+    float n[2];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < 2; i++) {
       v[i] = make_float2(0.0f, 0.0f);
       n[i] = 0.0f;
       if (i * 32 + lane < all) v[i] = pair(i * 32 + lane, &n[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaf(n[i], v[i].x - m0, m);
+    for (int i = 0; i < 2; i++) m = fmaf(n[i], v[i].x - m0, m);
     m = m0 + warp_sum(m) / count;
 #pragma unroll
-    for (int i = 0; i < 8; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
+    for (int i = 0; i < 2; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
   } else {
     float n;
     for (int i = lane; i < all; i += 32) {
@@ -473,63 +609,77 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
 }
 
 template <class T, int VE, bool FP8, bool AL>
-__global__ void __launch_bounds__(NORM_THREADS, 2) norm_apply(const NormSpec p, const NormChunks q) {
+__global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p, const NormChunks q) {
   constexpr bool FAST = !FP8 && sizeof(T) == 2;
+  using V = Vec<T, VE, AL>;
   extern __shared__ __align__(16) float2 stat[];  // of the tile's groups
-  // the chunks backwards, the latest map first
+  // the pixels backwards, the latest map first
   const int tile = blockIdx.y, z = (int)gridDim.z - 1 - (int)blockIdx.z, map = q.map0 + z;
   const int c0 = tile * q.tile_c, c = min(q.tile_c, p.c - c0), vecs = c / VE, cg = p.c / p.groups;
   const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
+  constexpr int LANES = FP8 ? FP8_BLOCK / VE : 1;
+  const int slots = (vecs + LANES - 1) / LANES * LANES, rows = APPLY_THREADS / slots;
+  const int r = threadIdx.x / slots, slot = threadIdx.x - r * slots;
+  const bool live = r < rows && slot < vecs;
+  const int ch = c0 + (live ? slot * VE : 0);
+  Affine<VE> affine;
+  affine.fetch(p, ch, live);
   griddep_launch_dependents();
   griddep_wait();
-  for (int g = g0 + (int)(threadIdx.x >> 5); g <= g1; g += NORM_THREADS / 32) {
+  for (int g = g0 + (int)(threadIdx.x >> 5); g <= g1; g += APPLY_THREADS / 32) {
     const float2 st = norm_join(p, q, z, g);
     if ((threadIdx.x & 31) == 0) stat[g - g0] = st;
   }
   __syncthreads();
-  constexpr int LANES = FP8 ? FP8_BLOCK / VE : 1;
-  const int slots = (vecs + LANES - 1) / LANES * LANES;
-  const int slot = threadIdx.x % slots, r = threadIdx.x / slots, rows = NORM_THREADS / slots;
-  const bool live = r < rows && slot < vecs;
-  const int ch = c0 + slot * VE;
-  float mean[VE], scale[VE], beta[VE];
-#pragma unroll
-  for (int e = 0; e < VE; e++) {
-    const float2 st = live ? stat[(ch + e) / cg - g0] : make_float2(0.0f, 0.0f);
-    mean[e] = st.x;
-    scale[e] = live && p.gamma ? st.y * p.gamma[ch + e] : st.y;
-    beta[e] = live && p.beta ? p.beta[ch + e] : 0.0f;
-  }
+  affine.set(stat, ch, g0, cg);
   const long long span = (p.pixels + gridDim.x - 1) / gridDim.x;
-  const long long first = ((long long)gridDim.x - 1 - blockIdx.x) * span, last = min(first + span, p.pixels);
-  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + ch;
-  T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + ch;
-  const int steps = first < last ? (int)((last - first + rows - 1) / rows) : 0;
+  const long long first = ((long long)gridDim.x - 1 - blockIdx.x) * span;
+  const int px = (int)max(0ll, min(span, p.pixels - first));
+  constexpr int U = VE == 1 ? 8 : 4;
+  const int per = U * rows, full = px / per;
+  const long long x_step = (long long)rows * p.x_stride, out_step = (long long)rows * p.out_stride;
+  // threads without a pixel of their own go through the motions on row 0's
+  const int own = r < rows ? r : 0;
+  const long long at = first + (long long)full * per + own;
+  const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + at * p.x_stride + ch;
+  T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + at * p.out_stride + ch;
+  long long row = map * p.pixels + at;
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    constexpr int U = VE == 1 ? 8 : 4;
-    for (int s = (steps - 1) / U * U; s >= 0 && steps; s -= U) {
-      typename Vec<T, VE, AL>::Raw raw[U];
+    auto put = [&](typename V::Raw raw, int u, bool here) {
+      float v[VE];
+      V::expand(raw, v);
+      affine.apply(v);
+      op_act_vec<ACT, FAST, VE>(v);
+      if constexpr (FP8)
+        store_fp8<VE, AL>(p.q, row + u * rows, ch, here, v);
+      else if (here)
+        V::store(out + u * out_step, v);
+    };
+    for (int u = 0, left = px - full * per; u * rows < left; u++) {
+      const bool here = live && u * rows + r < left;
+      put(here ? V::fetch(x + u * x_step) : V::zero(), u, here);
+    }
+    if (!FP8 && !live) return;
+    // Whole fours of steps, the next ones' loads ahead of this one's work.
+    typename V::Raw raw[U];
+    if (full) {
+      x -= U * x_step;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const long long px = first + (long long)(s + u) * rows + r;
-        raw[u] = Vec<T, VE, AL>::zero();
-        if (live && px < last) raw[u] = Vec<T, VE, AL>::fetch(x + px * p.x_stride);
-      }
+      for (int u = 0; u < U; u++) raw[u] = V::fetch(x + u * x_step);
+    }
+    for (int f = full; f > 0; f--) {
+      typename V::Raw next[U];
+      x -= U * x_step;
+      if (f > 1)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const long long px = first + (long long)(s + u) * rows + r;
-        const bool here = live && px < last;
-        float v[VE];
-        Vec<T, VE, AL>::expand(raw[u], v);
+        for (int u = 0; u < U; u++) next[u] = V::fetch(x + u * x_step);
+      row -= per;
+      if (!FP8) out -= U * out_step;
 #pragma unroll
-        for (int e = 0; e < VE; e++) v[e] = fmaf(v[e] - mean[e], scale[e], beta[e]);
-        op_act_vec<ACT, FAST, VE>(v);
-        if constexpr (FP8)
-          store_fp8<VE, AL>(p.q, map * p.pixels + px, ch, here, v);
-        else if (here)
-          Vec<T, VE, AL>::store(out + px * p.out_stride, v);
-      }
+      for (int u = 0; u < U; u++) put(raw[u], u, live);
+#pragma unroll
+      for (int u = 0; u < U; u++) raw[u] = next[u];
     }
   });
 }

@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "fp8_sm100.cuh"
+#include "ops_launch.h"
 
 namespace iec {
 
@@ -41,56 +42,6 @@ bool on_16(const void* values, long long stride, int rows) {
   return reinterpret_cast<uintptr_t>(values) % 16 == 0 && (rows == 1 || stride * (long long)sizeof(T) % 16 == 0);
 }
 
-template <auto Kernel>
-void allow_smem(Device& dev, int bytes) {
-  static bool done[64] = {};
-  bool& d = done[dev.ordinal() & 63];
-  if (!d) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  d = true;
-}
-
-// CTAs of `Kernel` in clusters of `cluster` that the device holds at once.
-template <auto Kernel>
-int resident(Device& dev, int threads, int smem, int cluster) {
-  static int found[64] = {};
-  int& f = found[dev.ordinal() & 63];
-  if (f == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(dev.sms() / cluster * cluster));
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int clusters = 0;
-    IEC_CUDA(cudaOccupancyMaxActiveClusters(&clusters, Kernel, &cfg));
-    if (clusters < 1) throw Error(ERR_GPU, "no room for a cluster of CTAs");
-    f = std::min(clusters * cluster, dev.sms());
-  }
-  return f;
-}
-
-// launch_pdl in clusters of `cluster` CTAs along x.
-template <class... KArgs, class... Args>
-void launch_clusters(void (*kernel)(KArgs...), int grid, int threads, size_t smem, int cluster, cudaStream_t s,
-                     Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  IEC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-}
-
 template <class T, int PAIR>
 void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s) {
   using L = Fp8Smem;
@@ -114,12 +65,9 @@ void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s)
   p.tiles = p.tiles_m * p.tiles_n;
   p.div_group = FastDiv((uint32_t)(FP8_GROUP * p.tiles_n));
   p.div_rest = FastDiv((uint32_t)std::max(1, p.tiles_m % FP8_GROUP));
-  const int most = PAIR ? resident<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster) : dev.sms();
-  const int grid = std::min(p.tiles * cluster, most);
-  if (PAIR)
-    launch_clusters(kernel, grid, FP8_THREADS, (size_t)L::DYN_BYTES, cluster, s, a_map, w_map, out_map, res_map, p);
-  else
-    launch_pdl(kernel, dim3(grid), dim3(FP8_THREADS), (size_t)L::DYN_BYTES, s, a_map, w_map, out_map, res_map, p);
+  const int most = resident_ctas<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster);
+  launch_ops(kernel, dim3(std::min(p.tiles * cluster, most)), FP8_THREADS, (size_t)L::DYN_BYTES, cluster, s, a_map,
+             w_map, out_map, res_map, p);
 }
 
 template <class T>

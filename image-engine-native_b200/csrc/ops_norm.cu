@@ -4,39 +4,14 @@
 #include <numeric>
 
 #include "norm_sm100.cuh"
+#include "ops_launch.h"
 
 namespace iec {
 
 namespace {
 
 constexpr int RESIDENT_BYTES = 180 * 1024;  // of a CTA's values in shared memory
-constexpr int CLUSTER = 16;
-
-template <auto Kernel>
-void allow_smem(Device& dev, int bytes) {
-  static int most[64] = {};
-  int& m = most[dev.ordinal() & 63];
-  if (m == 0) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  if (bytes > m) IEC_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  m = std::max(m, bytes);
-}
-
-template <class... KArgs, class... Args>
-void launch(void (*kernel)(KArgs...), dim3 grid, size_t smem, int cluster, cudaStream_t s, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(NORM_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  IEC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-}
+constexpr int CLUSTER = 16, STATS_CLUSTER = 4;
 
 // The resident kernel's shape, or false where a segment outgrows a cluster.
 // A segment is the smallest run of whole groups, vectors (and with fp8 whole
@@ -78,47 +53,60 @@ template <class T, int VE, bool AL>
 void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   const int cg = p.c / p.groups;
   NormChunks q = {};
-  q.tile_c = std::min(p.c, NORM_THREADS * VE);
+  q.tile_c = std::min(p.c, APPLY_THREADS * VE);
   q.tiles = (p.c + q.tile_c - 1) / q.tile_c;
   q.slots = std::min(p.groups, (q.tile_c + cg - 2) / cg + 1);
   if (q.tiles > 65535) throw Error(ERR_INPUT, "too many channels");
-  // Maps at a time: as many as their pairs take a few MB for.
-  const int rows = std::max(1, NORM_THREADS / (std::min(q.tile_c, p.c) / VE));
-  const long long ctas = 2LL * dev.sms();  // two an SM
-  auto chunks_of = [&](long long maps) {
-    const long long want = std::max<long long>(1, ctas / (maps * q.tiles));
-    return std::max<long long>(1, std::min(want, (p.pixels + 8LL * rows - 1) / (8LL * rows)));
+  const size_t ring = VE > 1 && AL ? (size_t)NORM_RING * 4 * NORM_THREADS * 16 : 0;
+  // the ring, or the threads' statistics and (where they are many) pairs
+  const size_t stats_smem =
+      std::max(ring, (size_t)NORM_THREADS * VE * 8 + (q.slots > NORM_THREADS ? (size_t)q.slots * 8 : 0));
+  constexpr auto stats = norm_stats<T, VE, AL>;
+  allow_smem<stats>(dev, stats_smem);
+  const long long resident = resident_ctas<stats>(dev, NORM_THREADS, stats_smem, STATS_CLUSTER);
+  // CTAs of the statistics: as many as are resident, of at least eight steps
+  // each, in clusters that join their pairs. Maps at a time: as many as their pairs
+  // take 64 MB for.
+  const int rows = std::max(1, NORM_THREADS / (q.tile_c / VE));
+  auto ctas_of = [&](long long maps) {
+    const long long most = (p.pixels + 8LL * rows - 1) / (8LL * rows), room = resident / (maps * q.tiles);
+    if (most < STATS_CLUSTER || room < STATS_CLUSTER) return std::max<long long>(1, std::min(most, room));
+    return std::min((most + STATS_CLUSTER - 1) / STATS_CLUSTER, room / STATS_CLUSTER) * STATS_CLUSTER;
   };
   long long maps = p.n;
+  auto chunks_of = [&](long long n) { return (ctas_of(n) + STATS_CLUSTER - 1) / STATS_CLUSTER; };
   while (maps > 1 && maps * chunks_of(maps) * q.tiles * q.slots > (8 << 20)) maps = (maps + 1) / 2;
-  q.chunk = (p.pixels + chunks_of(maps) - 1) / chunks_of(maps);
-  q.chunks = (int)((p.pixels + q.chunk - 1) / q.chunk);
+  const long long ctas = ctas_of(maps);
+  q.cluster = (int)std::min<long long>(ctas, STATS_CLUSTER);
+  q.chunks = (int)((ctas + q.cluster - 1) / q.cluster);
+  q.span = (p.pixels + q.chunks * q.cluster - 1) / (q.chunks * q.cluster);
   q.part = static_cast<float2*>(dev.scratch((size_t)maps * q.chunks * q.tiles * q.slots * sizeof(float2), s));
-  const size_t stats_smem = (size_t)NORM_THREADS * VE * 8;
   const double values = (double)p.pixels * p.c;
   for (q.map0 = 0; q.map0 < p.n; q.map0 += (int)maps) {
     const int now = (int)std::min<long long>(maps, p.n - q.map0);
     timed_launch("norm_stats", 4 * values * now, values * now * sizeof(T), s, [&] {
-      constexpr auto kernel = norm_stats<T, VE, AL>;
-      launch(kernel, dim3(q.chunks, q.tiles, now), stats_smem, 1, s, p, q);
+      launch_ops(stats, dim3(q.chunks * q.cluster, q.tiles, now), NORM_THREADS, stats_smem, q.cluster, s, p, q);
     });
     timed_launch("norm_apply", 10 * values * now, values * now * (sizeof(T) + (p.out ? sizeof(T) : 1)), s, [&] {
-      const dim3 grid(q.chunks, q.tiles, now);
+      // two CTAs an SM, of at least eight steps
+      const int step = std::max(1, APPLY_THREADS / (std::min(q.tile_c, p.c) / VE));
+      const long long per = std::max<long long>(1, 2LL * dev.sms() / ((long long)now * q.tiles));
+      const dim3 grid((unsigned)std::min(per, (p.pixels + 8LL * step - 1) / (8LL * step)), q.tiles, now);
       const size_t smem = (size_t)q.slots * sizeof(float2);
       if (p.out) {
         constexpr auto kernel = norm_apply<T, VE, false, AL>;
-        allow_smem<kernel>(dev, (int)smem);
-        launch(kernel, grid, smem, 1, s, p, q);
+        allow_smem<kernel>(dev, smem);
+        launch_ops(kernel, grid, APPLY_THREADS, smem, 1, s, p, q);
       } else if constexpr (VE > 1) {
         constexpr auto kernel = norm_apply<T, VE, true, AL>;
-        allow_smem<kernel>(dev, (int)smem);
-        launch(kernel, grid, smem, 1, s, p, q);
+        allow_smem<kernel>(dev, smem);
+        launch_ops(kernel, grid, APPLY_THREADS, smem, 1, s, p, q);
       } else {
         constexpr auto kernel = norm_apply_fp8_odd<T>;
         const int blocks = (p.c + FP8_BLOCK - 1) / FP8_BLOCK;
-        const long long want = std::max<long long>(1, 2LL * ctas / ((long long)now * blocks));
+        const long long want = std::max<long long>(1, 4LL * dev.sms() / ((long long)now * blocks));
         const long long px = (p.pixels + NORM_THREADS / 32 - 1) / (NORM_THREADS / 32);
-        launch(kernel, dim3((unsigned)std::min(want, px), blocks, now), FP8_BLOCK * sizeof(float2), 1, s, p, q);
+        launch_ops(kernel, dim3((unsigned)std::min(want, px), blocks, now), NORM_THREADS, FP8_BLOCK * sizeof(float2), 1, s, p, q);
       }
     });
   }
@@ -131,18 +119,27 @@ void run_vectors(Device& dev, const NormSpec& p, cudaStream_t s) {
   NormResident q;
   int cluster = 1;
   size_t smem = 0;
-  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE, AL>(dev, p, s);
+  constexpr auto wide = norm_resident<T, false, AL>;
+  constexpr auto codes = norm_resident<T, true, AL>;
+  bool fits = plan_resident<T>(dev, p, fp8, &q, &cluster, &smem);
+  if (fits) {
+    // Only where all its clusters run at once: one after another, their
+    // loads, statistics and stores take turns (8 x 128 x 128 x 256 f16: 90 us
+    // in four waves of clusters of 16, 40 in chunks through L2).
+    const long long ctas = (long long)cluster * (p.c / q.seg_c) * p.n;
+    fits = ctas <= (fp8 ? resident_ctas<codes>(dev, NORM_THREADS, smem, cluster)
+                        : resident_ctas<wide>(dev, NORM_THREADS, smem, cluster));
+  }
+  if (!fits) return run_chunks<T, VE, AL>(dev, p, s);
   const double values = (double)p.n * p.pixels * p.c;
   timed_launch("norm_resident", 12 * values, values * (sizeof(T) + (fp8 ? 1 : sizeof(T))), s, [&] {
     const dim3 grid(cluster, p.c / q.seg_c, p.n);
     if (fp8) {
-      constexpr auto kernel = norm_resident<T, true, AL>;
-      allow_smem<kernel>(dev, (int)smem);
-      launch(kernel, grid, smem, cluster, s, p, q);
+      allow_smem<codes>(dev, smem);
+      launch_ops(codes, grid, NORM_THREADS, smem, cluster, s, p, q);
     } else {
-      constexpr auto kernel = norm_resident<T, false, AL>;
-      allow_smem<kernel>(dev, (int)smem);
-      launch(kernel, grid, smem, cluster, s, p, q);
+      allow_smem<wide>(dev, smem);
+      launch_ops(wide, grid, NORM_THREADS, smem, cluster, s, p, q);
     }
   });
 }

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "ops.h"
+#include "sm100.cuh"
 
 namespace iec {
 
@@ -38,52 +39,36 @@ __device__ __forceinline__ uint32_t pack_2(float lo, float hi) {
   return v;
 }
 
-// Activations. Two kinds of accuracy: FAST for results that are rounded to 16
-// bits (a few units of f32), exact to about one unit for f32 results and for
-// values that are quantised (where every unit moves more of them across a
-// rounding boundary).
-//
-// e^-v for -43.6 <= v: t = -v log2(e), 2^t by the special-function unit, and
-// for the exact kind the rounding of t put back: 2^(t + d) = 2^t (1 + d ln 2).
-// Arguments are clamped from below, where v / (1 + e^-v) is less than 1e-17
-// either way, so that two denominators multiply without overflow
-// (op_sigmoid_pair), and for the exact kind from above, where 1 + e^-v is 1.
-template <bool FAST>
-__device__ __forceinline__ float op_exp_neg(float v) {
-  v = fmaxf(v, -43.6f);
-  if (!FAST) v = fminf(v, 87.0f);
-  constexpr float L = -1.4426950408889634f, L_LO = -1.925963033500e-8f;  // log2(e) = -(L + L_LO)
-  const float t = v * L;
+// Activations, each good to a few units of f32: quantised, e4m3 codes come
+// out as often beside the nearest one as with exact exponentials (the
+// normalisation's own roundings move more of them: 230 of 67 M either way).
+__device__ __forceinline__ float op_ex2(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  if (!FAST) e = fmaf(e * 0.6931471805599453f, fmaf(v, L_LO, fmaf(v, L, -t)), e);
   return e;
 }
-
-// 1 / d; one Newton step for the exact kind.
-template <bool FAST>
 __device__ __forceinline__ float op_rcp(float d) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  if (!FAST) r = fmaf(r, fmaf(-d, r, 1.0f), r);
   return r;
 }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-template <bool FAST>
-__device__ __forceinline__ float op_sigmoid(float v) { return op_rcp<FAST>(1.0f + op_exp_neg<FAST>(v)); }
-
-// Two sigmoids by one reciprocal, of the denominators' product: the unit for
-// exponentials and reciprocals has an eighth of the multiplies' rate and
-// bounds these activations.
-template <bool FAST>
-__device__ __forceinline__ void op_sigmoid_pair(float v, float w, float* sv, float* sw) {
-  const float a = 1.0f + op_exp_neg<FAST>(v), b = 1.0f + op_exp_neg<FAST>(w), r = op_rcp<FAST>(a * b);
-  *sv = r * b;
-  *sw = r * a;
+// The sigmoids 1 / (1 + e^-v) of two values, on packed pairs (their
+// instructions bound these kernels next to memory) and with one reciprocal,
+// of the denominators' product (the unit for exponentials and reciprocals
+// has an eighth of the multiplies' rate). Arguments are clamped from below,
+// where v / (1 + e^-v) is less than 1e-17 either way, so that the product
+// does not overflow.
+__device__ __forceinline__ float2 op_sigmoid_pair(float2 v) {
+  const float2 t = fmul2(make_float2(fmaxf(v.x, -43.6f), fmaxf(v.y, -43.6f)), both(-1.4426950408889634f));
+  const float2 a = fadd2(make_float2(op_ex2(t.x), op_ex2(t.y)), both(1.0f));
+  const float r = op_rcp(a.x * a.y);
+  return make_float2(r * a.y, r * a.x);
 }
 
-// GELU for FAST, as max(v, 0) - |v| / (2 P^16) (igemm_sm100.cuh); |error| at
-// most 1.5e-7 |v|.
+// GELU as max(v, 0) - |v| / (2 P^16) (igemm_sm100.cuh), |error| at most 1.5e-7
+// |v|: a third of erff's instructions, for results of 16 bits (FAST).
 __device__ __forceinline__ float op_gelu_fast(float v) {
   const float av = fabsf(v), a = av * 0.70710678118654752f;
   float q = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(4.30638e-5f, a, 2.765672e-4f), a, 1.520143e-4f), a, 9.2705272e-3f), a,
@@ -94,7 +79,7 @@ __device__ __forceinline__ float op_gelu_fast(float v) {
   q *= q;
   q *= q;
   q *= q;
-  return fmaf(-0.5f * av, op_rcp<true>(q), fmaxf(v, 0.0f));
+  return fmaf(-0.5f * av, op_rcp(q), fmaxf(v, 0.0f));
 }
 
 // The activation of N values. The products that end an activation are not
@@ -110,16 +95,13 @@ __device__ __forceinline__ void op_act_vec(float* v) {
     for (int e = 0; e < N; e++)
       v[e] = FAST ? op_gelu_fast(v[e]) : __fmul_rn(0.5f * v[e], 1.0f + erff(v[e] * 0.70710678118654752f));
   } else if constexpr (ACT == OP_SIGMOID || ACT == OP_SILU) {
-    float s[N];
-    if constexpr (N % 2 == 0) {
 #pragma unroll
-      for (int e = 0; e < N; e += 2) op_sigmoid_pair<FAST>(v[e], v[e + 1], &s[e], &s[e + 1]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; e++) s[e] = op_sigmoid<FAST>(v[e]);
+    for (int e = 0; e < N; e += 2) {
+      const float2 x = make_float2(v[e], v[N == 1 ? e : e + 1]), s = op_sigmoid_pair(x);
+      const float2 y = ACT == OP_SILU ? fmul2(x, s) : make_float2(x.x != x.x ? x.x : s.x, x.y != x.y ? x.y : s.y);
+      v[e] = y.x;
+      if (N > 1) v[e + 1] = y.y;
     }
-#pragma unroll
-    for (int e = 0; e < N; e++) v[e] = ACT == OP_SILU ? __fmul_rn(v[e], s[e]) : v[e] != v[e] ? v[e] : s[e];
   }
 }
 
@@ -136,21 +118,34 @@ __device__ __forceinline__ void op_act_switch(int act, F&& f) {
   }
 }
 
+// max(|a|, b), NaN if one of them is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float m;
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %1;\n\tmax.NaN.f32 %0, t, %2;\n\t}" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 constexpr int FP8_BLOCK = 128;  // values along k that share a scale
 
 // The magnitudes' bits order as unsigned integers the way the magnitudes do,
 // with infinity above every finite value and NaN above infinity, so an
-// integer maximum keeps both where fmaxf would drop a NaN.
+// integer maximum keeps both.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // A block's factor (values to codes) and scale (codes to values) from its
 // largest magnitude: 448 / amax and amax / 448, or 1 and 1 below 2^-100,
 // where the factor would leave f32's range and every code rounds to zero.
+// The quotient by a reciprocal and a Newton step (the division's general
+// form took a quarter of the kernels' instructions), except where the
+// reciprocal or amax is not a normal number.
 __device__ __forceinline__ void fp8_scale(uint32_t amax_bits, float* factor, float* scale) {
   const float amax = __uint_as_float(amax_bits);
-  const bool tiny = amax < 7.888609052210118e-31f;  // 2^-100; false for NaN
-  *factor = tiny ? 1.0f : 448.0f / amax;
-  *scale = tiny ? 1.0f : amax / 448.0f;
+  *scale = amax * (1.0f / 448.0f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(amax));
+  *factor = fmaf(r, fmaf(-amax, r, 1.0f), r) * 448.0f;
+  if (!(amax <= 8.0e37f)) *factor = 448.0f / amax;  // also infinity and NaN
+  if (amax < 7.888609052210118e-31f) *factor = *scale = 1.0f;  // 2^-100
 }
 
 // Two values to two e4m3 codes (`lo` in the low byte), round to nearest
