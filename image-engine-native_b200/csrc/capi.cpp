@@ -760,7 +760,7 @@ NormSpec norm_spec(const iec_group_norm_args* a) {
   need(a, "args");
   check_dtype(a->dtype);
   check_act(a->act);
-  check_count(a->c, MAX_COLS, "channels");
+  check_count(a->c, 65535, "channels");
   check_count(a->n, 65535, "maps");
   check_count(a->pixels, MAX_ROWS, "pixels");
   if (a->n) check_count(a->pixels, MAX_ROWS / a->n, "pixels a map of the batch");

@@ -32,91 +32,8 @@
 namespace iec {
 
 constexpr int NORM_THREADS = 512;
-constexpr int NORM_RING = 3;
+constexpr int NORM_RING = 2;
 constexpr int APPLY_THREADS = 256;
-
-// VE values of T next to each other: 16 bytes where the map has a multiple
-// of them as channels (AL: its base and strides let them be read at once),
-// else one value.
-template <class T, int VE, bool AL>
-struct Vec {
-  using Raw = std::conditional_t<VE == 1, T, uint4>;
-  static __device__ __forceinline__ Raw zero() {
-    if constexpr (VE == 1)
-      return from_f32<T>(0.0f);
-    else
-      return make_uint4(0, 0, 0, 0);
-  }
-  static __device__ __forceinline__ Raw fetch(const T* p) {
-    if constexpr (VE == 1 || AL) {
-      return *reinterpret_cast<const Raw*>(p);
-    } else {
-      T v[VE];
-#pragma unroll
-      for (int e = 0; e < VE; e++) v[e] = p[e];
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4)
-          w[i] = __float_as_uint(v[i]);
-        else
-          w[i] = (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i]) |
-                 (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i + 1]) << 16;
-      }
-      return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  static __device__ __forceinline__ void expand(Raw q, float* v) {
-    if constexpr (VE == 1) {
-      v[0] = to_f32(q);
-    } else {
-      expand_16(q, v);
-    }
-  }
-  // The values of the i-th 32-bit word (VE 1: the one value).
-  static __device__ __forceinline__ void word(Raw q, int i, float* v) {
-    if constexpr (VE == 1) {
-      v[0] = to_f32(q);
-    } else {
-      const uint32_t w = i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w;
-      if constexpr (sizeof(T) == 4) {
-        v[0] = __uint_as_float(w);
-      } else {
-        const uint16_t lo = (uint16_t)(w & 0xffffu), hi = (uint16_t)(w >> 16);
-        v[0] = to_f32(reinterpret_cast<const T&>(lo));
-        v[1] = to_f32(reinterpret_cast<const T&>(hi));
-      }
-    }
-  }
-  // Channels 2 i and 2 i + 1 (VE 1: the one value, twice).
-  static __device__ __forceinline__ float2 pair(Raw q, int i) {
-    float v[2];
-    if constexpr (VE == 1) {
-      v[0] = v[1] = to_f32(q);
-    } else if constexpr (VE == 8) {
-      word(q, i, v);
-    } else {
-      word(q, 2 * i, v);
-      word(q, 2 * i + 1, v + 1);
-    }
-    return make_float2(v[0], v[1]);
-  }
-  static __device__ __forceinline__ void expand_16(uint4 q, float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) word(q, i, v + i * (VE / 4));
-  }
-  static __device__ __forceinline__ void store(T* p, const float* v) {
-    if constexpr (VE == 1 || !AL) {
-#pragma unroll
-      for (int e = 0; e < VE; e++) p[e] = from_f32<T>(v[e]);
-    } else if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      *reinterpret_cast<uint4*>(p) =
-          make_uint4(pack_2<T>(v[0], v[1]), pack_2<T>(v[2], v[3]), pack_2<T>(v[4], v[5]), pack_2<T>(v[6], v[7]));
-    }
-  }
-};
 
 // A thread's VE values of a pixel as e4m3 codes with the scale of their block
 // of 128: the block's threads are 128 / VE consecutive lanes. `live`: the
@@ -217,94 +134,139 @@ struct Running {
 };
 
 // The largest power of two, at most VE, that divides a group's channels: so
-// many of a thread's channels next to each other are of one group.
+// many (1 << shift) of a thread's channels next to each other are of one group.
 template <int VE>
-__host__ __device__ __forceinline__ int norm_run(int cg) {
-  return min(VE, cg & -cg);
+__host__ __device__ __forceinline__ int norm_shift(int cg) {
+  int s = 0;
+  while ((1 << s) < VE && cg % (2 << s) == 0) s++;
+  return s;
 }
 
-// Joins a thread's channels (each of n pixels) in runs of `run`, and stores
-// the VE / run statistics at mean[] and dev[].
-template <int VE>
-__device__ __forceinline__ void store_runs(Running<VE>& s, int run, float* mean, float* dev) {
-  const float half = 0.5f * (float)s.n;
+// Joins a thread's channels (each of n pixels) in runs of 1 << shift, and
+// stores the statistics of the VE >> shift runs at mean[] and dev[].
+template <int VE, int K>
+__device__ __forceinline__ void join_runs(Running<VE>& s, float half) {
 #pragma unroll
-  for (int k = 1; k < VE; k *= 2)
-    if (k < run)
-#pragma unroll
-      for (int e = 0; e < VE; e += 2 * k) {
-        const float x = s.mean[e] - s.mean[e + k];
-        s.dev[e] = s.dev[e] + s.dev[e + k] + x * x * (half * (float)k);
-        s.mean[e] = fmaf(-0.5f, x, s.mean[e]);
-      }
-#pragma unroll
-  for (int e = 0; e < VE; e++)
-    if (e % run == 0) {
-      mean[e / run] = s.mean[e];
-      dev[e / run] = s.dev[e];
-    }
+  for (int e = 0; e < VE; e += 2 * K) {
+    const float x = s.mean[e] - s.mean[e + K];
+    s.dev[e] = s.dev[e] + s.dev[e + K] + x * x * (half * (float)K);
+    s.mean[e] = fmaf(-0.5f, x, s.mean[e]);
+  }
 }
+template <int VE, int K>
+__device__ __forceinline__ void put_runs(const Running<VE>& s, float* mean, float* dev) {
+#pragma unroll
+  for (int e = 0; e < VE; e += K) {
+    mean[e / K] = s.mean[e];
+    dev[e / K] = s.dev[e];
+  }
+}
+template <int VE>
+__device__ __forceinline__ void store_runs(Running<VE>& s, int shift, float* mean, float* dev) {
+  const float half = 0.5f * (float)s.n;
+  if (shift == 0) return put_runs<VE, 1>(s, mean, dev);
+  if constexpr (VE > 1) {
+    join_runs<VE, 1>(s, half);
+    if (shift == 1) return put_runs<VE, 2>(s, mean, dev);
+    join_runs<VE, 2>(s, half);
+    if (shift == 2) return put_runs<VE, 4>(s, mean, dev);
+    if constexpr (VE == 8) {
+      join_runs<VE, 4>(s, half);
+      put_runs<VE, 8>(s, mean, dev);
+    }
+  }
+}
+
+// What the joining of a CTA's threads needs, found on the host (a division
+// on the device is a chain of a hundred cycles, and this code is one chain):
+// the runs of a tile, and the same of the last, shorter tile.
+struct NormJoin {
+  int rows, shift;   // rows of threads; channels of a run
+  int cg, runs[2];   // runs of a group, of a tile
+  FastDiv by_rows, by_cg, by_runs[2];
+};
+
+// Entries that join_threads keeps: shared floats, three for each.
+__host__ __device__ __forceinline__ int norm_entries(int runs) { return max(runs, NORM_THREADS); }
 
 // Joins the statistics of a CTA's threads per group: mean[r * c + ch] and
-// dev[] of the ch-th run of `run` channels over the pixels r, r + rows, ...
-// of `px` > 0 (both arrays are overwritten; c, c0 and cg count runs). Calls
-// put(group, mean, dev) in one lane for each group of cg runs that has some
-// of the runs c0 .. c0 + c - 1.
+// dev[] of the ch-th of c runs over the pixels r, r + rows, ... of `px` > 0.
+// The tile starts with run c0. `entries` takes 3 norm_entries(c) floats.
+// Calls put(group, mean, dev) in one lane for each group that has some of
+// the tile's runs.
 template <class F>
-__device__ __forceinline__ void join_threads(float* mean, float* dev, int c, int rows, int px, int c0, int cg, int run,
-                                             F&& put) {
-  __shared__ float counts[NORM_THREADS];
+__device__ __forceinline__ void join_threads(const NormJoin& q, bool last, const float* mean, const float* dev,
+                                             float* entries, int px, int c0, F&& put) {
+  const int c = q.runs[last];
+  float* emean = entries;
+  float* edev = entries + norm_entries(c);
+  float* en = entries + 2 * norm_entries(c);
   __syncthreads();
-  // First each run over the rows part, part + parts, ... ; row r has q +
-  // (r < rem) pixels.
-  const int full = min(rows, px), parts = max(1, min(NORM_THREADS / c, full));
-  const int q = px / rows, rem = px - q * rows;
-  const float k0 = (float)q, k1 = (float)(q + 1);
-  const int part = threadIdx.x / c, stride = c * parts;
+  // First each run over the rows part, part + parts, ...; row r has k0 + (r <
+  // rem) pixels. Entry ch * parts + part: a group's entries are one stretch.
+  const int full = min(q.rows, px);
+  const int part = (int)q.by_runs[last].div(threadIdx.x), ch0 = (int)threadIdx.x - part * c;
+  const int parts = max(1, min((int)q.by_runs[last].div(NORM_THREADS), full));
+  const int k0 = (int)q.by_rows.div((uint32_t)px), rem = px - k0 * q.rows;
+  const float few = (float)k0, more = (float)(k0 + 1), width = (float)(1 << q.shift);
   if (part < parts)
 #pragma unroll 1
-    for (int i = threadIdx.x; i < (c > NORM_THREADS ? c : stride); i += NORM_THREADS) {
-      const float m0 = mean[i];
+    for (int ch = ch0; ch < c; ch += parts == 1 ? NORM_THREADS : c) {
+      const float m0 = mean[part * c + ch];
       float m = 0.0f, d = 0.0f, n = 0.0f;
+      if (part + parts >= full) {  // one row
+        m = m0;
+        d = dev[part * c + ch];
+        n = part < rem ? more : few;
+      } else {
 #pragma unroll 1
-      for (int r = part, at = i; r < full; r += parts, at += stride) {
-        const float k = r < rem ? k1 : k0;
-        m = fmaf(k, mean[at] - m0, m);
-        n += k;
-      }
-      m = fmaf(m, op_rcp(n), m0);
+        for (int r = part, at = part * c + ch; r < full; r += parts, at += parts * c) {
+          const float k = r < rem ? more : few;
+          m = fmaf(k, mean[at] - m0, m);
+          n += k;
+        }
+        m = fmaf(m, op_rcp(n), m0);
 #pragma unroll 1
-      for (int r = part, at = i; r < full; r += parts, at += stride) {
-        const float x = mean[at] - m;
-        d += fmaf((r < rem ? k1 : k0) * (float)run * x, x, dev[at]);
+        for (int r = part, at = part * c + ch; r < full; r += parts, at += parts * c) {
+          const float x = mean[at] - m;
+          d += fmaf((r < rem ? more : few) * width * x, x, dev[at]);
+        }
       }
-      mean[i] = m;  // row `part`, which only this thread has read
-      dev[i] = d;
-      counts[part] = n;
+      const int to = ch * parts + part;
+      emean[to] = m;
+      edev[to] = d;
+      en[to] = n;
     }
   __syncthreads();
-  // Then a group's runs and parts, one warp a group: `per` parts of w runs
-  // at a time.
+  // Then a group's entries, one warp a group.
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
+  const int g0 = (int)q.by_cg.div((uint32_t)c0), g1 = (int)q.by_cg.div((uint32_t)(c0 + c - 1));
 #pragma unroll 1
   for (int g = g0 + warp; g <= g1; g += NORM_THREADS / 32) {
-    const int a = max(g * cg, c0) - c0, w = min((g + 1) * cg, c0 + c) - c0 - a;
-    const int per = w < 32 ? 32 / w : 1, first = w < 32 ? lane / w : 0, j0 = lane - first * w;
-    const float m0 = mean[a];
+    const int a = max(g * q.cg - c0, 0), w = min((g + 1) * q.cg - c0, c) - a;
+    const int from = a * parts + lane, to = (a + w) * parts;
+    const float m0 = emean[a * parts], inv = op_rcp((float)px * (float)w);
     float m = 0.0f, d = 0.0f;
-    if (first < per)
+    if (w * parts <= 4 * 32) {  // the usual case, from registers
+      float v[4], n[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const bool some = from + 32 * i < to;
+        v[i] = some ? emean[from + 32 * i] : m0;
+        n[i] = some ? en[from + 32 * i] : 0.0f;
+        d += some ? edev[from + 32 * i] : 0.0f;
+        m = fmaf(n[i], v[i] - m0, m);
+      }
+      m = fmaf(warp_sum(m), inv, m0);
+#pragma unroll
+      for (int i = 0; i < 4; i++) d = fmaf(n[i] * width * (v[i] - m), v[i] - m, d);
+    } else {
 #pragma unroll 1
-      for (int k = first; k < parts; k += per)
-        for (int j = j0; j < w; j += 32) m = fmaf(counts[k], mean[k * c + a + j] - m0, m);
-    m = m0 + warp_sum(m) / ((float)px * (float)w);
-    if (first < per)
+      for (int i = from; i < to; i += 32) m = fmaf(en[i], emean[i] - m0, m);
+      m = fmaf(warp_sum(m), inv, m0);
 #pragma unroll 1
-      for (int k = first; k < parts; k += per)
-        for (int j = j0; j < w; j += 32) {
-          const float x = mean[k * c + a + j] - m;
-          d += fmaf(counts[k] * (float)run * x, x, dev[k * c + a + j]);
-        }
+      for (int i = from; i < to; i += 32) d += fmaf(en[i] * width * (emean[i] - m), emean[i] - m, edev[i]);
+    }
     d = warp_sum(d);
     if (lane == 0) put(g, m, d);
   }
@@ -324,8 +286,8 @@ struct Affine {
     }
   }
   // `ch`: the first channel; stat[0] is group `g0`'s.
-  __device__ __forceinline__ void set(const float2* stat, int ch, int g0, int cg) {
-    int g = ch / cg, left = (g + 1) * cg - ch;
+  __device__ __forceinline__ void set(const float2* stat, int ch, int g0, int cg, const FastDiv& by_cg) {
+    int g = (int)by_cg.div((uint32_t)ch), left = (g + 1) * cg - ch;
 #pragma unroll
     for (int e = 0; e < VE; e++) {
       const float2 st = stat[g - g0];
@@ -352,11 +314,17 @@ struct Affine {
   }
 };
 
+// 1 / sqrt(v), within two units.
+__device__ __forceinline__ float norm_rstd(float v) { return rsqrtf(v); }
+
 // ---------------------------------------------------------------- resident
 struct NormResident {
   int seg_c, vecs, rows;  // channels of a segment, their vectors, pixels a CTA takes per step
   int slots;              // threads of a pixel: vecs, rounded up to whole blocks of 128 channels with fp8
   int pixels;             // of a CTA
+  int groups;             // of a segment
+  FastDiv by_slots, by_rows, by_cg;
+  NormJoin join;
 };
 
 template <class T, bool FP8, bool AL>
@@ -366,20 +334,21 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   extern __shared__ __align__(16) uint8_t smem[];
   const int rank = blockIdx.x, ctas = gridDim.x, seg = blockIdx.y, map = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cg = p.c / p.groups, groups = q.seg_c / cg;
-  const int steps = (q.pixels + q.rows - 1) / q.rows;
+  const int cg = q.join.cg << q.join.shift, groups = q.groups;
+  const int steps = (int)q.by_rows.div((uint32_t)(q.pixels + q.rows - 1));
   // [step][thread] vectors, the threads' statistics, the groups' statistics
   // over this CTA and their mean and rstd over the cluster.
   uint4* data = reinterpret_cast<uint4*>(smem) + threadIdx.x;
   float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * NORM_THREADS * 16);
   float* tdev = tmean + NORM_THREADS * VE;
-  float2* own = reinterpret_cast<float2*>(tdev + NORM_THREADS * VE);
-  float2* stat = own + groups;
-  const int r = threadIdx.x / q.slots, slot = threadIdx.x - r * q.slots;
+  float* entries = tdev + NORM_THREADS * VE;
+  float2* own = reinterpret_cast<float2*>(entries + 3 * norm_entries(q.join.runs[0]));
+  float2* stat = own + (groups + 1) / 2 * 2;
+  const int r = (int)q.by_slots.div(threadIdx.x), slot = (int)threadIdx.x - r * q.slots;
   const bool live = r < q.rows && slot < q.vecs;
   const int first = rank * q.pixels, px = max(0, (int)min((long long)q.pixels, p.pixels - first));
   const int ch = seg * q.seg_c + slot * VE;
-  const int n = live && r < px ? (px - r + q.rows - 1) / q.rows : 0;  // this thread's vectors
+  const int n = live && r < px ? (int)q.by_rows.div((uint32_t)(px - r + q.rows - 1)) : 0;  // this thread's vectors
   griddep_launch_dependents();
   griddep_wait();
 
@@ -410,8 +379,14 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       for (int u = 0; u < 4; u++) raw[u] = data[(i + u) * NORM_THREADS];
       run.template add<V, 4>(raw);
     }
-    if (end == n)
-      for (; i < end; i++) run.template add<V, 1>(data + i * NORM_THREADS);
+    if (end == n && i < end) {
+      const uint4 two[2] = {data[i * NORM_THREADS], data[min(i + 1, end - 1) * NORM_THREADS]};
+      if (i + 2 <= end) {
+        run.template add<V, 2>(two);
+        i += 2;
+      }
+      if (i < end) run.template add<V, 1>(data + i * NORM_THREADS);
+    }
   };
   cp_async_wait<3>();
   add_until(min(n, batch));
@@ -421,13 +396,15 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   add_until(min(n, 3 * batch));
   cp_async_wait<0>();
   add_until(n);
-  const int w = norm_run<VE>(cg), runs = q.seg_c / w;
-  if (live) store_runs<VE>(run, w, tmean + r * runs + slot * VE / w, tdev + r * runs + slot * VE / w);
+  if (live) {
+    const int at = r * q.join.runs[0] + (slot * VE >> q.join.shift);
+    store_runs<VE>(run, q.join.shift, tmean + at, tdev + at);
+  }
   if (px > 0)
-    join_threads(tmean, tdev, runs, q.rows, px, 0, cg / w, w,
+    join_threads(q.join, false, tmean, tdev, entries, px, 0,
                  [&](int g, float m, float d) { own[g] = make_float2(m, d); });
   cluster_sync();
-  const float inv = 1.0f / ((float)p.pixels * (float)cg);
+  const float inv = op_rcp((float)p.pixels * (float)cg);
 #pragma unroll 1
   for (int g = warp; g < groups; g += NORM_THREADS / 32) {
     float2 v = make_float2(0.0f, 0.0f);
@@ -440,10 +417,10 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     const float m0 = __shfl_sync(~0u, v.x, 0);  // the first CTA always has pixels
     const float m = m0 + warp_sum(k * (v.x - m0)) * inv, d = v.x - m;
     const float dev = warp_sum(fmaf(k * d, d, v.y));
-    if (lane == 0) stat[g] = make_float2(m, 1.0f / sqrtf(dev * inv + p.eps));
+    if (lane == 0) stat[g] = make_float2(m, norm_rstd(dev * inv + p.eps));
   }
   __syncthreads();
-  affine.set(stat, live ? slot * VE : 0, 0, cg);
+  affine.set(stat, live ? slot * VE : 0, 0, cg, q.by_cg);
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     // with fp8 the lanes of a block go through the shuffles together
@@ -476,6 +453,8 @@ struct NormChunks {
   int tiles, tile_c, chunks, slots, cluster;
   long long span;  // pixels of a CTA of norm_stats
   int map0;        // the first map of this launch
+  FastDiv by_cg;   // by the channels of a group
+  NormJoin join;
   float2* part;
 };
 
@@ -484,7 +463,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) norm_stats(const NormSpec p, 
   extern __shared__ __align__(16) float tmean[];  // [2][rows][channels of the tile]
   const int tile = blockIdx.y, map = q.map0 + blockIdx.z;
   const int c0 = tile * q.tile_c, c = min(q.tile_c, p.c - c0), vecs = c / VE, cg = p.c / p.groups;
-  const int r = threadIdx.x / vecs, slot = threadIdx.x - r * vecs, rows = NORM_THREADS / vecs;
+  const int rows = q.join.rows, r = threadIdx.x / vecs, slot = threadIdx.x - r * vecs;
   const long long first = blockIdx.x * q.span;
   const int px = (int)max(0ll, min(q.span, p.pixels - first));
   griddep_launch_dependents();
@@ -536,13 +515,17 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) norm_stats(const NormSpec p, 
     run.template add<V, 1>(&raw);
   }
   float* tdev = tmean + NORM_THREADS * VE;
-  const int w = norm_run<VE>(cg), runs = c / w;
-  if (r < rows) store_runs<VE>(run, w, tmean + r * runs + slot * VE / w, tdev + r * runs + slot * VE / w);
+  const bool short_tile = c < q.tile_c;
+  const int runs = q.join.runs[short_tile];
+  if (r < rows) {
+    const int at = r * runs + (slot * VE >> q.join.shift);
+    store_runs<VE>(run, q.join.shift, tmean + at, tdev + at);
+  }
+  float* entries = tdev + NORM_THREADS * VE;
+  float2* pairs = reinterpret_cast<float2*>(entries + 3 * norm_entries(runs));
   const int g0 = c0 / cg, g1 = (c0 + c - 1) / cg;
-  __shared__ float2 own[NORM_THREADS];
-  float2* const pairs = q.slots <= NORM_THREADS ? own : reinterpret_cast<float2*>(tdev + NORM_THREADS * VE);
   if (px > 0)
-    join_threads(tmean, tdev, runs, rows, px, c0 / w, cg / w, w,
+    join_threads(q.join, short_tile, tmean, tdev, entries, px, c0 >> q.join.shift,
                  [&](int g, float m, float d) { pairs[g - g0] = make_float2(m, d); });
   cluster_sync();
   const int rank = blockIdx.x % q.cluster, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -605,7 +588,7 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
       d += fmaf(n * (v.x - m), v.x - m, v.y);
     }
   }
-  return make_float2(m, 1.0f / sqrtf(warp_sum(d) / count + p.eps));
+  return make_float2(m, norm_rstd(warp_sum(d) / count + p.eps));
 }
 
 template <class T, int VE, bool FP8, bool AL>
@@ -631,7 +614,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
     if ((threadIdx.x & 31) == 0) stat[g - g0] = st;
   }
   __syncthreads();
-  affine.set(stat, ch, g0, cg);
+  affine.set(stat, ch, g0, cg, q.by_cg);
   const long long span = (p.pixels + gridDim.x - 1) / gridDim.x;
   const long long first = ((long long)gridDim.x - 1 - blockIdx.x) * span;
   const int px = (int)max(0ll, min(span, p.pixels - first));

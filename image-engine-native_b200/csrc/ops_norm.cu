@@ -11,7 +11,25 @@ namespace iec {
 namespace {
 
 constexpr int RESIDENT_BYTES = 180 * 1024;  // of a CTA's values in shared memory
-constexpr int CLUSTER = 16, STATS_CLUSTER = 4;
+constexpr int CLUSTER = 16, STATS_CLUSTER = 2;
+
+// The joining of a tile of `c` channels (and of the last one, of `c_last`)
+// over `rows` rows of threads.
+template <int VE>
+NormJoin join_shape(int cg, int c, int c_last, int rows) {
+  NormJoin j;
+  j.rows = rows;
+  j.shift = norm_shift<VE>(cg);
+  j.cg = cg >> j.shift;
+  j.by_rows = FastDiv((uint32_t)rows);
+  j.by_cg = FastDiv((uint32_t)j.cg);
+  const int tile[2] = {c, c_last};
+  for (int i = 0; i < 2; i++) {
+    j.runs[i] = tile[i] >> j.shift;
+    j.by_runs[i] = FastDiv((uint32_t)j.runs[i]);
+  }
+  return j;
+}
 
 // The resident kernel's shape, or false where a segment outgrows a cluster.
 // A segment is the smallest run of whole groups, vectors (and with fp8 whole
@@ -32,7 +50,7 @@ bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, in
   q->vecs = (int)seg / VE;
   const int lanes = fp8 ? FP8_BLOCK / VE : 1;
   q->slots = (q->vecs + lanes - 1) / lanes * lanes;
-  if (q->slots > NORM_THREADS || p.pixels > (1 << 24)) return false;
+  if (q->slots > NORM_THREADS || p.pixels > (1 << 23)) return false;
   q->rows = NORM_THREADS / q->slots;
   const int segs = p.c / q->seg_c, most_steps = RESIDENT_BYTES / (NORM_THREADS * 16);
   const long long need = (p.pixels + (long long)most_steps * q->rows - 1) / ((long long)most_steps * q->rows);
@@ -45,7 +63,13 @@ bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, in
   q->pixels = (int)((p.pixels + n - 1) / n);
   *cluster = n;
   const int steps = (q->pixels + q->rows - 1) / q->rows;
-  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 8 + (size_t)(q->seg_c / cg) * 16;
+  q->groups = q->seg_c / cg;
+  q->by_slots = FastDiv((uint32_t)q->slots);
+  q->by_rows = FastDiv((uint32_t)q->rows);
+  q->by_cg = FastDiv((uint32_t)cg);
+  q->join = join_shape<VE>(cg, q->seg_c, q->seg_c, q->rows);
+  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 8 +
+          (size_t)norm_entries(q->join.runs[0]) * 12 + (size_t)(q->groups + 1) * 16;
   return *smem <= 220 * 1024;
 }
 
@@ -58,9 +82,12 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   q.slots = std::min(p.groups, (q.tile_c + cg - 2) / cg + 1);
   if (q.tiles > 65535) throw Error(ERR_INPUT, "too many channels");
   const size_t ring = VE > 1 && AL ? (size_t)NORM_RING * 4 * NORM_THREADS * 16 : 0;
-  // the ring, or the threads' statistics and (where they are many) pairs
-  const size_t stats_smem =
-      std::max(ring, (size_t)NORM_THREADS * VE * 8 + (q.slots > NORM_THREADS ? (size_t)q.slots * 8 : 0));
+  const int c_last = p.c - (q.tiles - 1) * q.tile_c;
+  q.join = join_shape<VE>(cg, q.tile_c, c_last, NORM_THREADS / (q.tile_c / VE));
+  q.by_cg = FastDiv((uint32_t)cg);
+  // the ring, or the threads' statistics, their entries and pairs
+  const size_t stats_smem = std::max(
+      ring, (size_t)NORM_THREADS * VE * 8 + (size_t)norm_entries(q.join.runs[0]) * 12 + (size_t)(q.slots + 1) * 8);
   constexpr auto stats = norm_stats<T, VE, AL>;
   allow_smem<stats>(dev, stats_smem);
   const long long resident = resident_ctas<stats>(dev, NORM_THREADS, stats_smem, STATS_CLUSTER);
@@ -69,7 +96,7 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   // take 64 MB for.
   const int rows = std::max(1, NORM_THREADS / (q.tile_c / VE));
   auto ctas_of = [&](long long maps) {
-    const long long most = (p.pixels + 8LL * rows - 1) / (8LL * rows), room = resident / (maps * q.tiles);
+    const long long most = (p.pixels + 8LL * rows - 1) / (8LL * rows), room = std::max<long long>(resident / (maps * q.tiles), (p.pixels >> 23) + 1);
     if (most < STATS_CLUSTER || room < STATS_CLUSTER) return std::max<long long>(1, std::min(most, room));
     return std::min((most + STATS_CLUSTER - 1) / STATS_CLUSTER, room / STATS_CLUSTER) * STATS_CLUSTER;
   };

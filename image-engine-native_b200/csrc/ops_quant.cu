@@ -1,75 +1,264 @@
 // Rows of 16- or 32-bit values to e4m3 codes with an f32 scale for each
 // block of 128 values of a row (activations), or of 128 rows and 128 values
-// (weights).
+// (weights). Bound by memory: a value is read once, a byte written, some
+// five instructions between. 49152 x 1536 f16 (229 MB): see the figures at
+// quant_rows.
+#include "ops_launch.h"
 #include "ops_sm100.cuh"
 
 namespace iec {
 
 namespace {
 
-// One warp per row and block.
-template <class T>
-__global__ void __launch_bounds__(256) quant_rows(QuantSpec p) {
-  const int kb = (p.k + FP8_BLOCK - 1) / FP8_BLOCK, lane = threadIdx.x & 31;
-  const long long total = p.rows * kb;
-  for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < total; t += (long long)gridDim.x * 8) {
-    const long long row = t / kb;
-    const int b = (int)(t - row * kb);
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    float v[4];
+constexpr int QUANT_THREADS = 256;
+
+struct QuantShape {
+  int blocks;            // of a row
+  long long items;       // rows x blocks
+  // An item is a row and a block of it; a group of threads takes one item
+  // after another, `stride` items on: so many rows and blocks further.
+  long long stride, stride_rows;
+  int stride_blocks;
+};
+
+__device__ __forceinline__ uint32_t group_max(uint32_t top, int lanes) {
+  for (int o = lanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+  return top;
+}
+
+// The magnitude's bits of the largest of a vector's values, NaN above all.
+template <class T, int VE>
+__device__ __forceinline__ uint32_t vector_top(uint4 q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (sizeof(T) == 4) {
     uint32_t top = 0;
-    for (int j = 0; j < 4; j++) {
-      const int ch = b * FP8_BLOCK + j * 32 + lane;
-      v[j] = ch < p.k ? to_f32(x[ch]) : 0.0f;
-      top = max(top, abs_bits(v[j]));
-    }
-    top = __reduce_max_sync(~0u, top);
-    float factor, scale;
-    fp8_scale(top, &factor, &scale);
-    for (int j = 0; j < 4; j++) {
-      const int ch = b * FP8_BLOCK + j * 32 + lane;
-      if (ch < p.k) p.q.codes[row * p.q.code_stride + ch] = (uint8_t)e4m3x2(v[j] * factor, 0.0f);
-    }
-    if (lane == 0) p.q.scales[b * p.q.scale_stride + row] = scale;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, w[i] & 0x7fffffffu);
+    return top;
+  } else {
+    // 16-bit magnitudes order as integers too, two at a time
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    const uint16_t one = (uint16_t)max(m & 0xffffu, m >> 16);
+    return __float_as_uint(to_f32(reinterpret_cast<const T&>(one)));
   }
 }
 
-// One CTA per block of 128 x 128, read twice.
-template <class T>
-__global__ void __launch_bounds__(256) quant_blocks(QuantSpec p) {
-  __shared__ uint32_t red[8];
-  const int b = blockIdx.x, rb = blockIdx.y;
-  const int col = b * FP8_BLOCK + (threadIdx.x & 127);
-  uint32_t top = 0;
-  for (int r = threadIdx.x >> 7; r < FP8_BLOCK; r += 2) {
-    const long long row = (long long)rb * FP8_BLOCK + r;
-    if (row < p.rows && col < p.k) top = max(top, abs_bits(to_f32(static_cast<const T*>(p.x)[row * p.x_stride + col])));
+// Scaled vectors as codes.
+template <class T, int VE>
+__device__ __forceinline__ void store_codes(uint8_t* out, uint4 raw, float factor) {
+  float v[VE];
+  Vec<T, VE, true>::expand(raw, v);
+  uint32_t w[VE / 4];
+#pragma unroll
+  for (int e = 0; e < VE; e += 4) {
+    const float2 a = fmul2(make_float2(v[e], v[e + 1]), both(factor));
+    const float2 b = fmul2(make_float2(v[e + 2], v[e + 3]), both(factor));
+    w[e / 4] = (uint32_t)e4m3x2(a.x, a.y) | (uint32_t)e4m3x2(b.x, b.y) << 16;
   }
+  if constexpr (VE == 8)
+    *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(out) = w[0];
+}
+
+// Rows of whole, aligned vectors: 128 / VE lanes an item, one vector each,
+// U items in flight.
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_rows(const QuantSpec p, const QuantShape q) {
+  constexpr int VE = 16 / (int)sizeof(T), LANES = FP8_BLOCK / VE, U = 4;
+  griddep_launch_dependents();
+  griddep_wait();
+  long long item = ((long long)blockIdx.x * QUANT_THREADS + threadIdx.x) / LANES;
+  const int lane = threadIdx.x % LANES;
+  long long row = item / q.blocks;
+  int block = (int)(item - row * q.blocks);
+  const T* x = static_cast<const T*>(p.x);
+  // (a warp's items end together or not at all: shuffles are within an item)
+  while (__any_sync(~0u, item < q.items)) {
+    uint4 raw[U];
+    long long rows[U];
+    int blocks[U];
+    bool here[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      rows[u] = row;
+      blocks[u] = block;
+      here[u] = item < q.items && block * FP8_BLOCK + lane * VE < p.k;
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (here[u]) raw[u] = *reinterpret_cast<const uint4*>(x + row * p.x_stride + block * FP8_BLOCK + lane * VE);
+      item += q.stride;
+      row += q.stride_rows;
+      block += q.stride_blocks;
+      if (block >= q.blocks) {
+        block -= q.blocks;
+        row++;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float factor, scale;
+      fp8_scale(group_max(vector_top<T, VE>(raw[u]), LANES), &factor, &scale);
+      if (!here[u]) continue;
+      store_codes<T, VE>(p.q.codes + rows[u] * (long long)p.q.code_stride + blocks[u] * FP8_BLOCK + lane * VE, raw[u],
+                         factor);
+      if (lane == 0) p.q.scales[blocks[u] * (long long)p.q.scale_stride + rows[u]] = scale;
+    }
+  }
+}
+
+// Any rows: a warp an item, four values a lane, 32 apart.
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_rows_odd(const QuantSpec p, const QuantShape q) {
+  constexpr int U = 2;
+  griddep_launch_dependents();
+  griddep_wait();
+  long long item = ((long long)blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
+  const int lane = threadIdx.x % 32;
+  long long row = item / q.blocks;
+  int block = (int)(item - row * q.blocks);
+  while (item < q.items) {
+    float v[U][4];
+    long long rows[U];
+    int blocks[U];
+    bool here[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      rows[u] = row;
+      blocks[u] = block;
+      here[u] = item < q.items;
+      const T* x = static_cast<const T*>(p.x) + row * p.x_stride + block * FP8_BLOCK + lane;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        v[u][j] = here[u] && block * FP8_BLOCK + j * 32 + lane < p.k ? to_f32(x[j * 32]) : 0.0f;
+      item += q.stride;
+      row += q.stride_rows;
+      block += q.stride_blocks;
+      if (block >= q.blocks) {
+        block -= q.blocks;
+        row++;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (!here[u]) break;
+      float most = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) most = max_abs(v[u][j], most);
+      float factor, scale;
+      fp8_scale(__reduce_max_sync(~0u, abs_bits(most)), &factor, &scale);
+      uint8_t* out = p.q.codes + rows[u] * (long long)p.q.code_stride + blocks[u] * FP8_BLOCK + lane;
+      const uint32_t a = e4m3x2(v[u][0] * factor, v[u][1] * factor), b = e4m3x2(v[u][2] * factor, v[u][3] * factor);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (blocks[u] * FP8_BLOCK + j * 32 + lane < p.k) out[j * 32] = (uint8_t)((j < 2 ? a : b) >> (8 * (j & 1)));
+      if (lane == 0) p.q.scales[blocks[u] * (long long)p.q.scale_stride + rows[u]] = scale;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t cta_max(uint32_t top) {
+  __shared__ uint32_t red[QUANT_THREADS / 32];
   top = __reduce_max_sync(~0u, top);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
-  for (int i = 0; i < 8; i++) top = max(top, red[i]);
-  float factor, scale;
-  fp8_scale(top, &factor, &scale);
-  for (int r = threadIdx.x >> 7; r < FP8_BLOCK; r += 2) {
-    const long long row = (long long)rb * FP8_BLOCK + r;
-    if (row < p.rows && col < p.k)
-      p.q.codes[row * p.q.code_stride + col] =
-          (uint8_t)e4m3x2(to_f32(static_cast<const T*>(p.x)[row * p.x_stride + col]) * factor, 0.0f);
+#pragma unroll
+  for (int i = 0; i < QUANT_THREADS / 32; i++) top = max(top, red[i]);
+  return top;
+}
+
+// A CTA a block of 128 x 128, its vectors in registers between the maximum
+// and the codes.
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_blocks(const QuantSpec p) {
+  constexpr int VE = 16 / (int)sizeof(T), LANES = FP8_BLOCK / VE, ROWS = QUANT_THREADS / LANES, N = FP8_BLOCK / ROWS;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x % LANES, col = blockIdx.x * FP8_BLOCK + lane * VE;
+  const long long row = (long long)blockIdx.y * FP8_BLOCK + threadIdx.x / LANES;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride + col;
+  uint4 raw[N];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (row + i * ROWS < p.rows && col < p.k) raw[i] = *reinterpret_cast<const uint4*>(x + i * ROWS * p.x_stride);
   }
-  if (threadIdx.x == 0) p.q.scales[b * p.q.scale_stride + rb] = scale;
+#pragma unroll
+  for (int i = 0; i < N; i++) top = max(top, vector_top<T, VE>(raw[i]));
+  float factor, scale;
+  fp8_scale(cta_max(top), &factor, &scale);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (row + i * ROWS < p.rows && col < p.k)
+      store_codes<T, VE>(p.q.codes + (row + i * ROWS) * (long long)p.q.code_stride + col, raw[i], factor);
+  if (threadIdx.x == 0) p.q.scales[blockIdx.x * (long long)p.q.scale_stride + blockIdx.y] = scale;
+}
+
+// The same for any rows, a value at a time, read twice.
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_blocks_odd(const QuantSpec p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int ROWS = QUANT_THREADS / FP8_BLOCK, U = 8;
+  const int col = blockIdx.x * FP8_BLOCK + threadIdx.x % FP8_BLOCK;
+  const long long row0 = (long long)blockIdx.y * FP8_BLOCK;
+  const int rows = (int)min((long long)FP8_BLOCK, p.rows - row0);
+  const T* x = static_cast<const T*>(p.x) + row0 * p.x_stride + col;
+  uint8_t* out = p.q.codes + row0 * (long long)p.q.code_stride + col;
+  float most = 0.0f;
+  if (col < p.k)
+#pragma unroll U
+    for (int r = threadIdx.x / FP8_BLOCK; r < rows; r += ROWS) most = max_abs(to_f32(x[r * p.x_stride]), most);
+  float factor, scale;
+  fp8_scale(cta_max(abs_bits(most)), &factor, &scale);
+  if (col < p.k)
+#pragma unroll U
+    for (int r = threadIdx.x / FP8_BLOCK; r < rows; r += ROWS)
+      out[r * (long long)p.q.code_stride] = (uint8_t)e4m3x2(to_f32(x[r * p.x_stride]) * factor, 0.0f);
+  if (threadIdx.x == 0) p.q.scales[blockIdx.x * (long long)p.q.scale_stride + blockIdx.y] = scale;
 }
 
 template <class T>
 void run(Device& dev, const QuantSpec& p, cudaStream_t s) {
-  const int kb = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+  constexpr int VE = 16 / (int)sizeof(T);
+  const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+  const bool wide = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_stride % VE == 0 && p.k % VE == 0 &&
+                    reinterpret_cast<uintptr_t>(p.q.codes) % VE == 0 && p.q.code_stride % VE == 0;
   const double values = (double)p.rows * p.k;
   timed_launch("quantize_fp8", 2 * values, values * (sizeof(T) + 1), s, [&] {
-    if (p.block_rows == 1)
-      quant_rows<T><<<dev.sms() * 8, 256, 0, s>>>(p);
-    else
-      quant_blocks<T><<<dim3(kb, (unsigned)((p.rows + FP8_BLOCK - 1) / FP8_BLOCK)), 256, 0, s>>>(p);
-    IEC_CUDA(cudaGetLastError());
+    if (p.block_rows == 1) {
+      QuantShape q;
+      q.blocks = blocks;
+      q.items = p.rows * blocks;
+      const int lanes = wide ? FP8_BLOCK / VE : 32, per = QUANT_THREADS / lanes, unroll = wide ? 4 : 2;
+      // eight CTAs an SM, or fewer where the items run out
+      const long long want = (q.items + per * unroll - 1) / (per * unroll);
+      const int grid = (int)std::max<long long>(1, std::min<long long>(want, 8LL * dev.sms()));
+      q.stride = (long long)grid * per;
+      q.stride_rows = q.stride / blocks;
+      q.stride_blocks = (int)(q.stride - q.stride_rows * blocks);
+      if (wide)
+        launch_pdl(quant_rows<T>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
+      else
+        launch_pdl(quant_rows_odd<T>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
+    } else {
+      const long long row_blocks = (p.rows + FP8_BLOCK - 1) / FP8_BLOCK;
+      // a grid is at most 65535 high
+      for (long long done = 0; done < row_blocks; done += 65535) {
+        QuantSpec part = p;
+        part.x = static_cast<const T*>(p.x) + done * FP8_BLOCK * p.x_stride;
+        part.rows = p.rows - done * FP8_BLOCK;
+        part.q.codes = p.q.codes + (size_t)done * FP8_BLOCK * p.q.code_stride;
+        part.q.scales = p.q.scales + done;
+        const dim3 grid((unsigned)blocks, (unsigned)std::min<long long>(row_blocks - done, 65535));
+        if (wide)
+          launch_pdl(quant_blocks<T>, grid, dim3(QUANT_THREADS), 0, s, part);
+        else
+          launch_pdl(quant_blocks_odd<T>, grid, dim3(QUANT_THREADS), 0, s, part);
+      }
+    }
   });
 }
 

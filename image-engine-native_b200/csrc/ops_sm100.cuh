@@ -155,4 +155,87 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// VE values of T next to each other: 16 bytes where the map has a multiple
+// of them as channels (AL: its base and strides let them be read at once),
+// else one value.
+template <class T, int VE, bool AL>
+struct Vec {
+  using Raw = std::conditional_t<VE == 1, T, uint4>;
+  static __device__ __forceinline__ Raw zero() {
+    if constexpr (VE == 1)
+      return from_f32<T>(0.0f);
+    else
+      return make_uint4(0, 0, 0, 0);
+  }
+  static __device__ __forceinline__ Raw fetch(const T* p) {
+    if constexpr (VE == 1 || AL) {
+      return *reinterpret_cast<const Raw*>(p);
+    } else {
+      T v[VE];
+#pragma unroll
+      for (int e = 0; e < VE; e++) v[e] = p[e];
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4)
+          w[i] = __float_as_uint(v[i]);
+        else
+          w[i] = (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i]) |
+                 (uint32_t) reinterpret_cast<const uint16_t&>(v[2 * i + 1]) << 16;
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  static __device__ __forceinline__ void expand(Raw q, float* v) {
+    if constexpr (VE == 1) {
+      v[0] = to_f32(q);
+    } else {
+      expand_16(q, v);
+    }
+  }
+  // The values of the i-th 32-bit word (VE 1: the one value).
+  static __device__ __forceinline__ void word(Raw q, int i, float* v) {
+    if constexpr (VE == 1) {
+      v[0] = to_f32(q);
+    } else {
+      const uint32_t w = i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w;
+      if constexpr (sizeof(T) == 4) {
+        v[0] = __uint_as_float(w);
+      } else {
+        const uint16_t lo = (uint16_t)(w & 0xffffu), hi = (uint16_t)(w >> 16);
+        v[0] = to_f32(reinterpret_cast<const T&>(lo));
+        v[1] = to_f32(reinterpret_cast<const T&>(hi));
+      }
+    }
+  }
+  // Channels 2 i and 2 i + 1 (VE 1: the one value, twice).
+  static __device__ __forceinline__ float2 pair(Raw q, int i) {
+    float v[2];
+    if constexpr (VE == 1) {
+      v[0] = v[1] = to_f32(q);
+    } else if constexpr (VE == 8) {
+      word(q, i, v);
+    } else {
+      word(q, 2 * i, v);
+      word(q, 2 * i + 1, v + 1);
+    }
+    return make_float2(v[0], v[1]);
+  }
+  static __device__ __forceinline__ void expand_16(uint4 q, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) word(q, i, v + i * (VE / 4));
+  }
+  static __device__ __forceinline__ void store(T* p, const float* v) {
+    if constexpr (VE == 1 || !AL) {
+#pragma unroll
+      for (int e = 0; e < VE; e++) p[e] = from_f32<T>(v[e]);
+    } else if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      *reinterpret_cast<uint4*>(p) =
+          make_uint4(pack_2<T>(v[0], v[1]), pack_2<T>(v[2], v[3]), pack_2<T>(v[4], v[5]), pack_2<T>(v[6], v[7]));
+    }
+  }
+};
+
 }  // namespace iec
