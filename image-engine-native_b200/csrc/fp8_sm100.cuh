@@ -10,10 +10,12 @@
 // lane quarter holds row t, so the scale of a is one register and that of w
 // is the same for all its columns.
 //
-// fp8_gemm_sm100<T, PAIR>: PAIR = 1 takes tiles of 256 x 256 by two CTAs of a
+// fp8_gemm_sm100<T, MODE>: FP8_PAIR takes tiles of 256 x 256 by two CTAs of a
 // cluster (cta_group::2: each loads its 128 rows of a and half the rows of w
-// and holds its rows' accumulators), 0 tiles of 128 x 128 by one. Persistent
-// CTAs of 12 warps walk the tiles: warp 0 loads (TMA, 128-byte swizzle), warp
+// and holds its rows' accumulators), FP8_SINGLE tiles of 128 x 128 by one;
+// FP8_SPLIT, for few tiles, has the CTAs of a cluster take a stretch of k
+// each of one 128 x 128 tile and add up their sums through distributed shared
+// memory, always in the same order. CTAs of 12 warps walk the tiles: warp 0 loads (TMA, 128-byte swizzle), warp
 // 1 issues the MMAs, warps 4..11 (two per TMEM lane quarter, half the columns
 // each) scale and add the blocks and write the tile; they take the registers
 // that the others give up (setmaxnreg), 128 of them for the sums of a row's
@@ -40,8 +42,11 @@ struct Fp8Params {
   void* out;
   long long residual_stride, out_stride;
   int tma_out;  // out and residual have tensor maps
+  int splits, split_blocks;  // FP8_SPLIT: CTAs of a tile, blocks along k of one
   int* dev_err;
 };
+
+enum Fp8Mode { FP8_SINGLE = 0, FP8_PAIR = 1, FP8_SPLIT = 2 };
 
 constexpr int FP8_THREADS = 384;
 constexpr int FP8_EPI_WARPS = 8;
@@ -108,12 +113,13 @@ __device__ __noinline__ void fp8_load_boxes(uint8_t* dst, const CUtensorMap* map
   for (int b = 0; b < BOXES; b++) tma_load_2d(dst + b * 4096, map, bar, col + b * BOX_COLS, row);
 }
 
-template <class T, int PAIR>
+template <class T, int MODE>
 __global__ void __launch_bounds__(FP8_THREADS, 1)
     fp8_gemm_sm100(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap w_map,
                    const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
                    const Fp8Params p) {
   using L = Fp8Smem;
+  constexpr bool PAIR = MODE == FP8_PAIR, SPLIT = MODE == FP8_SPLIT;
   constexpr int BM = PAIR ? 256 : 128, BN = BM, CW = BN / 2;  // CW: columns of a thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -126,8 +132,16 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0;
-  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const uint32_t split = SPLIT ? cluster_rank() : 0;
+  const int first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / p.splits : blockIdx.x;
+  const int step = PAIR ? gridDim.x >> 1 : SPLIT ? p.tiles : gridDim.x;
+  const int kb0 = SPLIT ? min((int)split * p.split_blocks, p.kblocks) : 0;
+  const int kb1 = SPLIT ? min(kb0 + p.split_blocks, p.kblocks) : p.kblocks;
 
+  if (threadIdx.x == 64 && p.kblocks) {
+    prefetch_tensor_map(&a_map);
+    prefetch_tensor_map(&w_map);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::NSTAGE; s++) {
       mbar_init(&full[s], 1);
@@ -168,7 +182,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         int mt, nt;
         fp8_tile(p, tile, &mt, &nt);
         const int row = mt * BM + (int)rank * 128, col = nt * BN + (int)rank * 128;
-        for (int kb = 0; kb < p.kblocks; kb++) {
+        for (int kb = kb0; kb < kb1; kb++) {
           if (!mbar_wait(&empty[s], phase ^ 1, abort_flag, p.dev_err, DEV_ERR_WAIT_EMPTY)) {
             ok = false;
             break;
@@ -204,7 +218,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first; tile < p.tiles && ok; tile += step)
-        for (int kb = 0; kb < p.kblocks; kb++, i++) {
+        for (int kb = kb0; kb < kb1; kb++, i++) {
           ok = __all_sync(~0u, mbar_wait(&full[s], phase, abort_flag, p.dev_err, DEV_ERR_WAIT_FULL));
           if (!ok) break;
           const int a = i & 1;
@@ -273,7 +287,9 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       col0 = nt * BN + part * CW;
       sa = p.a_scales + min(row0 + lane, p.m - 1);
       sw = p.w_scales + min(col0, p.n - 1) / FP8_BLOCK;
-      if (p.kblocks) {
+      if (kb0 < kb1) {
+        sa += kb0 * p.a_scale_stride;
+        sw += kb0 * p.w_scale_stride;
         sa_next = *sa;
         sw_next = *sw;
       }
@@ -294,10 +310,10 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       uint64_t acc[CW / 2];  // f32 pairs
 #pragma unroll
       for (int c = 0; c < CW / 2; c++) acc[c] = 0;
-      for (int kb = 0; kb < p.kblocks; kb++, i++) {
+      for (int kb = kb0; kb < kb1; kb++, i++) {
         const float s1 = sa_next * sw_next;
         const uint64_t s2 = pack_f32x2(s1, s1);
-        if (kb + 1 < p.kblocks) {
+        if (kb + 1 < kb1) {
           sa += p.a_scale_stride;
           sw += p.w_scale_stride;
           sa_next = *sa;
@@ -312,9 +328,13 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         tc_fence_after();
         const uint32_t t = lanes + (uint32_t)(a * BN);
         uint32_t r[2][16];
-        tmem_ld16(t, r[0]);
+        // Rows past the last only hand the accumulator back. (Looked at only
+        // where there are few rows: the test takes registers.)
+        const bool work = MODE == FP8_SPLIT ? any : true;
+        if (work) tmem_ld16(t, r[0]);
 #pragma unroll
         for (int c = 0; c < CW / 16; c++) {
+          if (!work && c + 1 < CW / 16) continue;
           tmem_wait_ld();
           if (c + 1 < CW / 16) {
             tmem_ld16(t + (uint32_t)(16 * (c + 1)), r[(c + 1) & 1]);
@@ -328,14 +348,22 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
             }
           }
 #pragma unroll
-          for (int q = 0; q < 8; q++) ffma2_acc(acc[c * 8 + q], r[c & 1][2 * q], r[c & 1][2 * q + 1], s2);
+          for (int q = 0; q < 8; q++)
+            if (work) ffma2_acc(acc[c * 8 + q], r[c & 1][2 * q], r[c & 1][2 * q + 1], s2);
         }
         // The residual, once the last tile has left the patch: behind the
         // first block, so that the wait for the patch delays nothing.
-        if (kb == 0 && p.tma_out && p.residual && any && lane == 0) {
+        if (!SPLIT && kb == 0 && p.tma_out && p.residual && any && lane == 0) {
           bulk_wait_read();
           load_residual(row_t, col_t, 0);
         }
+      }
+      if constexpr (SPLIT) {
+        // This CTA's sums as pairs, pair q of row `lane` at q ^ lane.
+        float2* mine = reinterpret_cast<float2*>(patch);
+#pragma unroll
+        for (int q = 0; q < CW / 2; q++) mine[lane * (CW / 2) + (q ^ lane)] = unpack_f32x2(acc[q]);
+        break;
       }
       if (!ok) break;
       if (tile + step < p.tiles) enter_tile(tile + step);  // its first scales and bias are on their way
@@ -444,15 +472,67 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       });
       __syncwarp();  // the patch is read
     }
+    if constexpr (SPLIT) {
+      cluster_sync();  // every CTA's sums are in its shared memory
+      // The warps of the cluster take the tile's rows' halves in turn: two
+      // columns a lane, the CTAs' sums added in their order.
+      int mt, nt;
+      fp8_tile(p, first, &mt, &nt);
+      const int rows = min(128, p.m - mt * 128);
+      op_act_switch(p.act, [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
+        constexpr int U = 4;  // of them at a time, for their loads to overlap
+        const int stride = p.splits * FP8_EPI_WARPS;
+#pragma unroll 1
+        for (int h0 = (int)split * FP8_EPI_WARPS + e; ok && h0 < 2 * rows; h0 += U * stride) {
+          float2 sum[U], more[U];
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            const int h = h0 + u * stride, col = nt * 128 + (h & 1) * 64 + 2 * lane;
+            const bool one = h < 2 * rows && col < p.n, two = one && col + 1 < p.n;
+            sum[u] = make_float2(one && p.bias ? p.bias[col] : 0.0f, two && p.bias ? p.bias[col + 1] : 0.0f);
+            more[u] = make_float2(0.0f, 0.0f);
+            if (p.residual) {
+              const T* res = static_cast<const T*>(p.residual) + (mt * 128 + (h >> 1)) * p.residual_stride + col;
+              if (one) more[u].x = to_f32(res[0]);
+              if (two) more[u].y = to_f32(res[1]);
+            }
+          }
+#pragma unroll 2
+          for (int k = 0; k < p.splits; k++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+              const int h = min(h0 + u * stride, 2 * rows - 1), r = h >> 1;
+              const uint8_t* at = smem + L::OUT_OFF + ((h & 1) * 4 + (r >> 5)) * L::OUT_WARP;
+              const float2* from = reinterpret_cast<const float2*>(at) + (r & 31) * (CW / 2) + (lane ^ (r & 31));
+              sum[u] = fadd2(sum[u], ld_cluster_f32x2(from, (uint32_t)k));
+            }
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            const int h = h0 + u * stride, col = nt * 128 + (h & 1) * 64 + 2 * lane;
+            float v[2] = {sum[u].x, sum[u].y};
+            op_act_vec<ACT, true, 2>(v);
+            if (p.residual) {
+              v[0] += more[u].x;
+              v[1] += more[u].y;
+            }
+            T* out = static_cast<T*>(p.out) + (mt * 128 + (h >> 1)) * p.out_stride + col;
+            if (h < 2 * rows && col < p.n) out[0] = from_f32<T>(v[0]);
+            if (h < 2 * rows && col + 1 < p.n) out[1] = from_f32<T>(v[1]);
+          }
+        }
+      });
+    }
     if (lane == 0) {
       bulk_wait();
       // after an abort: a residual still on its way lands first
       if (res_flying) mbar_wait(&res_full[e], res_phase, abort_flag, p.dev_err, 0);
     }
   }
+  if (SPLIT && warp < 4) cluster_sync();  // (of the epilogue's first one above)
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync();  // nothing of the other CTA is in flight to this one
+  if (PAIR || SPLIT) cluster_sync();  // nothing of another CTA is in flight to this one, or reads it
   if (warp == 1) {
     if (PAIR)
       tmem_dealloc_pair(tmem_base, 2 * BN);

@@ -76,12 +76,6 @@ template <int LEFT>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
-__device__ __forceinline__ float2 ld_cluster_f32x2(const float2* p, uint32_t rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(p, rank)) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);

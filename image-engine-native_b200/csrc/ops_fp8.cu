@@ -42,18 +42,20 @@ bool on_16(const void* values, long long stride, int rows) {
   return reinterpret_cast<uintptr_t>(values) % 16 == 0 && (rows == 1 || stride * (long long)sizeof(T) % 16 == 0);
 }
 
-template <class T, int PAIR>
+template <class T, int MODE>
 void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s) {
   using L = Fp8Smem;
-  constexpr auto kernel = fp8_gemm_sm100<T, PAIR>;
-  constexpr int edge = PAIR ? 256 : 128, cluster = PAIR ? 2 : 1;
+  constexpr auto kernel = fp8_gemm_sm100<T, MODE>;
+  constexpr int edge = MODE == FP8_PAIR ? 256 : 128;
+  const int cluster = MODE == FP8_PAIR ? 2 : p.splits;
   allow_smem<kernel>(dev, L::DYN_BYTES);
   CUtensorMap a_map = {}, w_map = {}, out_map = {}, res_map = {};
   if (q.k) {
     a_map = code_map(q.a, q.a_stride, q.m, q.k, 128);
     w_map = code_map(q.w, q.w_stride, q.n, q.k, 128);
   }
-  p.tma_out = on_16<T>(q.out, q.out_stride, q.m) && (!q.residual || on_16<T>(q.residual, q.residual_stride, q.m));
+  p.tma_out = MODE != FP8_SPLIT && on_16<T>(q.out, q.out_stride, q.m) &&
+              (!q.residual || on_16<T>(q.residual, q.residual_stride, q.m));
   if (p.tma_out) {
     out_map = value_map<T>(q.out, q.out_stride, q.m, q.n);
     if (q.residual) res_map = value_map<T>(q.residual, q.residual_stride, q.m, q.n);
@@ -65,9 +67,20 @@ void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s)
   p.tiles = p.tiles_m * p.tiles_n;
   p.div_group = FastDiv((uint32_t)(FP8_GROUP * p.tiles_n));
   p.div_rest = FastDiv((uint32_t)std::max(1, p.tiles_m % FP8_GROUP));
-  const int most = resident_ctas<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster);
-  launch_ops(kernel, dim3(std::min(p.tiles * cluster, most)), FP8_THREADS, (size_t)L::DYN_BYTES, cluster, s, a_map,
-             w_map, out_map, res_map, p);
+  int grid = p.tiles * cluster;
+  if (MODE != FP8_SPLIT) grid = std::min(grid, resident_ctas<kernel>(dev, FP8_THREADS, L::DYN_BYTES, cluster));
+  launch_ops(kernel, dim3(grid), FP8_THREADS, (size_t)L::DYN_BYTES, cluster, s, a_map, w_map, out_map, res_map, p);
+}
+
+// CTAs that share a tile's blocks along k: where the tiles leave at least
+// half the SMs idle, as many as fill them, of at least two blocks each.
+template <class T>
+int splits_of(Device& dev, int tiles, int kblocks) {
+  constexpr auto kernel = fp8_gemm_sm100<T, FP8_SPLIT>;
+  int n = std::min({16, dev.sms() / std::max(tiles, 1), kblocks / 2});
+  // clusters that do not all run at once would take turns
+  while (n > 1 && resident_ctas<kernel>(dev, FP8_THREADS, Fp8Smem::DYN_BYTES, n) < tiles * n) n--;
+  return std::max(n, 1);
 }
 
 template <class T>
@@ -89,14 +102,19 @@ void run(Device& dev, const Fp8MatmulSpec& q, cudaStream_t s) {
   p.dev_err = dev.dev_err();
   const double m = q.m, n = q.n, k = q.k;
   const long long pairs = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256);
-  const bool pair = pairs * 2 >= dev.sms();
+  const long long tiles = (long long)((q.m + 127) / 128) * ((q.n + 127) / 128);
+  p.splits = tiles * 2 <= dev.sms() ? splits_of<T>(dev, (int)tiles, p.kblocks) : 1;
+  p.split_blocks = (p.kblocks + p.splits - 1) / p.splits;
+  const int mode = pairs * 2 >= dev.sms() ? FP8_PAIR : p.splits > 1 ? FP8_SPLIT : FP8_SINGLE;
   char name[96] = "";
-  if (dev.timing()) snprintf(name, sizeof name, "fp8_gemm_sm100<%d> %dx%dx%d", pair ? 1 : 0, q.m, q.n, q.k);
+  if (dev.timing()) snprintf(name, sizeof name, "fp8_gemm_sm100<%d> %dx%dx%d", mode, q.m, q.n, q.k);
   timed_launch(name, 2 * m * n * k, m * k + n * k + m * n * sizeof(T) * (q.residual ? 2 : 1), s, [&] {
-    if (pair)
-      run_tiles<T, 1>(dev, q, p, s);
+    if (mode == FP8_PAIR)
+      run_tiles<T, FP8_PAIR>(dev, q, p, s);
+    else if (mode == FP8_SPLIT)
+      run_tiles<T, FP8_SPLIT>(dev, q, p, s);
     else
-      run_tiles<T, 0>(dev, q, p, s);
+      run_tiles<T, FP8_SINGLE>(dev, q, p, s);
   });
 }
 
