@@ -101,11 +101,17 @@ void run(Device& dev, const Fp8MatmulSpec& q, cudaStream_t s) {
   p.out_stride = q.out_stride;
   p.dev_err = dev.dev_err();
   const double m = q.m, n = q.n, k = q.k;
+  // The least rounds of 128 x 128 outputs an SM: pairs of CTAs take two at a
+  // time, at 1.3 times the rate (9472 x 2048 x 1024, whole rounds either way:
+  // 31 us in pairs, 39 in single tiles; 4096 x 1536 x 384, four rounds in
+  // pairs and three single: 16.9 and 15.2 us).
+  const int sms = dev.sms();
   const long long pairs = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256);
   const long long tiles = (long long)((q.m + 127) / 128) * ((q.n + 127) / 128);
-  p.splits = tiles * 2 <= dev.sms() ? splits_of<T>(dev, (int)tiles, p.kblocks) : 1;
+  p.splits = tiles * 2 <= sms ? splits_of<T>(dev, (int)tiles, p.kblocks) : 1;
   p.split_blocks = (p.kblocks + p.splits - 1) / p.splits;
-  const int mode = pairs * 2 >= dev.sms() ? FP8_PAIR : p.splits > 1 ? FP8_SPLIT : FP8_SINGLE;
+  const long long by_pairs = 2 * ((pairs + sms / 2 - 1) / (sms / 2)), by_tiles = (tiles + sms - 1) / sms;
+  const int mode = p.splits > 1 ? FP8_SPLIT : 10 * by_pairs <= 13 * by_tiles ? FP8_PAIR : FP8_SINGLE;
   char name[96] = "";
   if (dev.timing()) snprintf(name, sizeof name, "fp8_gemm_sm100<%d> %dx%dx%d", mode, q.m, q.n, q.k);
   timed_launch(name, 2 * m * n * k, m * k + n * k + m * n * sizeof(T) * (q.residual ? 2 : 1), s, [&] {
