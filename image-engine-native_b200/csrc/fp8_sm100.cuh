@@ -104,6 +104,47 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
+// A row of a patch's box (128 bytes: 128 / sizeof(T) columns from `col`) to or
+// from global memory at `row`, by one warp, wherever the row starts: a lane
+// takes one 32-bit word, and where the row's words straddle global memory's,
+// the halves of two lanes' words.
+__device__ __forceinline__ uint32_t* fp8_word(uint8_t* box, int r, int lane) {
+  return reinterpret_cast<uint32_t*>(box + r * 128 + ((((lane >> 2) ^ r) & 7) << 4) + (lane & 3) * 4);
+}
+template <class T>
+__device__ __forceinline__ void fp8_drain_row(uint8_t* box, int r, int lane, T* row, int col, int n) {
+  const uint32_t word = *fp8_word(box, r, lane);
+  if constexpr (sizeof(T) == 4) {
+    if (col + lane < n) reinterpret_cast<uint32_t*>(row)[col + lane] = word;
+  } else {
+    uint16_t* at = reinterpret_cast<uint16_t*>(row) + col + 2 * lane;
+    const int left = n - col - 2 * lane;  // columns from this lane's first on
+    if ((reinterpret_cast<uintptr_t>(at) & 3) == 0) {
+      if (left > 1) *reinterpret_cast<uint32_t*>(at) = word;
+      if (left == 1) at[0] = (uint16_t)word;
+    } else {
+      const uint32_t next = __shfl_down_sync(~0u, word, 1);
+      if (lane == 0 && left > 0) at[0] = (uint16_t)word;
+      if (lane < 31 && left > 2)
+        *reinterpret_cast<uint32_t*>(at + 1) = word >> 16 | next << 16;
+      else if (left > 1)
+        at[1] = (uint16_t)(word >> 16);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void fp8_fill_row(uint8_t* box, int r, int lane, const T* row, int col, int n) {
+  uint32_t word = 0;
+  if constexpr (sizeof(T) == 4) {
+    if (col + lane < n) word = reinterpret_cast<const uint32_t*>(row)[col + lane];
+  } else {
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(row) + col + 2 * lane;
+    if (col + 2 * lane < n) word = at[0];
+    if (col + 2 * lane + 1 < n) word |= (uint32_t)at[1] << 16;
+  }
+  *fp8_word(box, r, lane) = word;
+}
+
 // `BOXES` boxes of 4 KB next to each other in a row. (Out of line: inlined
 // where it is used, it took registers from the sums.)
 template <int BOXES, int BOX_COLS>
@@ -359,10 +400,11 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
         }
       }
       if constexpr (SPLIT) {
-        // This CTA's sums as pairs, pair q of row `lane` at q ^ lane.
-        float2* mine = reinterpret_cast<float2*>(patch);
+        // This CTA's sums in fours, four q of row `lane` at q ^ (lane % 16).
+        ulonglong2* mine = reinterpret_cast<ulonglong2*>(patch) + lane * (CW / 4);
+        if (any)
 #pragma unroll
-        for (int q = 0; q < CW / 2; q++) mine[lane * (CW / 2) + (q ^ lane)] = unpack_f32x2(acc[q]);
+          for (int q = 0; q < CW / 4; q++) mine[q ^ (lane & 15)] = make_ulonglong2(acc[2 * q], acc[2 * q + 1]);
         break;
       }
       if (!ok) break;
@@ -382,9 +424,11 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       auto write_tile = [&](auto act_c, auto res_c) {
         constexpr int ACT = decltype(act_c)::value;
         constexpr bool RES = decltype(res_c)::value;
-        if (p.tma_out) {
+        const int rows = min(32, p.m - row_t);
 #pragma unroll
-          for (int h = 0; h < ROUNDS; h++) {
+        for (int h = 0; h < ROUNDS; h++) {
+          const int col_h = col_t + h * BOXES * BOX_COLS;
+          if (p.tma_out) {
             if (h) {
               if (lane == 0) {
                 bulk_wait_read();
@@ -397,70 +441,52 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               res_phase ^= 1;
               res_flying = false;
             }
+          } else if (RES) {
+            const T* res = static_cast<const T*>(p.residual) + (long long)row_t * p.residual_stride;
+#pragma unroll 1
+            for (int b = 0; b < BOXES; b++)
+#pragma unroll 4
+              for (int r = 0; r < rows; r++)
+                fp8_fill_row<T>(patch + b * 4096, r, lane, res + r * p.residual_stride, col_h + b * BOX_COLS, p.n);
+            __syncwarp();
+          }
 #pragma unroll
-            for (int j = 0; j < BOXES * 8; j++) {
-              const int at = h * BOXES * BOX_COLS + j * V;  // the chunk's first column
-              float v[V];
+          for (int j = 0; j < BOXES * 8; j++) {
+            const int at = h * BOXES * BOX_COLS + j * V;  // the chunk's first column
+            float v[V];
 #pragma unroll
-              for (int q = 0; q < V; q += 4) {
-                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sbias + at + q);
-                const float2 x = unpack_f32x2(fadd2_pair(acc[(at + q) / 2], b.x));
-                const float2 y = unpack_f32x2(fadd2_pair(acc[(at + q) / 2 + 1], b.y));
-                v[q] = x.x;
-                v[q + 1] = x.y;
-                v[q + 2] = y.x;
-                v[q + 3] = y.y;
-              }
-              op_act_vec<ACT, true, V>(v);
-              uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
-              if (RES) add_16<T>(v, *chunk);
-              *chunk = make_16<T>(v);
+            for (int q = 0; q < V; q += 4) {
+              const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sbias + at + q);
+              const float2 x = unpack_f32x2(fadd2_pair(acc[(at + q) / 2], b.x));
+              const float2 y = unpack_f32x2(fadd2_pair(acc[(at + q) / 2 + 1], b.y));
+              v[q] = x.x;
+              v[q + 1] = x.y;
+              v[q + 2] = y.x;
+              v[q + 3] = y.y;
             }
+            op_act_vec<ACT, true, V>(v);
+            uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
+            if (RES) add_16<T>(v, *chunk);
+            *chunk = make_16<T>(v);
+          }
+          if (p.tma_out) {
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) {
 #pragma unroll
-              for (int b = 0; b < BOXES; b++) {
-                const int col = col_t + (h * BOXES + b) * BOX_COLS;
-                if (col < p.n) tma_store_2d(&out_map, patch + b * 4096, col, row_t);
-              }
+              for (int b = 0; b < BOXES; b++)
+                if (col_h + b * BOX_COLS < p.n) tma_store_2d(&out_map, patch + b * 4096, col_h + b * BOX_COLS, row_t);
               bulk_commit();
             }
-          }
-        } else {
-          // 32 rows x 64 columns at a time through the patch, so that a
-          // warp's accesses are runs of a row wherever the rows start.
-          float* stg = reinterpret_cast<float*>(patch);
-          const int rows = min(32, p.m - row_t);
-#pragma unroll
-          for (int h = 0; h < CW / 64; h++) {
+          } else {
             __syncwarp();
-#pragma unroll
-            for (int q = 0; q < 32; q++) {
-              const float2 pr = unpack_f32x2(acc[h * 32 + q]);
-              stg[lane * 64 + ((2 * q) ^ lane)] = pr.x;
-              stg[lane * 64 + ((2 * q + 1) ^ lane)] = pr.y;
-            }
-            __syncwarp();
-            // two columns a lane: the pairs whose activations go together
-            const int at = h * 64 + 2 * lane, col = col_t + at;
-            if (col < p.n) {
-              const float2 b = *reinterpret_cast<const float2*>(sbias + at);
-              const T* res = static_cast<const T*>(p.residual) + (long long)row_t * p.residual_stride + col;
-              T* out = static_cast<T*>(p.out) + (long long)row_t * p.out_stride + col;
-              const bool two = col + 1 < p.n;
+            T* out = static_cast<T*>(p.out) + (long long)row_t * p.out_stride;
 #pragma unroll 1
-              for (int r = 0; r < rows; r++) {
-                float v[2] = {stg[r * 64 + ((2 * lane) ^ r)] + b.x, stg[r * 64 + ((2 * lane + 1) ^ r)] + b.y};
-                op_act_vec<ACT, true, 2>(v);
-                if (RES) {
-                  v[0] += to_f32(res[r * p.residual_stride]);
-                  if (two) v[1] += to_f32(res[r * p.residual_stride + 1]);
-                }
-                out[r * p.out_stride] = from_f32<T>(v[0]);
-                if (two) out[r * p.out_stride + 1] = from_f32<T>(v[1]);
-              }
-            }
+            for (int b = 0; b < BOXES; b++)
+#pragma unroll 4
+              for (int r = 0; r < rows; r++)
+                fp8_drain_row<T>(patch + b * 4096, r, lane, out + r * p.out_stride, col_h + b * BOX_COLS, p.n);
+            __syncwarp();
           }
         }
       };
@@ -473,52 +499,55 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
       __syncwarp();  // the patch is read
     }
     if constexpr (SPLIT) {
-      cluster_sync();  // every CTA's sums are in its shared memory
-      // The warps of the cluster take the tile's rows' halves in turn: two
-      // columns a lane, the CTAs' sums added in their order.
+      // The warps of the cluster take the tile's rows in turn: four columns a
+      // lane, the CTAs' sums added in their order.
       int mt, nt;
       fp8_tile(p, first, &mt, &nt);
-      const int rows = min(128, p.m - mt * 128);
+      const int rows = min(128, p.m - mt * 128), col = nt * 128 + 4 * lane, cols = min(4, p.n - col);
+      float bias[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) bias[q] = p.bias && q < cols ? p.bias[col + q] : 0.0f;
+      cluster_sync();  // every CTA's sums are in its shared memory
       op_act_switch(p.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
-        constexpr int U = 4;  // of them at a time, for their loads to overlap
+        constexpr int U = 4;  // rows at a time, for their loads to overlap
         const int stride = p.splits * FP8_EPI_WARPS;
 #pragma unroll 1
-        for (int h0 = (int)split * FP8_EPI_WARPS + e; ok && h0 < 2 * rows; h0 += U * stride) {
-          float2 sum[U], more[U];
+        for (int r0 = (int)split * FP8_EPI_WARPS + e; ok && r0 < rows; r0 += U * stride) {
+          float v[U][4], more[U][4];
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            const int h = h0 + u * stride, col = nt * 128 + (h & 1) * 64 + 2 * lane;
-            const bool one = h < 2 * rows && col < p.n, two = one && col + 1 < p.n;
-            sum[u] = make_float2(one && p.bias ? p.bias[col] : 0.0f, two && p.bias ? p.bias[col + 1] : 0.0f);
-            more[u] = make_float2(0.0f, 0.0f);
-            if (p.residual) {
-              const T* res = static_cast<const T*>(p.residual) + (mt * 128 + (h >> 1)) * p.residual_stride + col;
-              if (one) more[u].x = to_f32(res[0]);
-              if (two) more[u].y = to_f32(res[1]);
+            const int r = r0 + u * stride;
+            const T* res = static_cast<const T*>(p.residual) + (mt * 128 + r) * p.residual_stride + col;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+              v[u][q] = bias[q];
+              more[u][q] = p.residual && r < rows && q < cols ? to_f32(res[q]) : 0.0f;
             }
           }
 #pragma unroll 2
           for (int k = 0; k < p.splits; k++)
 #pragma unroll
             for (int u = 0; u < U; u++) {
-              const int h = min(h0 + u * stride, 2 * rows - 1), r = h >> 1;
-              const uint8_t* at = smem + L::OUT_OFF + ((h & 1) * 4 + (r >> 5)) * L::OUT_WARP;
-              const float2* from = reinterpret_cast<const float2*>(at) + (r & 31) * (CW / 2) + (lane ^ (r & 31));
-              sum[u] = fadd2(sum[u], ld_cluster_f32x2(from, (uint32_t)k));
+              const int r = r0 + u * stride;
+              if (r >= rows) break;
+              const uint8_t* at = smem + L::OUT_OFF + ((lane >> 4) * 4 + (r >> 5)) * L::OUT_WARP;
+              const float4 x = ld_cluster_f32x4(
+                  reinterpret_cast<const float4*>(at) + (r & 31) * (CW / 4) + ((lane ^ r) & 15), (uint32_t)k);
+              v[u][0] += x.x;
+              v[u][1] += x.y;
+              v[u][2] += x.z;
+              v[u][3] += x.w;
             }
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            const int h = h0 + u * stride, col = nt * 128 + (h & 1) * 64 + 2 * lane;
-            float v[2] = {sum[u].x, sum[u].y};
-            op_act_vec<ACT, true, 2>(v);
-            if (p.residual) {
-              v[0] += more[u].x;
-              v[1] += more[u].y;
-            }
-            T* out = static_cast<T*>(p.out) + (mt * 128 + (h >> 1)) * p.out_stride + col;
-            if (h < 2 * rows && col < p.n) out[0] = from_f32<T>(v[0]);
-            if (h < 2 * rows && col + 1 < p.n) out[1] = from_f32<T>(v[1]);
+            const int r = r0 + u * stride;
+            op_act_vec<ACT, true, 4>(v[u]);
+            T* out = static_cast<T*>(p.out) + (mt * 128 + r) * p.out_stride + col;
+            if (r < rows)
+#pragma unroll
+              for (int q = 0; q < 4; q++)
+                if (q < cols) out[q] = from_f32<T>(p.residual ? v[u][q] + more[u][q] : v[u][q]);
           }
         }
       });

@@ -330,16 +330,17 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cg = q.join.cg << q.join.shift, groups = q.groups;
   const int steps = (int)q.by_rows.div((uint32_t)(q.pixels + q.rows - 1));
-  // [step][thread] vectors, the threads' statistics, the groups' statistics
-  // over this CTA and their mean and rstd over the cluster.
-  uint4* data = reinterpret_cast<uint4*>(smem) + threadIdx.x;
-  float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * NORM_THREADS * 16);
+  // [pixel][vector], the threads' statistics, the groups' statistics over this
+  // CTA and their mean and rstd over the cluster.
+  const int stride = q.rows * q.vecs;  // vectors of a step
+  float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * stride * 16);
   float* tdev = tmean + NORM_THREADS * VE;
   float* entries = tdev + NORM_THREADS * VE;
   float2* own = reinterpret_cast<float2*>(entries + 3 * norm_entries(q.join.runs[0]));
   float2* stat = own + (groups + 1) / 2 * 2;
   const int r = (int)q.by_slots.div(threadIdx.x), slot = (int)threadIdx.x - r * q.slots;
   const bool live = r < q.rows && slot < q.vecs;
+  uint4* data = reinterpret_cast<uint4*>(smem) + r * q.vecs + slot;
   const int first = rank * q.pixels, px = max(0, (int)min((long long)q.pixels, p.pixels - first));
   const int ch = seg * q.seg_c + slot * VE;
   const int n = live && r < px ? (int)q.by_rows.div((uint32_t)(px - r + q.rows - 1)) : 0;  // this thread's vectors
@@ -356,9 +357,9 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   for (int b = 0; b < 4; b++) {
     for (const int end = min(n, (b + 1) * batch); s < end; s++)
       if constexpr (AL)
-        cp_async_16(data + s * NORM_THREADS, x + s * step);
+        cp_async_16(data + s * stride, x + s * step);
       else
-        data[s * NORM_THREADS] = Vec<T, VE, AL>::fetch(x + s * step);
+        data[s * stride] = Vec<T, VE, AL>::fetch(x + s * step);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   Affine<VE> affine;
@@ -370,16 +371,16 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     for (; i + 4 <= end; i += 4) {
       uint4 raw[4];
 #pragma unroll
-      for (int u = 0; u < 4; u++) raw[u] = data[(i + u) * NORM_THREADS];
+      for (int u = 0; u < 4; u++) raw[u] = data[(i + u) * stride];
       run.template add<V, 4>(raw);
     }
     if (end == n && i < end) {
-      const uint4 two[2] = {data[i * NORM_THREADS], data[min(i + 1, end - 1) * NORM_THREADS]};
+      const uint4 two[2] = {data[i * stride], data[min(i + 1, end - 1) * stride]};
       if (i + 2 <= end) {
         run.template add<V, 2>(two);
         i += 2;
       }
-      if (i < end) run.template add<V, 1>(data + i * NORM_THREADS);
+      if (i < end) run.template add<V, 1>(data + i * stride);
     }
   };
   cp_async_wait<3>();
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
 #pragma unroll 1
     for (int i = 0; i < end; i++) {
       float v[VE];
-      Vec<T, VE, AL>::expand(i < n ? data[i * NORM_THREADS] : make_uint4(0, 0, 0, 0), v);
+      Vec<T, VE, AL>::expand(i < n ? data[i * stride] : make_uint4(0, 0, 0, 0), v);
       affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
       if (FP8)
@@ -556,20 +557,20 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
   const int all = q.chunks * span;
   float m = 0.0f, d = 0.0f, n0;
   const float m0 = pair(0, &n0).x;
-  if (all <= 2 * 32) {  // the usual case: all loads at once
-    float2 v[2];
-    float n[2];
+  if (all <= 5 * 32) {  // the usual case: all loads at once
+    float2 v[5];
+    float n[5];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 5; i++) {
       v[i] = make_float2(0.0f, 0.0f);
       n[i] = 0.0f;
       if (i * 32 + lane < all) v[i] = pair(i * 32 + lane, &n[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++) m = fmaf(n[i], v[i].x - m0, m);
+    for (int i = 0; i < 5; i++) m = fmaf(n[i], v[i].x - m0, m);
     m = m0 + warp_sum(m) / count;
 #pragma unroll
-    for (int i = 0; i < 2; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
+    for (int i = 0; i < 5; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
   } else {
     float n;
     for (int i = lane; i < all; i += 32) {
@@ -633,18 +634,21 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
       else if (here)
         V::store(out + u * out_step, v);
     };
-    for (int u = 0, left = px - full * per; u * rows < left; u++) {
-      const bool here = live && u * rows + r < left;
-      put(here ? V::fetch(x + u * x_step) : V::zero(), u, here);
-    }
-    if (!FP8 && !live) return;
-    // Whole fours of steps, the next ones' loads ahead of this one's work.
-    typename V::Raw raw[U];
+    // The last pixels, then whole fours of steps, the next ones' loads ahead
+    // of this one's work.
+    typename V::Raw raw[U], rest[U];
+    const int left = px - full * per;
+#pragma unroll
+    for (int u = 0; u < U; u++) rest[u] = live && u * rows + r < left ? V::fetch(x + u * x_step) : V::zero();
     if (full) {
       x -= U * x_step;
 #pragma unroll
       for (int u = 0; u < U; u++) raw[u] = V::fetch(x + u * x_step);
     }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (u * rows < left) put(rest[u], u, live && u * rows + r < left);
+    if (!FP8 && !live) return;
     for (int f = full; f > 0; f--) {
       typename V::Raw next[U];
       x -= U * x_step;

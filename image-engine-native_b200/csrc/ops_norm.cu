@@ -10,7 +10,7 @@ namespace iec {
 
 namespace {
 
-constexpr int RESIDENT_BYTES = 180 * 1024;  // of a CTA's values in shared memory
+constexpr int RESIDENT_BYTES = 184 * 1024;  // of a CTA's values in shared memory
 constexpr int CLUSTER = 16, STATS_CLUSTER = 2;
 
 // The joining of a tile of `c` channels (and of the last one, of `c_last`)
@@ -31,46 +31,66 @@ NormJoin join_shape(int cg, int c, int c_last, int rows) {
   return j;
 }
 
-// The resident kernel's shape, or false where a segment outgrows a cluster.
-// A segment is the smallest run of whole groups, vectors (and with fp8 whole
-// blocks) that has at least 128 bytes, so that segments read whole lines and
-// there are as many clusters as possible.
+// The resident kernel's shape with segments of `seg` channels, or false where
+// one outgrows a cluster.
 template <class T>
-bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, int* cluster, size_t* smem) {
+bool plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, NormResident* q, int* cluster, size_t* smem) {
   constexpr int VE = 16 / (int)sizeof(T);
-  const int cg = p.c / p.groups;
-  long long unit = std::lcm<long long>(cg, VE);
-  if (fp8) unit = std::lcm<long long>(unit, FP8_BLOCK);
-  long long seg = p.c;
-  if (unit < p.c && p.c % unit == 0) {
-    seg = unit;
-    while (seg < p.c && (seg * (long long)sizeof(T) < 128 || p.c % seg)) seg += unit;
-  }
-  q->seg_c = (int)seg;
-  q->vecs = (int)seg / VE;
-  const int lanes = fp8 ? FP8_BLOCK / VE : 1;
+  const int cg = p.c / p.groups, lanes = fp8 ? FP8_BLOCK / VE : 1;
+  q->seg_c = seg;
+  q->vecs = seg / VE;
   q->slots = (q->vecs + lanes - 1) / lanes * lanes;
   if (q->slots > NORM_THREADS || p.pixels > (1 << 23)) return false;
   q->rows = NORM_THREADS / q->slots;
-  const int segs = p.c / q->seg_c, most_steps = RESIDENT_BYTES / (NORM_THREADS * 16);
+  const int segs = p.c / seg, most_steps = RESIDENT_BYTES / (q->rows * q->vecs * 16);
   const long long need = (p.pixels + (long long)most_steps * q->rows - 1) / ((long long)most_steps * q->rows);
   if (need > CLUSTER || segs > 65535) return false;
   // as many CTAs as fill the GPU, but at least two steps each
   const long long spread = dev.sms() / std::max<long long>(1, (long long)segs * p.n);
   const long long fill = (p.pixels + 2LL * q->rows - 1) / (2LL * q->rows);
-  int n = (int)std::max(need, std::min({spread, fill, (long long)CLUSTER}));
-  n = std::max(n, 1);
+  const int n = (int)std::max<long long>(1, std::max(need, std::min({spread, fill, (long long)CLUSTER})));
   q->pixels = (int)((p.pixels + n - 1) / n);
   *cluster = n;
   const int steps = (q->pixels + q->rows - 1) / q->rows;
-  q->groups = q->seg_c / cg;
+  q->groups = seg / cg;
   q->by_slots = FastDiv((uint32_t)q->slots);
   q->by_rows = FastDiv((uint32_t)q->rows);
   q->by_cg = FastDiv((uint32_t)cg);
-  q->join = join_shape<VE>(cg, q->seg_c, q->seg_c, q->rows);
-  *smem = (size_t)steps * NORM_THREADS * 16 + (size_t)NORM_THREADS * VE * 8 +
+  q->join = join_shape<VE>(cg, seg, seg, q->rows);
+  *smem = (size_t)steps * q->rows * q->vecs * 16 + (size_t)NORM_THREADS * VE * 8 +
           (size_t)norm_entries(q->join.runs[0]) * 12 + (size_t)(q->groups + 1) * 16;
-  return *smem <= 220 * 1024;
+  if (*smem > 224 * 1024) return false;
+  // Only where all its clusters run at once: one after another, their loads,
+  // statistics and stores take turns (8 x 128 x 128 x 256 f16: 90 us in four
+  // waves of clusters of 16, 52 in chunks through L2). A cluster size that
+  // the GPU's parts divide badly is made smaller.
+  constexpr auto codes = norm_resident<T, true, true>;
+  constexpr auto wide = norm_resident<T, false, true>;
+  auto room = [&](int size) {
+    return fp8 ? resident_ctas<codes>(dev, NORM_THREADS, *smem, size)
+               : resident_ctas<wide>(dev, NORM_THREADS, *smem, size);
+  };
+  return (long long)n * segs * p.n <= room(n);
+}
+
+// The resident kernel's shape: segments of whole groups and vectors (and with
+// fp8 whole blocks), the smallest that have 128 bytes, so that they read
+// whole lines and there are many clusters; else the largest below that.
+template <class T>
+bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, int* cluster, size_t* smem) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  long long unit = std::lcm<long long>(p.c / p.groups, VE);
+  if (fp8) unit = std::lcm<long long>(unit, FP8_BLOCK);
+  if (unit >= p.c || p.c % unit) return plan_segment<T>(dev, p, fp8, p.c, q, cluster, smem);
+  const long long line = 128 / sizeof(T);
+  for (long long seg = (line + unit - 1) / unit * unit; seg <= p.c; seg += unit)
+    if (p.c % seg == 0) {
+      if (plan_segment<T>(dev, p, fp8, (int)seg, q, cluster, smem)) return true;
+      break;
+    }
+  for (long long seg = (line - 1) / unit * unit; seg >= unit; seg -= unit)
+    if (p.c % seg == 0) return plan_segment<T>(dev, p, fp8, (int)seg, q, cluster, smem);
+  return false;
 }
 
 template <class T, int VE, bool AL>
@@ -148,16 +168,7 @@ void run_vectors(Device& dev, const NormSpec& p, cudaStream_t s) {
   size_t smem = 0;
   constexpr auto wide = norm_resident<T, false, AL>;
   constexpr auto codes = norm_resident<T, true, AL>;
-  bool fits = plan_resident<T>(dev, p, fp8, &q, &cluster, &smem);
-  if (fits) {
-    // Only where all its clusters run at once: one after another, their
-    // loads, statistics and stores take turns (8 x 128 x 128 x 256 f16: 90 us
-    // in four waves of clusters of 16, 40 in chunks through L2).
-    const long long ctas = (long long)cluster * (p.c / q.seg_c) * p.n;
-    fits = ctas <= (fp8 ? resident_ctas<codes>(dev, NORM_THREADS, smem, cluster)
-                        : resident_ctas<wide>(dev, NORM_THREADS, smem, cluster));
-  }
-  if (!fits) return run_chunks<T, VE, AL>(dev, p, s);
+  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE, AL>(dev, p, s);
   const double values = (double)p.n * p.pixels * p.c;
   timed_launch("norm_resident", 12 * values, values * (sizeof(T) + (fp8 ? 1 : sizeof(T))), s, [&] {
     const dim3 grid(cluster, p.c / q.seg_c, p.n);

@@ -270,10 +270,18 @@ __device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-// A pair at this CTA's shared address `p` in CTA `rank`.
+// A pair (and four) at this CTA's shared address `p` in CTA `rank`.
 __device__ __forceinline__ float2 ld_cluster_f32x2(const float2* p, uint32_t rank) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(const float4* p, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_map(p, rank))
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void cluster_sync() {
