@@ -719,6 +719,8 @@ void iec_ops_free(iec_ops* ops) {
   if (valid_ops(ops)) delete ops;
 }
 
+int iec_ops_device(const iec_ops* ops) { return valid_ops(ops) ? ops->device->ordinal() : -1; }
+
 const char* iec_ops_device_name(const iec_ops* ops) { return valid_ops(ops) ? ops->device->name().c_str() : ""; }
 
 namespace {

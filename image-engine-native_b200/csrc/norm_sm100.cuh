@@ -35,11 +35,12 @@ constexpr int NORM_THREADS = 512;
 constexpr int NORM_RING = 2;
 constexpr int APPLY_THREADS = 256;
 
-// A thread's VE values of a pixel as e4m3 codes with the scale of their block
-// of 128: the block's threads are 128 / VE consecutive lanes. `live`: the
-// thread's channels exist.
+// A thread's VE values of a pixel as e4m3 codes at `out`, with the scale of
+// their block of 128 at `scale_at` (null but in the block's first thread):
+// the block's threads are 128 / VE consecutive lanes. `live`: the thread's
+// channels exist.
 template <int VE, bool AL>
-__device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch, bool live, const float* v) {
+__device__ __forceinline__ void store_fp8(uint8_t* out, float* scale_at, bool live, const float* v) {
   constexpr int LANES = FP8_BLOCK / VE;
   float most = 0.0f;
 #pragma unroll
@@ -57,7 +58,6 @@ __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch
     const float2 b = fmul2(make_float2(v[e + 2], v[e + 3]), both(factor));
     w[e / 4] = (uint32_t)e4m3x2(a.x, a.y) | (uint32_t)e4m3x2(b.x, b.y) << 16;
   }
-  uint8_t* out = q.codes + row * (long long)q.code_stride + ch;
   if constexpr (!AL) {
 #pragma unroll
     for (int e = 0; e < VE; e++) out[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
@@ -66,7 +66,7 @@ __device__ __forceinline__ void store_fp8(const Fp8Out& q, long long row, int ch
   } else {
     *reinterpret_cast<uint32_t*>(out) = w[0];
   }
-  if (ch % FP8_BLOCK == 0) q.scales[(long long)(ch / FP8_BLOCK) * (long long)q.scale_stride + row] = scale;
+  if (scale_at) *scale_at = scale;
 }
 
 __device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
@@ -271,7 +271,7 @@ __device__ __forceinline__ void join_threads(const NormJoin& q, bool last, const
 // operation less, but rounds at the size of mean scale.)
 template <int VE>
 struct Affine {
-  float mean[VE], scale[VE], shift[VE];
+  float minus[VE], scale[VE], shift[VE];  // minus the mean
   __device__ __forceinline__ void fetch(const NormSpec& p, int ch, bool live) {
 #pragma unroll
     for (int e = 0; e < VE; e++) {
@@ -285,7 +285,7 @@ struct Affine {
 #pragma unroll
     for (int e = 0; e < VE; e++) {
       const float2 st = stat[g - g0];
-      mean[e] = st.x;
+      minus[e] = -st.x;
       scale[e] *= st.y;
       if (--left == 0) {
         g++;
@@ -295,11 +295,11 @@ struct Affine {
   }
   __device__ __forceinline__ void apply(float* v) const {
     if constexpr (VE == 1) {
-      v[0] = fmaf(v[0] - mean[0], scale[0], shift[0]);
+      v[0] = fmaf(v[0] + minus[0], scale[0], shift[0]);
     } else {
 #pragma unroll
       for (int e = 0; e < VE; e += 2) {
-        const float2 d = fadd2(make_float2(v[e], v[e + 1]), make_float2(-mean[e], -mean[e + 1]));
+        const float2 d = fadd2(make_float2(v[e], v[e + 1]), make_float2(minus[e], minus[e + 1]));
         const float2 y = ffma2(d, make_float2(scale[e], scale[e + 1]), make_float2(shift[e], shift[e + 1]));
         v[e] = y.x;
         v[e + 1] = y.y;
@@ -420,7 +420,11 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     constexpr int ACT = decltype(act_c)::value;
     // with fp8 the lanes of a block go through the shuffles together
     const int end = FP8 ? steps : n;
-    const long long row0 = map * p.pixels + first + r;
+    const long long row0 = map * p.pixels + first + r, code_step = q.rows * (long long)p.q.code_stride;
+    uint8_t* codes = FP8 ? p.q.codes + row0 * (long long)p.q.code_stride + ch : nullptr;
+    float* scale_at = FP8 && ch % FP8_BLOCK == 0
+                          ? p.q.scales + (long long)(ch / FP8_BLOCK) * (long long)p.q.scale_stride + row0
+                          : nullptr;
     T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + (first + r) * p.out_stride + ch;
     const long long out_step = q.rows * p.out_stride;
 #pragma unroll 1
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
       if (FP8)
-        store_fp8<VE, AL>(p.q, row0 + (long long)i * q.rows, ch, i < n, v);
+        store_fp8<VE, AL>(codes + i * code_step, scale_at ? scale_at + i * q.rows : nullptr, i < n, v);
       else
         Vec<T, VE, AL>::store(out + i * out_step, v);
     }
@@ -600,10 +604,11 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
   const int r = threadIdx.x / slots, slot = threadIdx.x - r * slots;
   const bool live = r < rows && slot < vecs;
   const int ch = c0 + (live ? slot * VE : 0);
-  Affine<VE> affine;
-  affine.fetch(p, ch, live);
   griddep_launch_dependents();
   griddep_wait();
+  // (gamma and beta too may come from the kernels before)
+  Affine<VE> affine;
+  affine.fetch(p, ch, live);
   for (int g = g0 + (int)(threadIdx.x >> 5); g <= g1; g += APPLY_THREADS / 32) {
     const float2 st = norm_join(p, q, z, g);
     if ((threadIdx.x & 31) == 0) stat[g - g0] = st;
@@ -621,7 +626,11 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
   const long long at = first + (long long)full * per + own;
   const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + at * p.x_stride + ch;
   T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + at * p.out_stride + ch;
-  long long row = map * p.pixels + at;
+  const long long row = map * p.pixels + at, code_step = FP8 ? rows * (long long)p.q.code_stride : 0;
+  uint8_t* codes = FP8 ? p.q.codes + row * (long long)p.q.code_stride + ch : nullptr;
+  float* scale_at = FP8 && live && ch % FP8_BLOCK == 0
+                        ? p.q.scales + (long long)(ch / FP8_BLOCK) * (long long)p.q.scale_stride + row
+                        : nullptr;
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     auto put = [&](typename V::Raw raw, int u, bool here) {
@@ -630,7 +639,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
       affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
       if constexpr (FP8)
-        store_fp8<VE, AL>(p.q, row + u * rows, ch, here, v);
+        store_fp8<VE, AL>(codes + u * code_step, scale_at ? scale_at + u * rows : nullptr, here, v);
       else if (here)
         V::store(out + u * out_step, v);
     };
@@ -655,8 +664,12 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
       if (f > 1)
 #pragma unroll
         for (int u = 0; u < U; u++) next[u] = V::fetch(x + u * x_step);
-      row -= per;
-      if (!FP8) out -= U * out_step;
+      if (FP8) {
+        codes -= U * code_step;
+        if (scale_at) scale_at -= per;
+      } else {
+        out -= U * out_step;
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) put(raw[u], u, live);
 #pragma unroll

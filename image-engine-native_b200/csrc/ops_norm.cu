@@ -127,7 +127,7 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   q.cluster = (int)std::min<long long>(ctas, STATS_CLUSTER);
   q.chunks = (int)((ctas + q.cluster - 1) / q.cluster);
   q.span = (p.pixels + q.chunks * q.cluster - 1) / (q.chunks * q.cluster);
-  q.part = static_cast<float2*>(dev.scratch((size_t)maps * q.chunks * q.tiles * q.slots * sizeof(float2), s));
+  q.part = static_cast<float2*>(dev.lasting_scratch((size_t)maps * q.chunks * q.tiles * q.slots * sizeof(float2), s));
   const double values = (double)p.pixels * p.c;
   for (q.map0 = 0; q.map0 < p.n; q.map0 += (int)maps) {
     const int now = (int)std::min<long long>(maps, p.n - q.map0);

@@ -259,6 +259,7 @@ Device::~Device() {
   if (poisoned()) {
     dev_err_.leak();
     for (auto& e : scratch_) e.second.leak();
+    for (auto& e : lasting_) e.second.leak();
   }
   if (prev >= 0) cudaSetDevice(prev);
 }

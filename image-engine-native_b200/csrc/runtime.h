@@ -13,6 +13,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 #include <functional>
@@ -174,6 +175,18 @@ class Device {
     scratch_gen_++;
     return scratch_.back().second.get();
   }
+  // Scratch whose earlier buffers stay until the device goes when it grows: a
+  // graph that a caller captured goes on using the one it saw.
+  void* lasting_scratch(size_t bytes, cudaStream_t stream) {
+    DeviceBuffer* last = nullptr;
+    for (auto& e : lasting_)
+      if (e.first == stream) last = &e.second;  // the newest of the stream's is the largest
+    if (last && last->size() >= bytes) return last->get();
+    DeviceBuffer b;
+    b.reserve(std::max(bytes, last ? 2 * last->size() : (size_t)1 << 20));
+    lasting_.emplace_back(stream, std::move(b));
+    return lasting_.back().second.get();
+  }
   // Counts the scratch buffers' (re)allocations (a captured pass that used
   // an older one must not replay).
   uint64_t scratch_generation() const { return scratch_gen_; }
@@ -207,6 +220,7 @@ class Device {
   cudaStream_t copy_stream_ = nullptr;
   DeviceBuffer dev_err_;
   std::vector<std::pair<cudaStream_t, DeviceBuffer>> scratch_;
+  std::vector<std::pair<cudaStream_t, DeviceBuffer>> lasting_;
   uint64_t scratch_gen_ = 0;
   PinnedBuffer host_err_;
   std::string poisoned_;

@@ -45,17 +45,25 @@ def _dtype(t, what: str) -> int:
     return code
 
 
-def _f32_vector(t, n: int, what: str) -> int:
+def _elsewhere(t, device: int, what: str):
+    _bad(f"{what} is on {t.device}, the handle on cuda:{device}")
+
+
+def _f32_vector(t, n: int, device: int, what: str) -> int:
     """The address of n contiguous floats, 0 for None."""
     if t is None:
         return 0
+    if t.get_device() != device:
+        _elsewhere(t, device, what)
     if t.dtype is not _F32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         _bad(f"{what} must be {n} contiguous float32 values")
     return t.data_ptr()
 
 
-def _rows(t, shape, dtype, what: str) -> int:
+def _rows(t, shape, dtype, device: int, what: str) -> int:
     """The row stride of a matrix of `shape` whose rows are contiguous."""
+    if t.get_device() != device:
+        _elsewhere(t, device, what)
     if t.dtype is dtype and t.shape == shape:
         step, one = t.stride()
         if one == 1 or shape[1] <= 1:
@@ -64,8 +72,10 @@ def _rows(t, shape, dtype, what: str) -> int:
     _bad(f"{what} is {tuple(t.shape)} of {t.dtype}, not {tuple(shape)} of {dtype}")
 
 
-def _maps(t, what: str):
+def _maps(t, device: int, what: str):
     """(maps, pixels, channels, pixel stride, map stride) of n x ... x c."""
+    if t.get_device() != device:
+        _elsewhere(t, device, what)
     shape, stride = t.shape, t.stride()
     if len(shape) < 2:
         _bad(f"{what} must be maps x pixels (or height x width) x channels")
@@ -85,14 +95,14 @@ def _maps(t, what: str):
     return n, pixels, c, step, stride[0] if n > 1 else c
 
 
-def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device):
+def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device: int):
     if codes is None:
-        codes = empty_codes(rows, k, device)
-    code_step = _rows(codes, (rows, k), _FP8, "codes")
+        codes = empty_codes(rows, k, f"cuda:{device}")
+    code_step = _rows(codes, (rows, k), _FP8, device, "codes")
     blocks = -(-k // BLOCK)
     if scales is None:
-        scales = torch.empty((blocks, scale_rows), dtype=_F32, device=device)
-    return codes, code_step, scales, _rows(scales, (blocks, scale_rows), _F32, "scales")
+        scales = torch.empty((blocks, scale_rows), dtype=_F32, device=f"cuda:{device}")
+    return codes, code_step, scales, _rows(scales, (blocks, scale_rows), _F32, device, "scales")
 
 
 def _stream(stream, device: int) -> int:
@@ -117,6 +127,7 @@ class Ops:
         L.iec_ops_device_name.restype = ctypes.c_char_p
         L.iec_ops_device_name.argtypes = [vp]
         L.iec_ops_free.argtypes = [vp]
+        L.iec_ops_device.argtypes = [vp]
         L.iec_ops_sync.argtypes = [vp, vp]
         for f in (L.iec_ops_group_norm, L.iec_ops_group_norm_fp8, L.iec_ops_quantize_fp8, L.iec_ops_matmul_fp8):
             f.argtypes = [vp, ctypes.c_char_p, vp]
@@ -124,6 +135,7 @@ class Ops:
         self._h = vp()
         opt = Options(device, timeout_ms, 0)
         _check(L.iec_ops_open(ctypes.byref(opt), ctypes.byref(self._h)))
+        self._device = L.iec_ops_device(self._h)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -138,23 +150,23 @@ class Ops:
 
     def sync(self, stream=None):
         """Wait (bounded) for the stream's work and raise what went wrong."""
-        _check(self._lib.iec_ops_sync(self._h, _stream(stream, torch.cuda.current_device())))
+        _check(self._lib.iec_ops_sync(self._h, _stream(stream, self._device)))
 
     def group_norm(self, x, groups: int, gamma=None, beta=None, eps: float = 1e-5, act: int = NONE, out=None,
                    stream=None):
         """Group normalisation and activation of channels-last maps (n, ...,
         c); `out` (default: a new tensor) may be `x`."""
         dtype = _dtype(x, "x")
-        n, pixels, c, step, map_step = _maps(x, "x")
+        n, pixels, c, step, map_step = _maps(x, self._device, "x")
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         elif out.dtype is not x.dtype or out.shape != x.shape:
             _bad("out must have the shape and type of x")
-        _, _, _, out_step, out_map_step = _maps(out, "out")
-        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
-                               _f32_vector(beta, c, "beta"), out.data_ptr(), out_step, out_map_step, 0, 0, 0, 0, eps,
+        _, _, _, out_step, out_map_step = _maps(out, self._device, "out")
+        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
+                               _f32_vector(beta, c, self._device, "beta"), out.data_ptr(), out_step, out_map_step, 0, 0, 0, 0, eps,
                                dtype, act)
-        status = self._lib.iec_ops_group_norm(self._h, args, _stream(stream, x.get_device()))
+        status = self._lib.iec_ops_group_norm(self._h, args, _stream(stream, self._device))
         if status:
             _check(status)
         return out
@@ -164,12 +176,12 @@ class Ops:
         """group_norm with its result as 8-bit rows, one per pixel: (codes
         n*pixels x c, scales ceil(c / 128) x n*pixels)."""
         dtype = _dtype(x, "x")
-        n, pixels, c, step, map_step = _maps(x, "x")
-        codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, x.device)
-        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, "gamma"),
-                               _f32_vector(beta, c, "beta"), 0, 0, 0, codes.data_ptr(), code_step, scales.data_ptr(),
+        n, pixels, c, step, map_step = _maps(x, self._device, "x")
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, self._device)
+        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
+                               _f32_vector(beta, c, self._device, "beta"), 0, 0, 0, codes.data_ptr(), code_step, scales.data_ptr(),
                                scale_step, eps, dtype, act)
-        status = self._lib.iec_ops_group_norm_fp8(self._h, args, _stream(stream, x.get_device()))
+        status = self._lib.iec_ops_group_norm_fp8(self._h, args, _stream(stream, self._device))
         if status:
             _check(status)
         return codes, scales
@@ -183,12 +195,12 @@ class Ops:
         if len(shape) != 2:
             _bad("x must be rows x values")
         rows, k = shape
-        step = _rows(x, shape, x.dtype, "x")
+        step = _rows(x, shape, x.dtype, self._device, "x")
         scale_rows = rows if block_rows != BLOCK else -(-rows // BLOCK)
-        codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, x.device)
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, self._device)
         args = QUANTIZE.pack(x.data_ptr(), rows, k, step, block_rows, codes.data_ptr(), code_step, scales.data_ptr(),
                              scale_step, dtype)
-        status = self._lib.iec_ops_quantize_fp8(self._h, args, _stream(stream, x.get_device()))
+        status = self._lib.iec_ops_quantize_fp8(self._h, args, _stream(stream, self._device))
         if status:
             _check(status)
         return codes, scales
@@ -202,21 +214,21 @@ class Ops:
         if len(a_shape) != 2 or len(w_shape) != 2:
             _bad("a and w must be matrices")
         m, k = a_shape
-        n = w_shape[0]
+        n, dev = w_shape[0], self._device
         blocks = -(-k // BLOCK)
         if out is None:
             out = torch.empty((m, n), dtype=dtype, device=a.device)
         code = _dtype(out, "out")
         res, res_step = 0, 0
         if residual is not None:
-            res, res_step = residual.data_ptr(), _rows(residual, (m, n), out.dtype, "residual")
-        args = MATMUL.pack(a.data_ptr(), _rows(a, a_shape, _FP8, "a"),
-                           a_scales.data_ptr(), _rows(a_scales, (blocks, m), _F32, "a_scales"),
-                           w.data_ptr(), _rows(w, (n, k), _FP8, "w"),
-                           w_scales.data_ptr(), _rows(w_scales, (blocks, -(-n // BLOCK)), _F32, "w_scales"),
-                           _f32_vector(bias, n, "bias"), res, res_step,
-                           out.data_ptr(), _rows(out, (m, n), out.dtype, "out"), m, n, k, act, code)
-        status = self._lib.iec_ops_matmul_fp8(self._h, args, _stream(stream, a.get_device()))
+            res, res_step = residual.data_ptr(), _rows(residual, (m, n), out.dtype, dev, "residual")
+        args = MATMUL.pack(a.data_ptr(), _rows(a, a_shape, _FP8, dev, "a"),
+                           a_scales.data_ptr(), _rows(a_scales, (blocks, m), _F32, dev, "a_scales"),
+                           w.data_ptr(), _rows(w, (n, k), _FP8, dev, "w"),
+                           w_scales.data_ptr(), _rows(w_scales, (blocks, -(-n // BLOCK)), _F32, dev, "w_scales"),
+                           _f32_vector(bias, n, self._device, "bias"), res, res_step,
+                           out.data_ptr(), _rows(out, (m, n), out.dtype, dev, "out"), m, n, k, act, code)
+        status = self._lib.iec_ops_matmul_fp8(self._h, args, _stream(stream, self._device))
         if status:
             _check(status)
         return out

@@ -320,7 +320,9 @@ iec_status iec_birefnet_set_fused(iec_birefnet* model, int on);
  * channels-last maps, and layers in 8-bit floating point. All work is queued
  * on `stream` (a cudaStream_t; NULL: the handle's own stream, which does not
  * order itself with any other; cudaStreamLegacy names the legacy default
- * stream) and the calls return without waiting. Sizes of zero are allowed
+ * stream) and the calls return without waiting. They can be captured into a
+ * CUDA graph after a call of the same size on the same stream (which sets
+ * the kernels' attributes and the scratch that larger maps take). Sizes of zero are allowed
  * and queue nothing where they leave nothing to write. Strides count
  * elements; rows may be further apart than they are long (a channel slice
  * of a wider map), never overlap.
@@ -348,6 +350,7 @@ typedef enum iec_act {
 iec_status iec_ops_open(const iec_options* options, iec_ops** out);
 void iec_ops_free(iec_ops* ops);
 const char* iec_ops_device_name(const iec_ops* ops);
+int iec_ops_device(const iec_ops* ops); /* its CUDA ordinal, -1 for no handle */
 
 /* Wait (bounded) for the work queued on `stream` (NULL: the handle's) and
  * report what went wrong in it. */

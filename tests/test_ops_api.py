@@ -40,16 +40,19 @@ def test_tensor_views():
     from iec import ops
 
     t = torch.zeros(2, 5, 7, 24)
-    assert ops._maps(t, "t") == (2, 35, 24, 24, 35 * 24)
-    assert ops._maps(t[..., :10], "t") == (2, 35, 10, 24, 35 * 24)
-    assert ops._maps(t[:1], "t")[:4] == (1, 35, 24, 24)
-    assert ops._maps(t[:, :, :1], "t") == (2, 5, 24, 7 * 24, 35 * 24)
-    assert ops._maps(t[:, :1, :1], "t")[:3] == (2, 1, 24)
+    assert ops._maps(t, -1, "t") == (2, 35, 24, 24, 35 * 24)
+    assert ops._maps(t[..., :10], -1, "t") == (2, 35, 10, 24, 35 * 24)
+    assert ops._maps(t[:1], -1, "t")[:4] == (1, 35, 24, 24)
+    assert ops._maps(t[:, :, :1], -1, "t") == (2, 5, 24, 7 * 24, 35 * 24)
+    assert ops._maps(t[:, :1, :1], -1, "t")[:3] == (2, 1, 24)
     for bad in (t[:, :, ::2], t[:, :, :4], t.transpose(1, 2), t.transpose(2, 3), torch.zeros(4)):
         with pytest.raises(iec.IecError):
-            ops._maps(bad, "t")
+            ops._maps(bad, -1, "t")
+    with pytest.raises(iec.IecError) as e:  # -1 is the device of CPU tensors
+        ops._maps(t, 0, "t")
+    assert "cpu" in str(e.value)
     codes = ops.empty_codes(3, 50, "cpu")
     assert codes.shape == (3, 50) and codes.stride(0) == 64
-    assert ops._rows(codes, (3, 50), torch.float8_e4m3fn, "codes") == 64
+    assert ops._rows(codes, (3, 50), torch.float8_e4m3fn, -1, "codes") == 64
     with pytest.raises(iec.IecError):
-        ops._rows(codes.t(), (50, 3), torch.float8_e4m3fn, "codes")
+        ops._rows(codes.t(), (50, 3), torch.float8_e4m3fn, -1, "codes")

@@ -412,6 +412,59 @@ def test_offsets_past_32_bits(ops):
     assert torch.equal(ops.matmul_fp8(codes, sa, w, sw), want)
 
 
+def test_gamma_and_beta_from_the_product_before(ops):
+    """An adaptive normalisation: gamma and beta are what a product queued just
+    before writes. Every kernel may start while the one before it runs; none
+    reads its inputs before that one is done. (The map takes two kernels.)"""
+    x = randn(gen(22), 2, 40000, 256).half()
+    (a, sa), (w, sw) = operands(ops, gen(23), 2, 256, 8192)
+    big = randn(gen(24), 8192, 8192).half()
+    for _ in range(3):
+        both = torch.zeros((2, 256), device="cuda")
+        torch.cuda.synchronize()
+        ops.quantize_fp8(big)  # keeps the stream busy while the calls below are queued
+        ops.matmul_fp8(a, sa, w, sw, out=both, dtype=torch.float32)
+        got = ops.group_norm(x, 32, both[0], both[1], act=SILU)
+        torch.cuda.synchronize()
+        assert torch.equal(got, ops.group_norm(x, 32, both[0].clone(), both[1].clone(), act=SILU))
+
+
+def test_a_graph_keeps_its_scratch(ops):
+    """A captured call replays after larger calls on its stream."""
+    x = randn(gen(25), 1, 30000, 256).half()
+    side, out = torch.cuda.Stream(), torch.empty_like(x)
+    with torch.cuda.stream(side):
+        want = ops.group_norm(x, 32, act=SILU)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.group_norm(x, 32, act=SILU, out=out)
+    with torch.cuda.stream(side):
+        wide = randn(gen(26), 40, 600, 40003).half()  # one value at a time, a few MB of pairs
+        ops.group_norm(wide, 40003, out=wide)
+        del wide
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_launch_timing(ops):
+    """The launch record covers the operators' handle."""
+    import iec
+
+    x = randn(gen(27), 2, 64, 64, 256).half()
+    w, sw = ops.quantize_fp8(randn(gen(28), 512, 256), 128)
+    iec.set_launch_timing(ops, True)
+    codes, scales = ops.group_norm_fp8(x, 32)
+    ops.matmul_fp8(codes, scales, w, sw)
+    names = [r["name"] for r in iec.launch_timing(ops)]
+    iec.set_launch_timing(ops, False)
+    assert any(n.startswith("norm_") for n in names) and any("8192x512x256" in n for n in names)
+
+
 def test_refusals(ops):
     import iec
 
@@ -431,6 +484,8 @@ def test_refusals(ops):
     refused(lambda: ops.group_norm(x, 4, eps=float("nan")), "eps")
     refused(lambda: ops.group_norm(x, 4, act=9), "activation")
     refused(lambda: ops.group_norm(x.double(), 4), "float64")
+    refused(lambda: ops.group_norm(x.cpu(), 4), "cpu")
+    refused(lambda: ops.group_norm(x, 4, gamma=torch.ones(48)), "gamma", "cpu")
     refused(lambda: ops.group_norm(x, 4, gamma=torch.ones(47, device="cuda")), "gamma")
     refused(lambda: ops.group_norm(x, 4, out=torch.empty((2, 4, 47), **half)), "out")
     refused(lambda: ops.group_norm(x.transpose(1, 2), 4), "channels")
