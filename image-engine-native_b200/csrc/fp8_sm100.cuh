@@ -23,6 +23,14 @@
 // own 32 rows, and the residual comes in the same way while the tile's MMAs
 // run; where the rows of out or residual do not start on 16 bytes, they are
 // written through shared memory with plain accesses. All waits are bounded.
+//
+// What it measured: 16384 x 8192 x 2048 to bf16 274 us in a burst (2,000
+// TFLOP/s), 319 sustained under the power cap; 8192^3 500 us in a burst. The
+// bound is the accumulators' way back: per SM and block 128 x 256 values read
+// from TMEM and added, next to 512 cycles of MMAs (with the loads and MMAs
+// alone, and the output: 226 us). 256 x 256 is the largest tile whose sums (128
+// registers a thread) and two accumulators (512 TMEM columns) fit, and has the
+// least traffic from L2 for its MMAs: 64 bytes a cycle and SM.
 #pragma once
 
 #include "ops_sm100.cuh"

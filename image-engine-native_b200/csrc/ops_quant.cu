@@ -1,8 +1,7 @@
 // Rows of 16- or 32-bit values to e4m3 codes with an f32 scale for each
 // block of 128 values of a row (activations), or of 128 rows and 128 values
 // (weights). Bound by memory: a value is read once, a byte written, some
-// five instructions between. 49152 x 1536 f16 (229 MB): see the figures at
-// quant_rows.
+// five instructions between.
 #include "ops_launch.h"
 #include "ops_sm100.cuh"
 
@@ -63,8 +62,9 @@ __device__ __forceinline__ void store_codes(uint8_t* out, uint4 raw, float facto
     *reinterpret_cast<uint32_t*>(out) = w[0];
 }
 
-// Rows of whole, aligned vectors: 128 / VE lanes an item, one vector each,
-// U items in flight.
+// Rows of whole, aligned vectors: 128 / VE lanes an item, one vector each, U
+// items in flight. 49152 x 1536 f16 (229 MB with codes and scales): 44 us, 5.2
+// TB/s, 80 % of a copy's rate (one warp an item and a division per value: 127).
 template <class T>
 __global__ void __launch_bounds__(QUANT_THREADS) quant_rows(const QuantSpec p, const QuantShape q) {
   constexpr int VE = 16 / (int)sizeof(T), LANES = FP8_BLOCK / VE, U = 4;
