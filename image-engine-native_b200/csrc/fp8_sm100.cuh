@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               more[u][q] = p.residual && r < rows && q < cols ? to_f32(res[q]) : 0.0f;
             }
           }
-#pragma unroll 2
+#pragma unroll 4
           for (int k = 0; k < p.splits; k++)
 #pragma unroll
             for (int u = 0; u < U; u++) {

@@ -68,18 +68,22 @@ __device__ __forceinline__ float2 op_sigmoid_pair(float2 v) {
 }
 
 // GELU as max(v, 0) - |v| / (2 P^16) (igemm_sm100.cuh), |error| at most 1.5e-7
-// |v|: a third of erff's instructions, for results of 16 bits (FAST).
-__device__ __forceinline__ float op_gelu_fast(float v) {
-  const float av = fabsf(v), a = av * 0.70710678118654752f;
-  float q = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(4.30638e-5f, a, 2.765672e-4f), a, 1.520143e-4f), a, 9.2705272e-3f), a,
-                          4.22820123e-2f),
-                     a, 7.05230784e-2f),
-                a, 1.0f);
-  q *= q;
-  q *= q;
-  q *= q;
-  q *= q;
-  return fmaf(-0.5f * av, op_rcp(q), fmaxf(v, 0.0f));
+// |v|, of two values: a third of erff's instructions, for results of 16 bits
+// (FAST).
+__device__ __forceinline__ float2 op_gelu_pair(float2 v) {
+  const float2 av = make_float2(fabsf(v.x), fabsf(v.y)), a = fmul2(av, both(0.70710678118654752f));
+  float2 q = ffma2(both(4.30638e-5f), a, both(2.765672e-4f));
+  q = ffma2(q, a, both(1.520143e-4f));
+  q = ffma2(q, a, both(9.2705272e-3f));
+  q = ffma2(q, a, both(4.22820123e-2f));
+  q = ffma2(q, a, both(7.05230784e-2f));
+  q = ffma2(q, a, both(1.0f));
+  q = fmul2(q, q);
+  q = fmul2(q, q);
+  q = fmul2(q, q);
+  q = fmul2(q, q);
+  return ffma2(fmul2(both(-0.5f), av), make_float2(op_rcp(q.x), op_rcp(q.y)),
+               make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
 }
 
 // The activation of N values. The products that end an activation are not
@@ -91,9 +95,17 @@ __device__ __forceinline__ void op_act_vec(float* v) {
 #pragma unroll
     for (int e = 0; e < N; e++) v[e] = v[e] < 0.0f ? 0.0f : v[e];
   } else if constexpr (ACT == OP_GELU) {
+    if constexpr (FAST) {
 #pragma unroll
-    for (int e = 0; e < N; e++)
-      v[e] = FAST ? op_gelu_fast(v[e]) : __fmul_rn(0.5f * v[e], 1.0f + erff(v[e] * 0.70710678118654752f));
+      for (int e = 0; e < N; e += 2) {
+        const float2 y = op_gelu_pair(make_float2(v[e], v[N == 1 ? e : e + 1]));
+        v[e] = y.x;
+        if (N > 1) v[e + 1] = y.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++) v[e] = __fmul_rn(0.5f * v[e], 1.0f + erff(v[e] * 0.70710678118654752f));
+    }
   } else if constexpr (ACT == OP_SIGMOID || ACT == OP_SILU) {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {

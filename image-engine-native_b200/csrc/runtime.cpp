@@ -208,7 +208,10 @@ DeviceScope::DeviceScope(Device& d) {
     cudaGetLastError();
     prev_ = -1;
   }
-  d.enter();
+  if (prev_ == d.ordinal() && !d.poisoned())
+    prev_ = -1;  // current already: nothing to change, nothing to restore
+  else
+    d.enter();
   prev_device_ = g_scope_device;
   g_scope_device = &d;
 }

@@ -7,6 +7,10 @@ point, for networks built next to the four models.
     w, w_scales = ops.quantize_fp8(weights, block_rows=128)                    # once: n_out, c
     y = ops.matmul_fp8(codes, scales, w, w_scales, bias, residual=x.flatten(0, 2))
 
+Where all outputs are given, a call goes through the compiled binding
+(binding/ops_binding.cpp); what does not fit there comes back here, where
+outputs are allocated and arguments checked one by one.
+
 Tensors are torch tensors of the handle's device. Work is queued on
 torch's current stream unless `stream` (an integer cudaStream_t) is given,
 and the calls return without waiting. There is no CPU fallback.
@@ -20,6 +24,11 @@ from struct import Struct
 import torch
 
 from . import ERR_INPUT, IecError, Options, _check, lib
+
+try:
+    from . import _ops_binding as _fast
+except ImportError as e:
+    raise ImportError("iec/_ops_binding.so is missing: build it with __graft_entry__.build()") from e
 
 NONE, RELU, GELU, SIGMOID, SILU = range(5)
 BLOCK = 128  # values along a row that share a scale
@@ -136,9 +145,13 @@ class Ops:
         opt = Options(device, timeout_ms, 0)
         _check(L.iec_ops_open(ctypes.byref(opt), ctypes.byref(self._h)))
         self._device = L.iec_ops_device(self._h)
+        self._handle = self._h.value  # for the binding; 0 once closed
+        _fast.bind(*(ctypes.cast(f, vp).value for f in (L.iec_ops_group_norm, L.iec_ops_group_norm_fp8,
+                                                        L.iec_ops_quantize_fp8, L.iec_ops_matmul_fp8)))
 
     def close(self):
         if getattr(self, "_h", None):
+            self._handle = 0
             self._lib.iec_ops_free(self._h)
             self._h = None
 
@@ -156,6 +169,12 @@ class Ops:
                    stream=None):
         """Group normalisation and activation of channels-last maps (n, ...,
         c); `out` (default: a new tensor) may be `x`."""
+        if out is not None:
+            status = _fast.group_norm(self._handle, self._device, stream, x, groups, gamma, beta, eps, act, out)
+            if status == 0:
+                return out
+            if status > 0:
+                _check(status)
         dtype = _dtype(x, "x")
         n, pixels, c, step, map_step = _maps(x, self._device, "x")
         if out is None:
@@ -175,6 +194,13 @@ class Ops:
                        scales=None, stream=None):
         """group_norm with its result as 8-bit rows, one per pixel: (codes
         n*pixels x c, scales ceil(c / 128) x n*pixels)."""
+        if codes is not None and scales is not None:
+            status = _fast.group_norm_fp8(self._handle, self._device, stream, x, groups, gamma, beta, eps, act, codes,
+                                          scales)
+            if status == 0:
+                return codes, scales
+            if status > 0:
+                _check(status)
         dtype = _dtype(x, "x")
         n, pixels, c, step, map_step = _maps(x, self._device, "x")
         codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, self._device)
@@ -190,6 +216,12 @@ class Ops:
         """A rows x k matrix as 8-bit rows: (codes rows x k, scales
         ceil(k / 128) x rows), with block_rows 128 (weights) scales
         ceil(k / 128) x ceil(rows / 128)."""
+        if codes is not None and scales is not None:
+            status = _fast.quantize_fp8(self._handle, self._device, stream, x, block_rows, codes, scales)
+            if status == 0:
+                return codes, scales
+            if status > 0:
+                _check(status)
         dtype = _dtype(x, "x")
         shape = x.shape
         if len(shape) != 2:
@@ -210,6 +242,13 @@ class Ops:
         """act(a w^T + bias) + residual for 8-bit rows a (m x k) and w (n x
         k, quantised with block_rows 128); `out` (default: a new tensor of
         `dtype`) may be `residual`."""
+        if out is not None:
+            status = _fast.matmul_fp8(self._handle, self._device, stream, a, a_scales, w, w_scales, bias, act, residual,
+                                      out)
+            if status == 0:
+                return out
+            if status > 0:
+                _check(status)
         a_shape, w_shape = a.shape, w.shape
         if len(a_shape) != 2 or len(w_shape) != 2:
             _bad("a and w must be matrices")

@@ -56,3 +56,20 @@ def test_tensor_views():
     assert ops._rows(codes, (3, 50), torch.float8_e4m3fn, -1, "codes") == 64
     with pytest.raises(iec.IecError):
         ops._rows(codes.t(), (50, 3), torch.float8_e4m3fn, -1, "codes")
+
+
+def test_binding_leaves_what_does_not_fit():
+    """The compiled fast path calls nothing for tensors of another device, of
+    other shapes or types, or for missing arguments: it answers -1."""
+    import torch
+
+    from iec import _ops_binding as fast
+
+    x = torch.zeros(2, 16)
+    assert fast.quantize_fp8(0, 0, 5, x, 1, x, x) == -1
+    assert fast.quantize_fp8(0, 0, 5, None, 1, x, x) == -1
+    assert fast.quantize_fp8(0) == -1
+    assert fast.group_norm(0, 0, 5, x, 1, None, None, 1e-5, 0, x) == -1
+    assert fast.group_norm_fp8(0, 0, 5, x, 1, None, None, 1e-5, 0, x, x) == -1
+    assert fast.matmul_fp8(0, 0, 5, x, x, x, x, None, 0, None, x) == -1
+    assert fast.matmul_fp8("no handle", 0, 5, x, x, x, x, None, 0, None, x) == -1
