@@ -41,12 +41,11 @@ constexpr int NORM_THREADS = 512;
 constexpr int NORM_RING = 2;
 constexpr int APPLY_THREADS = 256;
 
-// A thread's VE values of a pixel as e4m3 codes at `out`, with the scale of
-// their block of 128 at `scale_at` (null but in the block's first thread):
-// the block's threads are 128 / VE consecutive lanes. `live`: the thread's
-// channels exist.
+// A thread's VE values of a pixel as e4m3 codes at `out`; the scale of their
+// block of 128, whose threads are 128 / VE consecutive lanes. `live`: the
+// thread's channels exist.
 template <int VE, bool AL>
-__device__ __forceinline__ void store_fp8(uint8_t* out, float* scale_at, bool live, const float* v) {
+__device__ __forceinline__ float store_fp8(uint8_t* out, bool live, const float* v) {
   constexpr int LANES = FP8_BLOCK / VE;
   float most = 0.0f;
 #pragma unroll
@@ -56,7 +55,7 @@ __device__ __forceinline__ void store_fp8(uint8_t* out, float* scale_at, bool li
   for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
   float factor, scale;
   fp8_scale(top, &factor, &scale);
-  if (!live) return;
+  if (!live) return scale;
   uint32_t w[VE / 4];
 #pragma unroll
   for (int e = 0; e < VE; e += 4) {
@@ -72,7 +71,7 @@ __device__ __forceinline__ void store_fp8(uint8_t* out, float* scale_at, bool li
   } else {
     *reinterpret_cast<uint32_t*>(out) = w[0];
   }
-  if (scale_at) *scale_at = scale;
+  return scale;
 }
 
 __device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
@@ -439,10 +438,12 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       Vec<T, VE, AL>::expand(i < n ? data[i * stride] : make_uint4(0, 0, 0, 0), v);
       affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
-      if (FP8)
-        store_fp8<VE, AL>(codes + i * code_step, scale_at ? scale_at + i * q.rows : nullptr, i < n, v);
-      else
+      if (FP8) {
+        const float sc = store_fp8<VE, AL>(codes + i * code_step, i < n, v);
+        if (scale_at && i < n) scale_at[i * q.rows] = sc;
+      } else {
         Vec<T, VE, AL>::store(out + i * out_step, v);
+      }
     }
   });
   cluster_sync();  // the others have read this CTA's statistics
@@ -626,58 +627,62 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
   const int px = (int)max(0ll, min(span, p.pixels - first));
   constexpr int U = VE == 1 ? 8 : 4;
   const int per = U * rows, full = px / per;
-  const long long x_step = (long long)rows * p.x_stride, out_step = (long long)rows * p.out_stride;
-  // threads without a pixel of their own go through the motions on row 0's
-  const int own = r < rows ? r : 0;
-  const long long at = first + (long long)full * per + own;
+  // A thread's U pixels lie next to each other. Threads without a pixel of
+  // their own go through the motions on row 0's.
+  const long long x_step = (long long)per * p.x_stride, out_step = (long long)per * p.out_stride;
+  const long long code_step = FP8 ? per * (long long)p.q.code_stride : 0;
+  const long long at = first + (long long)full * per + (r < rows ? r : 0) * U, row = map * p.pixels + at;
   const T* x = static_cast<const T*>(p.x) + map * p.x_map_stride + at * p.x_stride + ch;
   T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + at * p.out_stride + ch;
-  const long long row = map * p.pixels + at, code_step = FP8 ? rows * (long long)p.q.code_stride : 0;
   uint8_t* codes = FP8 ? p.q.codes + row * (long long)p.q.code_stride + ch : nullptr;
-  float* scale_at = FP8 && live && ch % FP8_BLOCK == 0
-                        ? p.q.scales + (long long)(ch / FP8_BLOCK) * (long long)p.q.scale_stride + row
+  // lane u of a block stores the u-th pixel's scale
+  const int lane = slot % LANES;
+  float* scale_at = FP8 ? p.q.scales + (long long)((c0 + slot * VE) / FP8_BLOCK) * (long long)p.q.scale_stride + row + lane
                         : nullptr;
+  const bool scales = FP8 && r < rows && lane < U && slot - lane < vecs;
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    auto put = [&](typename V::Raw raw, int u, bool here) {
-      float v[VE];
-      V::expand(raw, v);
-      affine.apply(v);
-      op_act_vec<ACT, FAST, VE>(v);
-      if constexpr (FP8)
-        store_fp8<VE, AL>(codes + u * code_step, scale_at ? scale_at + u * rows : nullptr, here, v);
-      else if (here)
-        V::store(out + u * out_step, v);
+    // U pixels, the first `some` of which exist.
+    auto put = [&](const typename V::Raw* raw, int some) {
+      float mine = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        float v[VE];
+        V::expand(raw[u], v);
+        affine.apply(v);
+        op_act_vec<ACT, FAST, VE>(v);
+        if constexpr (FP8) {
+          const float sc = store_fp8<VE, AL>(codes + u * (long long)p.q.code_stride, live && u < some, v);
+          mine = lane == u ? sc : mine;
+        } else if (live && u < some) {
+          V::store(out + u * p.out_stride, v);
+        }
+      }
+      if (scales && lane < some) *scale_at = mine;
     };
-    // The last pixels, then whole fours of steps, the next ones' loads ahead
-    // of this one's work.
+    // The last pixels, then whole steps, the next one's loads ahead of this
+    // one's work.
     typename V::Raw raw[U], rest[U];
-    const int left = px - full * per;
+    const int some = px - full * per - r * U;
 #pragma unroll
-    for (int u = 0; u < U; u++) rest[u] = live && u * rows + r < left ? V::fetch(x + u * x_step) : V::zero();
+    for (int u = 0; u < U; u++) rest[u] = live && u < some ? V::fetch(x + u * p.x_stride) : V::zero();
     if (full) {
-      x -= U * x_step;
+      x -= x_step;
 #pragma unroll
-      for (int u = 0; u < U; u++) raw[u] = V::fetch(x + u * x_step);
+      for (int u = 0; u < U; u++) raw[u] = V::fetch(x + u * p.x_stride);
     }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (u * rows < left) put(rest[u], u, live && u * rows + r < left);
+    if (px > full * per) put(rest, some);
     if (!FP8 && !live) return;
     for (int f = full; f > 0; f--) {
       typename V::Raw next[U];
-      x -= U * x_step;
+      x -= x_step;
       if (f > 1)
 #pragma unroll
-        for (int u = 0; u < U; u++) next[u] = V::fetch(x + u * x_step);
-      if (FP8) {
-        codes -= U * code_step;
-        if (scale_at) scale_at -= per;
-      } else {
-        out -= U * out_step;
-      }
-#pragma unroll
-      for (int u = 0; u < U; u++) put(raw[u], u, live);
+        for (int u = 0; u < U; u++) next[u] = V::fetch(x + u * p.x_stride);
+      out -= FP8 ? 0 : out_step;
+      codes -= code_step;
+      scale_at -= FP8 ? per : 0;
+      put(raw, U);
 #pragma unroll
       for (int u = 0; u < U; u++) raw[u] = next[u];
     }
