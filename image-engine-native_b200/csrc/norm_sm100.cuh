@@ -566,35 +566,66 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
   };
   const float count = (float)p.pixels * (float)cg;
   const int all = q.chunks * span;
-  float m = 0.0f, d = 0.0f, n0;
-  const float m0 = pair(0, &n0).x;
-  if (all <= 5 * 32) {  // the usual case: all loads at once
-    float2 v[5];
-    float n[5];
-#pragma unroll
-    for (int i = 0; i < 5; i++) {
-      v[i] = make_float2(0.0f, 0.0f);
-      n[i] = 0.0f;
-      if (i * 32 + lane < all) v[i] = pair(i * 32 + lane, &n[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 5; i++) m = fmaf(n[i], v[i].x - m0, m);
-    m = m0 + warp_sum(m) / count;
-#pragma unroll
-    for (int i = 0; i < 5; i++) d += fmaf(n[i] * (v[i].x - m), v[i].x - m, v[i].y);
-  } else {
-    float n;
-    for (int i = lane; i < all; i += 32) {
-      const float2 v = pair(i, &n);
-      m = fmaf(n, v.x - m0, m);
-    }
-    m = m0 + warp_sum(m) / count;
-    for (int i = lane; i < all; i += 32) {
-      const float2 v = pair(i, &n);
-      d += fmaf(n * (v.x - m), v.x - m, v.y);
-    }
+  float m = 0.0f, d = 0.0f, n;
+  const float m0 = pair(0, &n).x;
+  for (int i = lane; i < all; i += 32) {
+    const float2 v = pair(i, &n);
+    m = fmaf(n, v.x - m0, m);
+  }
+  m = m0 + warp_sum(m) / count;
+  for (int i = lane; i < all; i += 32) {
+    const float2 v = pair(i, &n);
+    d += fmaf(n * (v.x - m), v.x - m, v.y);
   }
   return make_float2(m, norm_rstd(warp_sum(d) / count + p.eps));
+}
+
+// The same for the groups g0 .. g1 of a tile into stat[], by a CTA of `warps`
+// warps. Where the map is one tile of at most 160 chunks, four groups at a
+// time: one group's loads, sums and root are a chain of 1.1 us.
+__device__ __forceinline__ void norm_join_all(const NormSpec& p, const NormChunks& q, int z, int g0, int g1, int warps,
+                                              float2* stat) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (q.tiles > 1 || q.chunks > 5 * 32) {
+    for (int g = g0 + warp; g <= g1; g += warps) {
+      const float2 st = norm_join(p, q, z, g);
+      if (lane == 0) stat[g - g0] = st;
+    }
+    return;
+  }
+  const long long chunk = q.span * q.cluster;
+  const float inv = op_rcp((float)p.pixels), cg = (float)(q.join.cg << q.join.shift);
+  float n[5];
+#pragma unroll
+  for (int i = 0; i < 5; i++) n[i] = (float)max(0ll, min(chunk, p.pixels - (i * 32 + lane) * chunk));
+  const float2* part = q.part + (long long)z * q.slots * q.chunks + lane;
+  for (int g = g0 + warp; g <= g1; g += 4 * warps) {
+    float2 v[4][5];
+    float m[4], d[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int i = 0; i < 5; i++) {
+        v[k][i] = make_float2(0.0f, 0.0f);
+        if (i * 32 + lane < q.chunks && g + k * warps <= g1) v[k][i] = part[(g + k * warps) * q.chunks + i * 32];
+      }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float m0 = __shfl_sync(~0u, v[k][0].x, 0);
+      m[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 5; i++) m[k] = fmaf(n[i], v[k][i].x - m0, m[k]);
+      m[k] = fmaf(warp_sum(m[k]), inv, m0);
+      d[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 5; i++) d[k] += fmaf(n[i] * cg * (v[k][i].x - m[k]), v[k][i].x - m[k], v[k][i].y);
+      d[k] = warp_sum(d[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (lane == k && g + k * warps <= g1)
+        stat[g + k * warps - g0] = make_float2(m[k], norm_rstd(d[k] * (inv * op_rcp(cg)) + p.eps));
+  }
 }
 
 template <class T, int VE, bool FP8, bool AL>
@@ -616,10 +647,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
   // (gamma and beta too may come from the kernels before)
   Affine<VE> affine;
   affine.fetch(p, ch, live);
-  for (int g = g0 + (int)(threadIdx.x >> 5); g <= g1; g += APPLY_THREADS / 32) {
-    const float2 st = norm_join(p, q, z, g);
-    if ((threadIdx.x & 31) == 0) stat[g - g0] = st;
-  }
+  norm_join_all(p, q, z, g0, g1, APPLY_THREADS / 32, stat);
   __syncthreads();
   affine.set(stat, ch, g0, cg, q.by_cg);
   const long long span = (p.pixels + gridDim.x - 1) / gridDim.x;
@@ -699,10 +727,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_fp8_odd(const NormSpe
   const int ga = block * FP8_BLOCK / cg, gb = min(block * FP8_BLOCK + FP8_BLOCK - 1, p.c - 1) / cg;
   griddep_launch_dependents();
   griddep_wait();
-  for (int g = ga + warp; g <= gb; g += NORM_THREADS / 32) {
-    const float2 st = norm_join(p, q, z, g);
-    if (lane == 0) stat[g - ga] = st;
-  }
+  norm_join_all(p, q, z, ga, gb, NORM_THREADS / 32, stat);
   __syncthreads();
   float mean[4], scale[4], beta[4];
 #pragma unroll

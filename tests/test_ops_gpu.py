@@ -199,6 +199,31 @@ def test_group_norm_takes_unaligned_maps(ops):
     assert torch.equal(ops.group_norm(x, 8, act=GELU), ops.group_norm(x.clone(), 8, act=GELU))
 
 
+@pytest.mark.parametrize("pixels", [600, 60000])
+@pytest.mark.parametrize("c", [64, 200])
+def test_group_norm_fp8_takes_unaligned_maps(ops, pixels, c):
+    """The same codes and scales from maps and into codes that start anywhere."""
+    base = randn(gen(30), 2 * pixels * (c + 1) + 1).half()
+    x = base[1:].reshape(2, pixels, c + 1)[..., :c]
+    want, scales = ops.group_norm_fp8(x.clone(), 8, act=SILU)
+    got = torch.zeros((2 * pixels, c + 3), device="cuda").to(torch.float8_e4m3fn)[:, 1:c + 1]
+    _, other = ops.group_norm_fp8(x, 8, act=SILU, codes=got)
+    assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)) and torch.equal(other, scales)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("n,pixels,c,groups", [(1, 40, 5000, 4), (2, 300, 5001, 3), (1, 9, 30000, 6000), (3, 2, 65535, 15)])
+def test_group_norm_of_many_channels(ops, n, pixels, c, groups, dtype):
+    """Groups that straddle the kernels' tiles of channels."""
+    g = gen(c)
+    x = (randn(g, n, pixels, c) + randn(g, c)).to(TYPES[dtype])
+    gamma, beta = 1 + 0.3 * randn(g, c), 0.3 * randn(g, c)
+    want, tol = norm64(x, groups, gamma, beta, 1e-5, SILU)
+    within(ops.group_norm(x, groups, gamma, beta, 1e-5, SILU), want, HALF[dtype] * want.abs() + SMALL[dtype] + tol)
+    codes, scales = ops.group_norm_fp8(x, groups, gamma, beta, 1e-5, SILU)
+    check_codes(codes, scales, want.reshape(-1, c), slack=tol.reshape(-1, c))
+
+
 def test_group_norm_is_the_same_every_time(ops):
     x = randn(gen(8), 3, 9000, 128).half()
     first = ops.group_norm(x, 32, act=SILU)
