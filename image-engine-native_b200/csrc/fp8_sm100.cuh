@@ -25,12 +25,14 @@
 // written through shared memory with plain accesses. All waits are bounded.
 //
 // What it measured: 16384 x 8192 x 2048 to bf16 274 us in a burst (2,000
-// TFLOP/s), 319 sustained under the power cap; 8192^3 500 us in a burst. The
+// TFLOP/s), 316 sustained under the power cap; 8192^3 484 and 557 us. The
 // bound is the accumulators' way back: per SM and block 128 x 256 values read
 // from TMEM and added, next to 512 cycles of MMAs (with the loads and MMAs
 // alone, and the output: 226 us). 256 x 256 is the largest tile whose sums (128
 // registers a thread) and two accumulators (512 TMEM columns) fit, and has the
-// least traffic from L2 for its MMAs: 64 bytes a cycle and SM.
+// least traffic from L2 for its MMAs: 64 bytes a cycle and SM. The sums are
+// read 16 columns at a time, the next 16 on their way (32 at a time: 531 us
+// at 8192^3, 64: 535).
 #pragma once
 
 #include "ops_sm100.cuh"

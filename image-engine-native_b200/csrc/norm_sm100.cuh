@@ -21,7 +21,7 @@
 // group; the second joins the chunks' pairs and applies them, walking the
 // pixels backwards, since the last ones are the likeliest to be in L2 still.
 // 2 x 768 x 512 x 128 bf16 (201 MB, twice the size of a map that L2 holds):
-// 119 us, 45 and 75 apart; 8 x 128 x 128 x 256 f16 to e4m3: 49 us.
+// 113 us, 45 and 68 of it; 8 x 128 x 128 x 256 f16 to e4m3: 46 us.
 //
 // Statistics: each thread takes a few pixels at a time from registers, their
 // mean and the squared deviations around it, and joins that to what it has

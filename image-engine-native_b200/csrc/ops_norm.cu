@@ -62,7 +62,7 @@ bool plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, NormResiden
   if (*smem > 224 * 1024) return false;
   // Only where all its clusters run at once: one after another, their loads,
   // statistics and stores take turns (8 x 128 x 128 x 256 f16: 90 us in four
-  // waves of clusters of 16, 52 in chunks through L2). A cluster size that
+  // waves of clusters of 16, 46 in chunks through L2). A cluster size that
   // the GPU's parts divide badly is made smaller.
   constexpr auto codes = norm_resident<T, true, true>;
   constexpr auto wide = norm_resident<T, false, true>;
