@@ -14,7 +14,11 @@
 //
 // 4 x 64 x 64 x 512 f16 with SiLU (34 MB): 11 us, of which the loads take 2.6,
 // the statistics 2 and results and stores 4.5, one after another; a single
-// small map, 16 x 16 x 512: 4.8 us.
+// small map, 16 x 16 x 512: 4.8 us. To e4m3, where groups end inside blocks
+// of 128 channels, segments of whole groups and blocks are long and few; CTAs
+// then write single blocks and read the groups around them twice (32 x 32 x
+// 768, groups of 24: 6.4 us in 6 x 16 CTAs, 9.7 in 2 x 16; 32 x 32 x 640,
+// groups of 20: 6.7 against 13.6).
 //
 // norm_stats + norm_apply: larger maps. The first kernel reduces chunks of
 // pixels, a cluster of CTAs each, to (mean, sum of squared deviations) per
@@ -317,12 +321,19 @@ struct Affine {
 __device__ __forceinline__ float norm_rstd(float v) { return rsqrtf(v); }
 
 // ---------------------------------------------------------------- resident
+// A CTA writes a segment of seg_c channels and reads its window: the segment
+// and, where groups cross its ends (only with fp8, whose x nobody writes),
+// the vectors around it that complete them. Two CTAs then both read what lies
+// between; in return segments may be as short as a block of 128 channels.
 struct NormResident {
-  int seg_c, vecs, rows;  // channels of a segment, their vectors, pixels a CTA takes per step
-  int slots;              // threads of a pixel: vecs, rounded up to whole blocks of 128 channels with fp8
-  int pixels;             // of a CTA
-  int groups;             // of a segment
-  FastDiv by_slots, by_rows, by_cg;
+  int seg_c, rows;  // channels of a segment, pixels a CTA takes per step
+  int vecs[2];      // vectors of a window, of the last one
+  int slots;        // threads of a pixel: a segment's vectors, rounded up to whole blocks of 128 channels with fp8
+  int parted;       // segments end inside groups
+  int around;       // then, behind all pixels' slots, threads of a pixel for the window's other vectors
+  int pixels;       // of a CTA
+  int groups;       // room for a window's
+  FastDiv by_slots, by_around, by_rows, by_cg;
   NormJoin join;
 };
 
@@ -333,21 +344,46 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   extern __shared__ __align__(16) uint8_t smem[];
   const int rank = blockIdx.x, ctas = gridDim.x, seg = blockIdx.y, map = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cg = q.join.cg << q.join.shift, groups = q.groups;
+  const int cg = q.join.cg << q.join.shift;
   const int steps = (int)q.by_rows.div((uint32_t)(q.pixels + q.rows - 1));
+  // The window: `vecs` vectors from channel `lo`, `left` of them before the
+  // segment's `own_vecs`; channel c0 and group g0 as counted from where groups
+  // begin. The outer two groups may be in part.
+  const int ch0 = seg * q.seg_c;
+  bool last = false;
+  int vecs = q.vecs[0], own_vecs = vecs, lo = ch0, left = 0, c0 = 0, g0 = 0, groups = q.groups;
+  if (FP8 && q.parted) {
+    last = seg == (int)gridDim.y - 1;
+    vecs = q.vecs[last];
+    own_vecs = min(q.seg_c, p.c - ch0) / VE;
+    c0 = lo = min((int)q.by_cg.div((uint32_t)ch0) * cg / VE * VE, p.c - vecs * VE);
+    left = (ch0 - lo) / VE;
+    g0 = (int)q.by_cg.div((uint32_t)lo);
+    groups = (int)q.by_cg.div((uint32_t)(lo + vecs * VE - 1)) - g0 + 1;
+  }
   // [pixel][vector], the threads' statistics, the groups' statistics over this
   // CTA and their mean and rstd over the cluster.
-  const int stride = q.rows * q.vecs;  // vectors of a step
-  float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * stride * 16);
+  const int stride = q.rows * vecs;  // vectors of a step
+  float* tmean = reinterpret_cast<float*>(smem + (size_t)steps * q.rows * q.vecs[0] * 16);
   float* tdev = tmean + NORM_THREADS * VE;
   float* entries = tdev + NORM_THREADS * VE;
   float2* own = reinterpret_cast<float2*>(entries + 3 * norm_entries(q.join.runs[0]));
-  float2* stat = own + (groups + 1) / 2 * 2;
-  const int r = (int)q.by_slots.div(threadIdx.x), slot = (int)threadIdx.x - r * q.slots;
-  const bool live = r < q.rows && slot < q.vecs;
-  uint4* data = reinterpret_cast<uint4*>(smem) + r * q.vecs + slot;
+  float2* stat = own + (q.groups + 1) / 2 * 2;
+  int r = (int)q.by_slots.div(threadIdx.x), vec = (int)threadIdx.x - r * q.slots;
+  const bool mine = r < q.rows && vec < own_vecs;  // a vector of the segment
+  bool live = mine;
+  if (FP8 && q.parted && r >= q.rows) {
+    const int u = (int)threadIdx.x - q.rows * q.slots;
+    r = (int)q.by_around.div((uint32_t)u);
+    vec = u - r * q.around;
+    live = r < q.rows && vec < vecs - own_vecs;
+    if (vec >= left) vec += own_vecs;
+  } else if (FP8) {
+    vec += left;
+  }
+  uint4* data = reinterpret_cast<uint4*>(smem) + r * vecs + vec;
   const int first = rank * q.pixels, px = max(0, (int)min((long long)q.pixels, p.pixels - first));
-  const int ch = seg * q.seg_c + slot * VE;
+  const int ch = lo + vec * VE;
   const int n = live && r < px ? (int)q.by_rows.div((uint32_t)(px - r + q.rows - 1)) : 0;  // this thread's vectors
   griddep_launch_dependents();
   griddep_wait();
@@ -368,7 +404,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   Affine<VE> affine;
-  affine.fetch(p, ch, live);
+  affine.fetch(p, ch, mine);
   using V = Vec<T, VE, AL>;
   Running<VE> run;
   auto add_until = [&](int end) {
@@ -397,12 +433,12 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
   cp_async_wait<0>();
   add_until(n);
   if (live) {
-    const int at = r * q.join.runs[0] + (slot * VE >> q.join.shift);
+    const int at = r * q.join.runs[last] + (vec * VE >> q.join.shift);
     store_runs<VE>(run, q.join.shift, tmean + at, tdev + at);
   }
   if (px > 0)
-    join_threads(q.join, false, tmean, tdev, entries, px, 0,
-                 [&](int g, float m, float d) { own[g] = make_float2(m, d); });
+    join_threads(q.join, last, tmean, tdev, entries, px, c0 >> q.join.shift,
+                 [&](int g, float m, float d) { own[g - g0] = make_float2(m, d); });
   cluster_sync();
   const float inv = op_rcp((float)p.pixels * (float)cg);
 #pragma unroll 1
@@ -420,14 +456,14 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     if (lane == 0) stat[g] = make_float2(m, norm_rstd(dev * inv + p.eps));
   }
   __syncthreads();
-  affine.set(stat, live ? slot * VE : 0, 0, cg, q.by_cg);
+  affine.set(stat, mine ? c0 + vec * VE : c0, g0, cg, q.by_cg);
   op_act_switch(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     // with fp8 the lanes of a block go through the shuffles together
-    const int end = FP8 ? steps : n;
+    const int end = !FP8 ? n : warp * 32 < q.rows * q.slots ? steps : 0;
     const long long row0 = map * p.pixels + first + r, code_step = q.rows * (long long)p.q.code_stride;
     uint8_t* codes = FP8 ? p.q.codes + row0 * (long long)p.q.code_stride + ch : nullptr;
-    float* scale_at = FP8 && ch % FP8_BLOCK == 0
+    float* scale_at = FP8 && mine && ch % FP8_BLOCK == 0
                           ? p.q.scales + (long long)(ch / FP8_BLOCK) * (long long)p.q.scale_stride + row0
                           : nullptr;
     T* out = FP8 ? nullptr : static_cast<T*>(p.out) + map * p.out_map_stride + (first + r) * p.out_stride + ch;
@@ -439,7 +475,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       affine.apply(v);
       op_act_vec<ACT, FAST, VE>(v);
       if (FP8) {
-        const float sc = store_fp8<VE, AL>(codes + i * code_step, i < n, v);
+        const float sc = store_fp8<VE, AL>(codes + i * code_step, mine && i < n, v);
         if (scale_at && i < n) scale_at[i * q.rows] = sc;
       } else {
         Vec<T, VE, AL>::store(out + i * out_step, v);

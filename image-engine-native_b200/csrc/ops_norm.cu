@@ -31,66 +31,119 @@ NormJoin join_shape(int cg, int c, int c_last, int rows) {
   return j;
 }
 
-// The resident kernel's shape with segments of `seg` channels, or false where
-// one outgrows a cluster.
+// The vectors that cover the whole groups of the segments of `seg` channels,
+// the most of any and those of the last one.
+template <int VE>
+void window_vecs(int c, int cg, int seg, int* vecs) {
+  const int segs = (c + seg - 1) / seg;
+  // where segments begin in a group repeats
+  const int every = std::min(segs - 1, cg / std::gcd(cg, seg));
+  auto width = [&](int s) {
+    const int lo = s * seg / cg * cg / VE, hi = std::min(c, ((std::min(c, (s + 1) * seg) + cg - 1) / cg * cg + VE - 1) / VE * VE);
+    return hi / VE - lo;
+  };
+  vecs[1] = vecs[0] = width(segs - 1);
+  for (int s = 0; s < every; s++) vecs[0] = std::max(vecs[0], width(s));
+}
+
+// The resident kernel's shape with segments of `seg` channels, of whole
+// groups or not (`around`: they may end inside one, the last one may be short), and its cost, vectors that a CTA reads and
+// writes; or a cost of zero where it does not fit.
+struct ResidentPlan {
+  NormResident q;
+  int cluster;
+  size_t smem;
+  long long cost;
+};
+
 template <class T>
-bool plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, NormResident* q, int* cluster, size_t* smem) {
+ResidentPlan plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, bool around) {
   constexpr int VE = 16 / (int)sizeof(T);
-  const int cg = p.c / p.groups, lanes = fp8 ? FP8_BLOCK / VE : 1;
-  q->seg_c = seg;
-  q->vecs = seg / VE;
-  q->slots = (q->vecs + lanes - 1) / lanes * lanes;
-  if (q->slots > NORM_THREADS || p.pixels > (1 << 23)) return false;
-  q->rows = NORM_THREADS / q->slots;
-  const int segs = p.c / seg, most_steps = RESIDENT_BYTES / (q->rows * q->vecs * 16);
-  const long long need = (p.pixels + (long long)most_steps * q->rows - 1) / ((long long)most_steps * q->rows);
-  if (need > CLUSTER || segs > 65535) return false;
-  // as many CTAs as fill the GPU, but at least two steps each
+  const int cg = p.c / p.groups, lanes = fp8 ? FP8_BLOCK / VE : 1, segs = (p.c + seg - 1) / seg;
+  ResidentPlan f = {};
+  NormResident& q = f.q;
+  q.seg_c = seg;
+  q.vecs[0] = q.vecs[1] = seg / VE;
+  q.slots = (seg / VE + lanes - 1) / lanes * lanes;
+  if (around) {
+    q.parted = 1;
+    window_vecs<VE>(p.c, cg, seg, q.vecs);
+    q.around = std::max(q.vecs[0] - seg / VE, q.vecs[1] - (p.c - (segs - 1) * seg) / VE);
+  }
+  if (q.slots + q.around > NORM_THREADS || p.pixels > (1 << 23)) return f;
+  q.rows = NORM_THREADS / (q.slots + q.around);
+  const int most_steps = RESIDENT_BYTES / (q.rows * q.vecs[0] * 16);
+  const long long need = (p.pixels + (long long)most_steps * q.rows - 1) / ((long long)most_steps * q.rows);
+  if (need > CLUSTER || segs > 65535) return f;
+  q.groups = around ? (q.vecs[0] * VE + cg - 1) / cg + 1 : seg / cg;
+  q.by_slots = FastDiv((uint32_t)q.slots);
+  q.by_around = FastDiv((uint32_t)std::max(1, q.around));
+  q.by_rows = FastDiv((uint32_t)q.rows);
+  q.by_cg = FastDiv((uint32_t)cg);
+  q.join = join_shape<VE>(cg, q.vecs[0] * VE, q.vecs[1] * VE, q.rows);
+  // As many CTAs as fill the GPU, but at least two steps each; a cluster size
+  // that the GPU's parts divide badly is made smaller. Only where all clusters
+  // run at once: one after another, their loads, statistics and stores take
+  // turns (8 x 128 x 128 x 256 f16: 90 us in four waves of clusters of 16, 46
+  // in chunks through L2).
   const long long spread = dev.sms() / std::max<long long>(1, (long long)segs * p.n);
-  const long long fill = (p.pixels + 2LL * q->rows - 1) / (2LL * q->rows);
-  const int n = (int)std::max<long long>(1, std::max(need, std::min({spread, fill, (long long)CLUSTER})));
-  q->pixels = (int)((p.pixels + n - 1) / n);
-  *cluster = n;
-  const int steps = (q->pixels + q->rows - 1) / q->rows;
-  q->groups = seg / cg;
-  q->by_slots = FastDiv((uint32_t)q->slots);
-  q->by_rows = FastDiv((uint32_t)q->rows);
-  q->by_cg = FastDiv((uint32_t)cg);
-  q->join = join_shape<VE>(cg, seg, seg, q->rows);
-  *smem = (size_t)steps * q->rows * q->vecs * 16 + (size_t)NORM_THREADS * VE * 8 +
-          (size_t)norm_entries(q->join.runs[0]) * 12 + (size_t)(q->groups + 1) * 16;
-  if (*smem > 224 * 1024) return false;
-  // Only where all its clusters run at once: one after another, their loads,
-  // statistics and stores take turns (8 x 128 x 128 x 256 f16: 90 us in four
-  // waves of clusters of 16, 46 in chunks through L2). A cluster size that
-  // the GPU's parts divide badly is made smaller.
+  const long long fill = (p.pixels + 2LL * q.rows - 1) / (2LL * q.rows);
   constexpr auto codes = norm_resident<T, true, true>;
   constexpr auto wide = norm_resident<T, false, true>;
-  auto room = [&](int size) {
-    return fp8 ? resident_ctas<codes>(dev, NORM_THREADS, *smem, size)
-               : resident_ctas<wide>(dev, NORM_THREADS, *smem, size);
-  };
-  return (long long)n * segs * p.n <= room(n);
+  for (long long n = std::max<long long>({1, need, std::min({spread, fill, (long long)CLUSTER})}); n >= std::max(1LL, need); n--) {
+    q.pixels = (int)((p.pixels + n - 1) / n);
+    const int steps = (q.pixels + q.rows - 1) / q.rows;
+    f.smem = (size_t)steps * q.rows * q.vecs[0] * 16 + (size_t)NORM_THREADS * VE * 8 +
+             (size_t)norm_entries(q.join.runs[0]) * 12 + (size_t)(q.groups + 1) * 16;
+    if (f.smem > 224 * 1024) break;
+    const int room = fp8 ? resident_ctas<codes>(dev, NORM_THREADS, f.smem, (int)n)
+                         : resident_ctas<wide>(dev, NORM_THREADS, f.smem, (int)n);
+    if (n * segs * p.n <= room) {
+      f.cluster = (int)n;
+      f.cost = (long long)q.pixels * (q.vecs[0] + seg / VE);
+      break;
+    }
+  }
+  return f;
 }
 
 // The resident kernel's shape: segments of whole groups and vectors (and with
 // fp8 whole blocks), the smallest that have 128 bytes, so that they read
-// whole lines and there are many clusters; else the largest below that.
+// whole lines and there are many clusters; else the largest below that. With
+// fp8, where groups and blocks share no small multiple, segments of one or two
+// blocks and what is around them, if each CTA has less to do then (1 x 64 x
+// 64 x 320 f16: 11.6 us in three clusters of 16, 22.8 in one). CTAs that have
+// too much to do of a small map lose against the chunks on all SMs: a resident
+// CTA takes 5 us and 0.8 ns a vector, chunks 12 us and 1.06 per million values
+// (1 x 96 x 96 x 384: 18.2 in three clusters, 15.8 in chunks).
 template <class T>
-bool plan_resident(Device& dev, const NormSpec& p, bool fp8, NormResident* q, int* cluster, size_t* smem) {
+ResidentPlan plan_resident(Device& dev, const NormSpec& p, bool fp8) {
   constexpr int VE = 16 / (int)sizeof(T);
   long long unit = std::lcm<long long>(p.c / p.groups, VE);
   if (fp8) unit = std::lcm<long long>(unit, FP8_BLOCK);
-  if (unit >= p.c || p.c % unit) return plan_segment<T>(dev, p, fp8, p.c, q, cluster, smem);
-  const long long line = 128 / sizeof(T);
-  for (long long seg = (line + unit - 1) / unit * unit; seg <= p.c; seg += unit)
-    if (p.c % seg == 0) {
-      if (plan_segment<T>(dev, p, fp8, (int)seg, q, cluster, smem)) return true;
-      break;
+  ResidentPlan best = {};
+  if (unit >= p.c || p.c % unit) {
+    best = plan_segment<T>(dev, p, fp8, p.c, false);
+  } else {
+    const long long line = 128 / sizeof(T);
+    for (long long seg = (line + unit - 1) / unit * unit; seg <= p.c && !best.cost; seg += unit)
+      if (p.c % seg == 0) {
+        best = plan_segment<T>(dev, p, fp8, (int)seg, false);
+        break;
+      }
+    for (long long seg = (line - 1) / unit * unit; seg >= unit && !best.cost; seg -= unit)
+      if (p.c % seg == 0) {
+        best = plan_segment<T>(dev, p, fp8, (int)seg, false);
+        break;
+      }
+  }
+  if (fp8)
+    for (int seg = FP8_BLOCK; seg <= 2 * FP8_BLOCK && seg < p.c && (unit > seg || p.c % unit); seg += FP8_BLOCK) {
+      const ResidentPlan f = plan_segment<T>(dev, p, fp8, seg, true);
+      if (f.cost && (!best.cost || f.cost < best.cost)) best = f;
     }
-  for (long long seg = (line - 1) / unit * unit; seg >= unit; seg -= unit)
-    if (p.c % seg == 0) return plan_segment<T>(dev, p, fp8, (int)seg, q, cluster, smem);
-  return false;
+  if (fp8 && best.cost > 9000 + p.n * p.pixels * p.c / 768) best.cost = 0;
+  return best;
 }
 
 template <class T, int VE, bool AL>
@@ -163,21 +216,19 @@ template <class T, bool AL>
 void run_vectors(Device& dev, const NormSpec& p, cudaStream_t s) {
   constexpr int VE = 16 / (int)sizeof(T);
   const bool fp8 = p.out == nullptr;
-  NormResident q;
-  int cluster = 1;
-  size_t smem = 0;
   constexpr auto wide = norm_resident<T, false, AL>;
   constexpr auto codes = norm_resident<T, true, AL>;
-  if (!plan_resident<T>(dev, p, fp8, &q, &cluster, &smem)) return run_chunks<T, VE, AL>(dev, p, s);
+  const ResidentPlan f = plan_resident<T>(dev, p, fp8);
+  if (!f.cost) return run_chunks<T, VE, AL>(dev, p, s);
   const double values = (double)p.n * p.pixels * p.c;
   timed_launch("norm_resident", 12 * values, values * (sizeof(T) + (fp8 ? 1 : sizeof(T))), s, [&] {
-    const dim3 grid(cluster, p.c / q.seg_c, p.n);
+    const dim3 grid(f.cluster, (p.c + f.q.seg_c - 1) / f.q.seg_c, p.n);
     if (fp8) {
-      allow_smem<codes>(dev, smem);
-      launch_ops(codes, grid, NORM_THREADS, smem, cluster, s, p, q);
+      allow_smem<codes>(dev, f.smem);
+      launch_ops(codes, grid, NORM_THREADS, f.smem, f.cluster, s, p, f.q);
     } else {
-      allow_smem<wide>(dev, smem);
-      launch_ops(wide, grid, NORM_THREADS, smem, cluster, s, p, q);
+      allow_smem<wide>(dev, f.smem);
+      launch_ops(wide, grid, NORM_THREADS, f.smem, f.cluster, s, p, f.q);
     }
   });
 }

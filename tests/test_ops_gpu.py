@@ -150,6 +150,39 @@ def test_group_norm_fp8(ops, n, pixels, c, groups, pad, act, affine, dtype):
     check_codes(codes, scales, want.reshape(-1, c), slack=tol.reshape(-1, c))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("n,pixels,c,groups", [
+    (1, 1024, 320, 32), (1, 1024, 960, 32), (2, 700, 768, 32), (1, 333, 992, 8),
+    (1, 3, 1032, 3), (1, 1, 640, 32), (1, 90, 136, 17), (2, 500, 200, 8), (1, 2000, 416, 32),
+    (1, 2304, 192, 6), (3, 400, 1000, 8), (1, 600, 1288, 7), (1, 64, 8184, 682), (1, 257, 264, 1)])
+def test_group_norm_fp8_of_groups_across_blocks(ops, n, pixels, c, groups, dtype):
+    """Groups that end inside the blocks of 128 channels, last blocks cut short."""
+    g = gen(n + pixels + c + groups)
+    wide = (randn(g, n, pixels, c + 8) + randn(g, c + 8)).to(TYPES[dtype])
+    x = wide[..., :c]
+    gamma, beta = 1 + 0.3 * randn(g, c), 0.3 * randn(g, c)
+    want, tol = norm64(x, groups, gamma, beta, 1e-5, SILU)
+    codes, scales = ops.group_norm_fp8(x, groups, gamma, beta, 1e-5, SILU)
+    check_codes(codes, scales, want.reshape(-1, c), slack=tol.reshape(-1, c))
+    again, same = ops.group_norm_fp8(x, groups, gamma, beta, 1e-5, SILU)
+    assert torch.equal(codes.view(torch.uint8), again.view(torch.uint8)) and torch.equal(scales, same)
+    # unaligned rows, the same bits
+    odd = torch.empty(n, pixels, c + 1, device="cuda", dtype=x.dtype)[..., 1:]
+    odd.copy_(x)
+    into = torch.zeros((n * pixels, c + 3), device="cuda").to(torch.float8_e4m3fn)[:, 1:c + 1]
+    _, same = ops.group_norm_fp8(odd, groups, gamma, beta, 1e-5, SILU, codes=into)
+    assert torch.equal(codes.view(torch.uint8), into.view(torch.uint8)) and torch.equal(scales, same)
+
+
+def test_group_norm_fp8_keeps_what_is_not_finite_within_its_group(ops):
+    """Segments read their neighbours' channels; only the group's own count."""
+    x = randn(gen(8), 1, 700, 320).half()
+    x[0, 350, 125] = float("nan")  # group 12 of 10 channels, 120 to 129: both sides of a block's end
+    codes, _ = ops.group_norm_fp8(x, 32)
+    nan = torch.isnan(codes.float())  # through their scales, all of both blocks; none of the third
+    assert nan[:, :256].all() and not nan[:, 256:].any()
+
+
 @pytest.mark.parametrize("offset", [100.0, -3000.0])
 def test_group_norm_keeps_its_digits_far_from_zero(ops, offset):
     """A mean thousands of deviations from zero: a variance from the mean of
