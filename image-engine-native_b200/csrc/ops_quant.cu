@@ -114,31 +114,65 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_rows(const QuantSpec p, c
   }
 }
 
-// Any rows: a warp an item, four values a lane, 32 apart.
+// Four values of a row from `col` on, wherever it starts; beyond its end the
+// last one again, which leaves the block's maximum as it is. (Each load has an
+// address of its own and stands under no condition: many are under way.)
 template <class T>
+__device__ __forceinline__ void load_four(const T* row, int block, int lane, int k, T* v) {
+  const int col = block * FP8_BLOCK + lane * 4;
+  if ((block + 1) * FP8_BLOCK <= k) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = row[col + e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = row[min(col + e, k - 1)];
+  }
+}
+template <class T>
+__device__ __forceinline__ uint32_t four_top(const T* v) {
+  float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) most = max_abs(to_f32(v[e]), most);
+  return abs_bits(most);
+}
+// Their codes; `words`: rows of codes start on words.
+template <class T>
+__device__ __forceinline__ void store_four(uint8_t* row, int col, int k, bool words, const T* v, float factor) {
+  const uint32_t w = (uint32_t)e4m3x2(to_f32(v[0]) * factor, to_f32(v[1]) * factor) |
+                     (uint32_t)e4m3x2(to_f32(v[2]) * factor, to_f32(v[3]) * factor) << 16;
+  if (words && col + 4 <= k) {
+    *reinterpret_cast<uint32_t*>(row + col) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (col + e < k) row[col + e] = (uint8_t)(w >> (8 * e));
+  }
+}
+__device__ __forceinline__ bool on_words(const Fp8Out& q) {
+  return ((reinterpret_cast<uintptr_t>(q.codes) | (uintptr_t)q.code_stride) & 3) == 0;
+}
+
+// Any rows: a warp an item, four values a lane, U items at a time (6607 x 7287
+// bf16: 48 us; with two items, a lane's values 32 apart and codes stored one by
+// one: 65).
+template <class T, int U>
 __global__ void __launch_bounds__(QUANT_THREADS) quant_rows_odd(const QuantSpec p, const QuantShape q) {
-  constexpr int U = 2;
   griddep_launch_dependents();
   griddep_wait();
   long long item = ((long long)blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
   const int lane = threadIdx.x % 32;
+  const bool words = on_words(p.q);
   long long row = item / q.blocks;
   int block = (int)(item - row * q.blocks);
   while (item < q.items) {
-    float v[U][4];
+    T v[U][4];
     long long rows[U];
     int blocks[U];
-    bool here[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       rows[u] = row;
       blocks[u] = block;
-      here[u] = item < q.items;
-      const T* x = static_cast<const T*>(p.x) + row * p.x_stride + block * FP8_BLOCK + lane;
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        v[u][j] = here[u] && block * FP8_BLOCK + j * 32 + lane < p.k ? to_f32(x[j * 32]) : 0.0f;
-      item += q.stride;
+      load_four(static_cast<const T*>(p.x) + min(row, p.rows - 1) * p.x_stride, block, lane, p.k, v[u]);
       row += q.stride_rows;
       block += q.stride_blocks;
       if (block >= q.blocks) {
@@ -146,20 +180,51 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_rows_odd(const QuantSpec 
         row++;
       }
     }
+    item += U * q.stride;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (!here[u]) break;
+      if (rows[u] >= p.rows) break;
+      float factor, scale;
+      fp8_scale(__reduce_max_sync(~0u, four_top(v[u])), &factor, &scale);
+      store_four(p.q.codes + rows[u] * (long long)p.q.code_stride, blocks[u] * FP8_BLOCK + lane * 4, p.k, words, v[u],
+                 factor);
+      if (lane == 0) p.q.scales[blocks[u] * (long long)p.q.scale_stride + rows[u]] = scale;
+    }
+  }
+}
+
+// Rows of one block: a warp a row, a lane's values 32 apart, so that in short
+// rows most lanes have some (40000 x 31 f16: 6.4 us, 9.3 side by side).
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_rows_short(const QuantSpec p, const QuantShape q) {
+  constexpr int U = 2;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x % 32;
+  for (long long row = ((long long)blockIdx.x * QUANT_THREADS + threadIdx.x) / 32; row < p.rows; row += U * q.stride) {
+    float v[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const T* x = static_cast<const T*>(p.x) + (row + u * q.stride) * p.x_stride + lane;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        v[u][j] = row + u * q.stride < p.rows && j * 32 + lane < p.k ? to_f32(x[j * 32]) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const long long at = row + u * q.stride;
+      if (at >= p.rows) break;
       float most = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; j++) most = max_abs(v[u][j], most);
       float factor, scale;
       fp8_scale(__reduce_max_sync(~0u, abs_bits(most)), &factor, &scale);
-      uint8_t* out = p.q.codes + rows[u] * (long long)p.q.code_stride + blocks[u] * FP8_BLOCK + lane;
+      uint8_t* out = p.q.codes + at * (long long)p.q.code_stride + lane;
       const uint32_t a = e4m3x2(v[u][0] * factor, v[u][1] * factor), b = e4m3x2(v[u][2] * factor, v[u][3] * factor);
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        if (blocks[u] * FP8_BLOCK + j * 32 + lane < p.k) out[j * 32] = (uint8_t)((j < 2 ? a : b) >> (8 * (j & 1)));
-      if (lane == 0) p.q.scales[blocks[u] * (long long)p.q.scale_stride + rows[u]] = scale;
+        if (j * 32 + lane < p.k) out[j * 32] = (uint8_t)((j < 2 ? a : b) >> (8 * (j & 1)));
+      if (lane == 0) p.q.scales[at] = scale;
     }
   }
 }
@@ -202,27 +267,30 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_blocks(const QuantSpec p)
   if (threadIdx.x == 0) p.q.scales[blockIdx.x * (long long)p.q.scale_stride + blockIdx.y] = scale;
 }
 
-// The same for any rows, a value at a time, read twice.
+// The same for any rows, four values a lane (62949 x 587 bf16: 45 us; a
+// column a thread, read twice: 64).
 template <class T>
 __global__ void __launch_bounds__(QUANT_THREADS) quant_blocks_odd(const QuantSpec p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int ROWS = QUANT_THREADS / FP8_BLOCK, U = 8;
-  const int col = blockIdx.x * FP8_BLOCK + threadIdx.x % FP8_BLOCK;
-  const long long row0 = (long long)blockIdx.y * FP8_BLOCK;
-  const int rows = (int)min((long long)FP8_BLOCK, p.rows - row0);
-  const T* x = static_cast<const T*>(p.x) + row0 * p.x_stride + col;
-  uint8_t* out = p.q.codes + row0 * (long long)p.q.code_stride + col;
-  float most = 0.0f;
-  if (col < p.k)
-#pragma unroll U
-    for (int r = threadIdx.x / FP8_BLOCK; r < rows; r += ROWS) most = max_abs(to_f32(x[r * p.x_stride]), most);
+  constexpr int ROWS = QUANT_THREADS / 32, N = FP8_BLOCK / ROWS;
+  const int lane = threadIdx.x % 32;
+  const long long row = (long long)blockIdx.y * FP8_BLOCK + threadIdx.x / 32;
+  const bool words = on_words(p.q);
+  T v[N][4];
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    load_four(static_cast<const T*>(p.x) + min(row + i * ROWS, p.rows - 1) * p.x_stride, (int)blockIdx.x, lane, p.k, v[i]);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) top = max(top, four_top(v[i]));
   float factor, scale;
-  fp8_scale(cta_max(abs_bits(most)), &factor, &scale);
-  if (col < p.k)
-#pragma unroll U
-    for (int r = threadIdx.x / FP8_BLOCK; r < rows; r += ROWS)
-      out[r * (long long)p.q.code_stride] = (uint8_t)e4m3x2(to_f32(x[r * p.x_stride]) * factor, 0.0f);
+  fp8_scale(cta_max(top), &factor, &scale);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (row + i * ROWS < p.rows)
+      store_four(p.q.codes + (row + i * ROWS) * (long long)p.q.code_stride, (int)blockIdx.x * FP8_BLOCK + lane * 4, p.k,
+                 words, v[i], factor);
   if (threadIdx.x == 0) p.q.scales[blockIdx.x * (long long)p.q.scale_stride + blockIdx.y] = scale;
 }
 
@@ -238,18 +306,24 @@ void run(Device& dev, const QuantSpec& p, cudaStream_t s) {
       QuantShape q;
       q.blocks = blocks;
       // a warp an item
-      const int column = wide ? QUANT_UNROLL * 32 * VE / FP8_BLOCK : 1, per = QUANT_THREADS / 32, unroll = wide ? 1 : 2;
+      const int column = wide ? QUANT_UNROLL * 32 * VE / FP8_BLOCK : 1, per = QUANT_THREADS / 32;
       q.items = (p.rows + column - 1) / column * blocks;
-      // eight CTAs an SM, or fewer where the items run out
-      const long long want = (q.items + per * unroll - 1) / (per * unroll);
-      const int grid = (int)std::max<long long>(1, std::min<long long>(want, 8LL * dev.sms()));
+      // as many CTAs an SM as fit, or fewer where the items run out; several
+      // items at a time only where each warp has them
+      const long long want = (q.items + per - 1) / per, most = 8LL * dev.sms();
+      const bool brief = !wide && blocks == 1, few = brief || want <= 8 * most;
+      const int grid = (int)std::max<long long>(1, std::min<long long>(want, wide || few ? most : most / 2));
       q.stride = (long long)grid * per;
       q.stride_rows = q.stride / blocks;
       q.stride_blocks = (int)(q.stride - q.stride_rows * blocks);
       if (wide)
         launch_pdl(quant_rows<T>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
+      else if (brief)
+        launch_pdl(quant_rows_short<T>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
+      else if (few)
+        launch_pdl(quant_rows_odd<T, 1>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
       else
-        launch_pdl(quant_rows_odd<T>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
+        launch_pdl(quant_rows_odd<T, 4>, dim3(grid), dim3(QUANT_THREADS), 0, s, p, q);
     } else {
       const long long row_blocks = (p.rows + FP8_BLOCK - 1) / FP8_BLOCK;
       // a grid is at most 65535 high

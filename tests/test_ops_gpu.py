@@ -279,6 +279,27 @@ def test_quantize(ops, rows, k, block_rows, dtype):
     check_codes(*ops.quantize_fp8(whole, block_rows), x.double(), block_rows)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("rows,k,block_rows", [(20000, 648, 1), (90001, 104, 1), (301, 1024, 1), (9000, 16, 1),
+                                               (700, 648, 128), (129, 8, 128)])
+def test_quantize_takes_rows_that_start_anywhere(ops, rows, k, block_rows, dtype):
+    """The same codes and scales as from aligned rows, also of what is not
+    finite, and into codes that start anywhere."""
+    base = randn(gen(rows + k), rows, k + 1).to(TYPES[dtype])
+    base[rows // 2, 3] = float("inf")
+    base[rows - 1, k] = float("nan")
+    base[0] = 0
+    x = base[:, 1:]
+    want, want_scales = ops.quantize_fp8(x.contiguous(), block_rows)
+    got, scales = ops.quantize_fp8(x, block_rows)
+    assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    assert torch.equal(scales.view(torch.int32), want_scales.view(torch.int32))
+    wide = torch.zeros((rows, k + 3), device="cuda").to(torch.float8_e4m3fn)
+    ops.quantize_fp8(x, block_rows, codes=wide[:, 1:k + 1])
+    assert torch.equal(wide[:, 1:k + 1].view(torch.uint8), want.view(torch.uint8))
+    assert (wide[:, 0].float() == 0).all() and (wide[:, k + 1:].float() == 0).all()
+
+
 @pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_zeros_and_extremes(ops, block_rows):
     x = torch.zeros(5, 512, device="cuda")
