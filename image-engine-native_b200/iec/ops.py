@@ -13,12 +13,15 @@ outputs are allocated and arguments checked one by one.
 
 Tensors are torch tensors of the handle's device. Work is queued on
 torch's current stream unless `stream` (an integer cudaStream_t) is given,
-and the calls return without waiting. There is no CPU fallback.
+and the calls return without waiting. Outputs that a call allocates belong
+to the stream it is queued on, as under torch.cuda.stream; inputs of another
+stream are the caller's to order. There is no CPU fallback.
 """
 
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from struct import Struct
 
 import torch
@@ -104,13 +107,14 @@ def _maps(t, device: int, what: str):
     return n, pixels, c, step, stride[0] if n > 1 else c
 
 
-def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device: int):
-    if codes is None:
-        codes = empty_codes(rows, k, f"cuda:{device}")
+def _fp8_out(codes, scales, rows: int, k: int, scale_rows: int, device: int, stream):
+    with _queued_on(stream, device):
+        if codes is None:
+            codes = empty_codes(rows, k, f"cuda:{device}")
+        blocks = -(-k // BLOCK)
+        if scales is None:
+            scales = torch.empty((blocks, scale_rows), dtype=_F32, device=f"cuda:{device}")
     code_step = _rows(codes, (rows, k), _FP8, device, "codes")
-    blocks = -(-k // BLOCK)
-    if scales is None:
-        scales = torch.empty((blocks, scale_rows), dtype=_F32, device=f"cuda:{device}")
     return codes, code_step, scales, _rows(scales, (blocks, scale_rows), _F32, device, "scales")
 
 
@@ -119,6 +123,17 @@ def _stream(stream, device: int) -> int:
     if stream is None:
         stream = torch._C._cuda_getCurrentRawStream(device)
     return stream or _LEGACY_STREAM
+
+
+def _queued_on(stream, device: int):
+    """Makes `stream` torch's current one while outputs are allocated: memory
+    that was just freed on torch's current stream may still be in use there,
+    and what a call's kernels write must not be handed out again behind them."""
+    if stream is None:
+        return nullcontext()
+    if stream in (0, _LEGACY_STREAM):
+        return torch.cuda.stream(torch.cuda.default_stream(device))
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def empty_codes(rows: int, k: int, device):
@@ -178,7 +193,8 @@ class Ops:
         dtype = _dtype(x, "x")
         n, pixels, c, step, map_step = _maps(x, self._device, "x")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            with _queued_on(stream, self._device):
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         elif out.dtype is not x.dtype or out.shape != x.shape:
             _bad("out must have the shape and type of x")
         _, _, _, out_step, out_map_step = _maps(out, self._device, "out")
@@ -203,7 +219,8 @@ class Ops:
                 _check(status)
         dtype = _dtype(x, "x")
         n, pixels, c, step, map_step = _maps(x, self._device, "x")
-        codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, self._device)
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, self._device,
+                                                     stream)
         args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
                                _f32_vector(beta, c, self._device, "beta"), 0, 0, 0, codes.data_ptr(), code_step, scales.data_ptr(),
                                scale_step, eps, dtype, act)
@@ -229,7 +246,7 @@ class Ops:
         rows, k = shape
         step = _rows(x, shape, x.dtype, self._device, "x")
         scale_rows = rows if block_rows != BLOCK else -(-rows // BLOCK)
-        codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, self._device)
+        codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, self._device, stream)
         args = QUANTIZE.pack(x.data_ptr(), rows, k, step, block_rows, codes.data_ptr(), code_step, scales.data_ptr(),
                              scale_step, dtype)
         status = self._lib.iec_ops_quantize_fp8(self._h, args, _stream(stream, self._device))
@@ -256,7 +273,8 @@ class Ops:
         n, dev = w_shape[0], self._device
         blocks = -(-k // BLOCK)
         if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=a.device)
+            with _queued_on(stream, self._device):
+                out = torch.empty((m, n), dtype=dtype, device=a.device)
         code = _dtype(out, "out")
         res, res_step = 0, 0
         if residual is not None:
