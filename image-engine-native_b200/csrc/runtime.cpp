@@ -262,9 +262,67 @@ Device::~Device() {
   if (poisoned()) {
     dev_err_.leak();
     for (auto& e : scratch_) e.second.leak();
-    for (auto& e : lasting_) e.second.leak();
+    for (auto& e : lasting_) e.buffer.leak();
   }
   if (prev >= 0) cudaSetDevice(prev);
+}
+
+namespace {
+
+// Lets this thread allocate while one of its streams is being captured (the
+// allocation is no part of the graph).
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// A flag that is set when `graph` and the executables made from it are gone.
+std::shared_ptr<std::atomic<bool>> watch_graph(cudaGraph_t graph) {
+  using Flag = std::shared_ptr<std::atomic<bool>>;
+  auto gone = std::make_shared<std::atomic<bool>>(false);
+  auto held = std::make_unique<Flag>(gone);
+  cudaUserObject_t object;
+  IEC_CUDA(cudaUserObjectCreate(
+      &object, held.get(),
+      [](void* p) {
+        std::unique_ptr<Flag> flag(static_cast<Flag*>(p));
+        (*flag)->store(true);
+      },
+      1, cudaUserObjectNoDestructorSync));
+  held.release();
+  const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);
+    throw Error(ERR_GPU, std::string("cudaGraphRetainUserObject: ") + cudaGetErrorString(e));
+  }
+  return gone;
+}
+
+}  // namespace
+
+void* Device::lasting_scratch(size_t bytes, cudaStream_t stream) {
+  cudaStreamCaptureStatus status;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  IEC_CUDA(cudaStreamGetCaptureInfo(stream, &status, &capture, &graph));
+  if (status != cudaStreamCaptureStatusActive) capture = 0;
+  const LastingScratch* last = nullptr;
+  for (const auto& e : lasting_)
+    if (e.stream == stream && e.capture == capture) last = &e;  // the newest is the largest
+  if (last && last->buffer.size() >= bytes) return last->buffer.get();
+  const size_t least = last ? 2 * last->buffer.size() : capture ? 0 : (size_t)1 << 20;
+  RelaxedCapture relaxed;
+  lasting_.erase(std::remove_if(lasting_.begin(), lasting_.end(),
+                                [](const LastingScratch& e) { return e.graph_gone && *e.graph_gone; }),
+                 lasting_.end());
+  LastingScratch now;
+  now.stream = stream;
+  now.capture = capture;
+  now.buffer.reserve(std::max(bytes, least));
+  if (capture) now.graph_gone = watch_graph(graph);
+  lasting_.push_back(std::move(now));
+  return lasting_.back().buffer.get();
 }
 
 void Device::set_timing(bool on) {

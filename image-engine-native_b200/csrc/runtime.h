@@ -14,11 +14,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <functional>
 #include <initializer_list>
 #include <map>
+#include <memory>
 #include <stdexcept>
 #include <string>
 #include <utility>
@@ -175,18 +177,14 @@ class Device {
     scratch_gen_++;
     return scratch_.back().second.get();
   }
-  // Scratch whose earlier buffers stay until the device goes when it grows: a
-  // graph that a caller captured goes on using the one it saw.
-  void* lasting_scratch(size_t bytes, cudaStream_t stream) {
-    DeviceBuffer* last = nullptr;
-    for (auto& e : lasting_)
-      if (e.first == stream) last = &e.second;  // the newest of the stream's is the largest
-    if (last && last->size() >= bytes) return last->get();
-    DeviceBuffer b;
-    b.reserve(std::max(bytes, last ? 2 * last->size() : (size_t)1 << 20));
-    lasting_.emplace_back(stream, std::move(b));
-    return lasting_.back().second.get();
-  }
+  // Scratch of at least `bytes` for the launches queued on `stream`, in the
+  // stream's order. Buffers that a growing one leaves behind stay: launches on
+  // their way go on using them. While `stream` is being captured the buffer is
+  // the capture's own (per stream, since a capture's branches run at once): a
+  // graph replays on any stream, beside other graphs captured on this one and
+  // beside calls that are not captured. It is freed after the graph and its
+  // executables are gone, at the latest with the device.
+  void* lasting_scratch(size_t bytes, cudaStream_t stream);
   // Counts the scratch buffers' (re)allocations (a captured pass that used
   // an older one must not replay).
   uint64_t scratch_generation() const { return scratch_gen_; }
@@ -220,7 +218,13 @@ class Device {
   cudaStream_t copy_stream_ = nullptr;
   DeviceBuffer dev_err_;
   std::vector<std::pair<cudaStream_t, DeviceBuffer>> scratch_;
-  std::vector<std::pair<cudaStream_t, DeviceBuffer>> lasting_;
+  struct LastingScratch {
+    cudaStream_t stream = nullptr;
+    unsigned long long capture = 0;                 // 0: not of a capture
+    std::shared_ptr<std::atomic<bool>> graph_gone;  // set once nothing holds the captured graph
+    DeviceBuffer buffer;
+  };
+  std::vector<LastingScratch> lasting_;
   uint64_t scratch_gen_ = 0;
   PinnedBuffer host_err_;
   std::string poisoned_;

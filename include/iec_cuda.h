@@ -321,11 +321,11 @@ iec_status iec_birefnet_set_fused(iec_birefnet* model, int on);
  * on `stream` (a cudaStream_t; NULL: the handle's own stream, which does not
  * order itself with any other; cudaStreamLegacy names the legacy default
  * stream) and the calls return without waiting. They can be captured into a
- * CUDA graph after a call of the same size on the same stream (which sets
- * the kernels' attributes and the scratch that larger maps take). Sizes of zero are allowed
- * and queue nothing where they leave nothing to write. Strides count
- * elements; rows may be further apart than they are long (a channel slice
- * of a wider map), never overlap.
+ * CUDA graph, which may be replayed on any stream, beside other graphs and
+ * calls; the handle stays open as long as the graph is replayed. Sizes of
+ * zero are allowed and queue nothing where they leave nothing to write.
+ * Strides count elements; rows may be further apart than they are long (a
+ * channel slice of a wider map), never overlap.
  *
  * 8-bit rows. A matrix of `rows` x `k` values is kept as e4m3 codes, row by
  * row, and f32 scales of its blocks of 128 values along k, block by block:
