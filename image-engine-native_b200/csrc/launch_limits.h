@@ -34,21 +34,21 @@ class SmemLimit {
 };
 
 // How many CTAs of a kernel a device holds at once, per cluster size and 16 KB
-// of shared memory. Threads that ask at once may each look it up; they find the
-// same.
+// of shared memory; 0 where a cluster has no room. Threads that ask at once may
+// each look it up; they find the same.
 class Residency {
  public:
   static constexpr size_t STEP = 16 * 1024;
   template <class Find>
   int get(int device, int cluster, size_t smem, Find&& find) {
     std::atomic<int>& f = found_[device % MAX_DEVICES][cluster][std::min<size_t>(15, smem / STEP)];
-    int n = f.load(std::memory_order_relaxed);
-    if (n == 0) f.store(n = find(), std::memory_order_relaxed);
-    return n;
+    int noted = f.load(std::memory_order_relaxed);
+    if (noted == 0) f.store(noted = find() + 1, std::memory_order_relaxed);
+    return noted - 1;
   }
 
  private:
-  std::atomic<int> found_[MAX_DEVICES][17][16] = {};
+  std::atomic<int> found_[MAX_DEVICES][17][16] = {};  // CTAs + 1
 };
 
 }  // namespace iec

@@ -46,7 +46,8 @@ void launch_ops(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, i
 }
 
 // CTAs of `Kernel` that the device holds at once, in clusters of `cluster`,
-// with `smem` rounded up to 16 KB.
+// with `smem` rounded up to 16 KB; 0 where such a cluster has no room (large
+// ones may not: the callers go on to smaller ones).
 template <auto Kernel>
 int resident_ctas(Device& dev, int threads, size_t smem, int cluster) {
   static Residency found;
@@ -65,7 +66,6 @@ int resident_ctas(Device& dev, int threads, size_t smem, int cluster) {
       IEC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, rounded));
       n *= dev.sms();
     }
-    if (n < 1) throw Error(ERR_GPU, "no room for a cluster of CTAs");
     return n * cluster;
   });
 }

@@ -55,6 +55,9 @@ int main() {
   if (found.get(0, 2, 1000, find) != 10 || found.get(0, 2, 2000, find) != 10 || found.get(0, 16, 1000, find) != 20 ||
       found.get(0, 2, 17000, find) != 30 || found.get(1, 2, 1000, find) != 40 || looked != 4)
     bad++;
+  // no room is an answer too, and kept
+  for (int i = 0; i < 2; i++)
+    if (found.get(0, 8, 0, [&] { looked++; return 0; }) != 0 || looked != 5) bad++;
   std::printf("%d\n", bad.load());
   return bad != 0;
 }
