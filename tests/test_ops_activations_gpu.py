@@ -6,7 +6,10 @@ Tolerances, u the output type's unit roundoff: results of f32 are the
 formula's own f32 functions, each within two units: 2^-21 of the value. For
 16 bits u + 2^-18: the exponent v log2(e) is rounded once, by up to 2^-17 / 2
 at |v| = 87, 2^-18.5 of the exponential. Below -87.3 the sigmoid is less than
-2^-126 and may be 0: 2^-119 of a SiLU, since |v| < 128 where that matters."""
+2^-126 and may be 0: 2^-119 of a SiLU, since |v| < 128 where that matters.
+GELU: a Phi(-a), a = |v|, has its exponent a^2 log2(e) / 2 rounded twice, which
+moves it by a^2 2^-24 of itself, next to 2^-20 for what else is rounded; for 16
+bits its own form is good to 2^-14."""
 
 import pytest
 
@@ -82,7 +85,46 @@ def test_sigmoid_and_silu_of_the_largest(ops, dtype):
     assert torch.isnan(silu[10]) and silu[11] == 0
 
 
-@pytest.mark.parametrize("act", [SIGMOID, SILU])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_gelu_over_its_range(ops, dtype, rows):
+    v = arguments()
+    got = of_bias(ops, v, GELU, dtype, rows)
+    want = act64(v.double(), GELU)
+    relative = 2.0 ** (-20 if dtype == "f32" else -14) + torch.clamp_max(v.double().abs(), 14) ** 2 * 2.0 ** -23
+    for y in (got[0], got[-1]):
+        close(y, want, dtype, relative, 2.0 ** -119)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gelu_of_the_largest(ops, dtype):
+    v = torch.tensor([-1e2, -1e4, -1e20, -3e38, 1e2, 1e4, 1e20, 3e38, INF, NAN, 0.0], device="cuda")
+    got = of_bias(ops, v, GELU, dtype)[0].float()
+    assert (got[:4] == 0).all() and torch.equal(got[4:9], v[4:9].to(TYPES[dtype]).float())
+    assert torch.isnan(got[9]) and got[10] == 0
+    least = of_bias(ops, torch.full((8,), -INF, device="cuda"), GELU, dtype)
+    assert (torch.isnan(least) | (least == 0)).all()  # -inf 0, or its limit
+
+
+@pytest.mark.parametrize("act,lo,hi", [(GELU, -6.0, 2.0), (GELU, -5.5, -4.5), (SILU, -12.0, -6.0), (SIGMOID, -70.0, -60.0)])
+@pytest.mark.parametrize("pixels", [33, 9000])
+def test_eight_bit_rows_of_tails(ops, act, lo, hi, pixels):
+    """Whole blocks in an activation's tail keep the codes' precision: the
+    value is within 2^-15 of itself before it is quantised, so codes and scales
+    are off by no more than that beside their own rounding."""
+    c = 256
+    beta = torch.linspace(lo, hi, c, device="cuda")
+    x = torch.zeros(1, pixels, c, device="cuda", dtype=torch.float16)
+    codes, scales = ops.group_norm_fp8(x, 2, torch.zeros(c, device="cuda"), beta, act=act)
+    want = act64(beta.double(), act).reshape(2, 128)
+    top = want.abs().amax(1)
+    assert ((scales.double() * 448 / top[:, None] - 1).abs() <= 2.0 ** -14).all()
+    back = codes.double().reshape(pixels, 2, 128) * scales.double().t()[:, :, None]
+    step = torch.clamp_min(want.abs() / 16, top[:, None] / 448 * 2.0 ** -10)  # half a step of the codes
+    assert ((back - want).abs() <= step + 2.0 ** -14 * want.abs()).all()
+
+
+@pytest.mark.parametrize("act", [GELU, SIGMOID, SILU])
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 def test_a_nan_or_infinity_leaves_its_neighbours_alone(ops, act, dtype):
     """Values that share a reciprocal."""
