@@ -408,7 +408,9 @@ iec_status iec_ops_quantize_fp8(iec_ops* ops, const iec_quantize_fp8_args* args,
  * (m x k, block_rows 1) and `w` (n x k, block_rows 128): a linear layer, or
  * a 1x1 convolution over channels-last pixels. The products of a block of
  * 128 along k are summed, scaled by both its scales and added up in f32;
- * the result is rounded once. `bias` (n floats) and `residual` (m x n of
+ * the result is rounded once. The two scales are multiplied first: a product
+ * of finite scales beyond f32's largest value counts as that value, one below
+ * 2^-126 has f32's steps of 2^-149. `bias` (n floats) and `residual` (m x n of
  * `dtype`, may be `out` itself with its stride) may be NULL. `a` and `w`
  * must start on 16 bytes, with strides a multiple of 16. */
 typedef struct iec_matmul_fp8_args {
