@@ -317,8 +317,8 @@ struct Affine {
   }
 };
 
-// 1 / sqrt(v), within two units.
-__device__ __forceinline__ float norm_rstd(float v) { return rsqrtf(v); }
+// 1 / sqrt(v), rounded once: rsqrtf's two units would be a whole group's.
+__device__ __forceinline__ float norm_rstd(float v) { return __frsqrt_rn(v); }
 
 // ---------------------------------------------------------------- resident
 // A CTA writes a segment of seg_c channels and reads its window: the segment
@@ -333,6 +333,7 @@ struct NormResident {
   int around;       // then, behind all pixels' slots, threads of a pixel for the window's other vectors
   int pixels;       // of a CTA
   int groups;       // room for a window's
+  float inv;        // 1 / the values of a group
   FastDiv by_slots, by_around, by_rows, by_cg;
   NormJoin join;
 };
@@ -440,7 +441,6 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
     join_threads(q.join, last, tmean, tdev, entries, px, c0 >> q.join.shift,
                  [&](int g, float m, float d) { own[g - g0] = make_float2(m, d); });
   cluster_sync();
-  const float inv = op_rcp((float)p.pixels * (float)cg);
 #pragma unroll 1
   for (int g = warp; g < groups; g += NORM_THREADS / 32) {
     float2 v = make_float2(0.0f, 0.0f);
@@ -451,9 +451,9 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       v = ld_cluster_f32x2(own + g, (uint32_t)lane);
     }
     const float m0 = __shfl_sync(~0u, v.x, 0);  // the first CTA always has pixels
-    const float m = m0 + warp_sum(k * (v.x - m0)) * inv, d = v.x - m;
+    const float m = m0 + warp_sum(k * (v.x - m0)) * q.inv, d = v.x - m;
     const float dev = warp_sum(fmaf(k * d, d, v.y));
-    if (lane == 0) stat[g] = make_float2(m, norm_rstd(dev * inv + p.eps));
+    if (lane == 0) stat[g] = make_float2(m, norm_rstd(dev * q.inv + p.eps));
   }
   __syncthreads();
   affine.set(stat, mine ? c0 + vec * VE : c0, g0, cg, q.by_cg);
@@ -495,6 +495,7 @@ struct NormChunks {
   int tiles, tile_c, chunks, slots, cluster;
   long long span;  // pixels of a CTA of norm_stats
   int map0;        // the first map of this launch
+  float inv;       // 1 / the values of a group
   FastDiv by_cg;   // by the channels of a group
   NormJoin join;
   float2* part;
@@ -600,7 +601,6 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
     *n = (float)max(0ll, min(chunk, p.pixels - k * chunk)) * (float)w;
     return q.part[((z * (long long)q.tiles + tile) * q.slots + g - c0 / cg) * q.chunks + k];
   };
-  const float count = (float)p.pixels * (float)cg;
   const int all = q.chunks * span;
   float m = 0.0f, d = 0.0f, n;
   const float m0 = pair(0, &n).x;
@@ -608,12 +608,12 @@ __device__ __forceinline__ float2 norm_join(const NormSpec& p, const NormChunks&
     const float2 v = pair(i, &n);
     m = fmaf(n, v.x - m0, m);
   }
-  m = m0 + warp_sum(m) / count;
+  m = m0 + warp_sum(m) * q.inv;
   for (int i = lane; i < all; i += 32) {
     const float2 v = pair(i, &n);
     d += fmaf(n * (v.x - m), v.x - m, v.y);
   }
-  return make_float2(m, norm_rstd(warp_sum(d) / count + p.eps));
+  return make_float2(m, norm_rstd(warp_sum(d) * q.inv + p.eps));
 }
 
 // The same for the groups g0 .. g1 of a tile into stat[], by a CTA of `warps`
@@ -660,7 +660,7 @@ __device__ __forceinline__ void norm_join_all(const NormSpec& p, const NormChunk
 #pragma unroll
     for (int k = 0; k < 4; k++)
       if (lane == k && g + k * warps <= g1)
-        stat[g + k * warps - g0] = make_float2(m[k], norm_rstd(d[k] * (inv * op_rcp(cg)) + p.eps));
+        stat[g + k * warps - g0] = make_float2(m[k], norm_rstd(d[k] * q.inv + p.eps));
   }
 }
 
@@ -725,7 +725,8 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
       if (scales && lane < some) *scale_at = mine;
     };
     // The last pixels, then whole steps, the next one's loads ahead of this
-    // one's work.
+    // one's work. (Each load has its condition: with one around them all, 2 x
+    // 768 x 512 x 128 bf16 with SiLU took 125 us instead of 115.)
     typename V::Raw raw[U], rest[U];
     const int some = px - full * per - r * U;
 #pragma unroll
@@ -740,9 +741,8 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
     for (int f = full; f > 0; f--) {
       typename V::Raw next[U];
       x -= x_step;
-      if (f > 1)
 #pragma unroll
-        for (int u = 0; u < U; u++) next[u] = V::fetch(x + u * p.x_stride);
+      for (int u = 0; u < U; u++) next[u] = f > 1 ? V::fetch(x + u * p.x_stride) : V::zero();
       out -= FP8 ? 0 : out_step;
       codes -= code_step;
       scale_at -= FP8 ? per : 0;

@@ -80,6 +80,7 @@ ResidentPlan plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, boo
   q.by_around = FastDiv((uint32_t)std::max(1, q.around));
   q.by_rows = FastDiv((uint32_t)q.rows);
   q.by_cg = FastDiv((uint32_t)cg);
+  q.inv = (float)(1.0 / ((double)p.pixels * cg));
   q.join = join_shape<VE>(cg, q.vecs[0] * VE, q.vecs[1] * VE, q.rows);
   // As many CTAs as fill the GPU, but at least two steps each; a cluster size
   // that the GPU's parts divide badly is made smaller. Only where all clusters
@@ -158,6 +159,7 @@ void run_chunks(Device& dev, const NormSpec& p, cudaStream_t s) {
   const int c_last = p.c - (q.tiles - 1) * q.tile_c;
   q.join = join_shape<VE>(cg, q.tile_c, c_last, NORM_THREADS / (q.tile_c / VE));
   q.by_cg = FastDiv((uint32_t)cg);
+  q.inv = (float)(1.0 / ((double)p.pixels * cg));
   // the ring, or the threads' statistics, their entries and pairs
   const size_t stats_smem = std::max(
       ring, (size_t)NORM_THREADS * VE * 8 + (size_t)norm_entries(q.join.runs[0]) * 12 + (size_t)(q.slots + 1) * 8);
