@@ -31,7 +31,7 @@ from . import ERR_INPUT, IecError, Options, _check, lib
 try:
     from . import _ops_binding as _fast
 except ImportError as e:
-    raise ImportError("iec/_ops_binding.so is missing: build it with __graft_entry__.build()") from e
+    raise ImportError("iec/_ops_binding.so is missing: build it with `make binding` or __graft_entry__.build()") from e
 
 NONE, RELU, GELU, SIGMOID, SILU = range(5)
 BLOCK = 128  # values along a row that share a scale
