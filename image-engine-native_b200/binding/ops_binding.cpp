@@ -7,6 +7,7 @@
 // something is not as the fast path takes it (an output to be allocated, a
 // type, shape, stride or device that does not fit): iec/ops.py then goes
 // through its checks one by one and says what is wrong.
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -46,7 +47,8 @@ struct Call {
   const at::Tensor* tensor(PyObject* o) {
     if (THPVariable_Check(o)) {
       const at::Tensor& t = THPVariable_Unpack(o);
-      if (t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device) return &t;
+      const bool lost = t.requires_grad() && c10::GradMode::is_enabled();  // its gradient
+      if (t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !lost) return &t;
     }
     ok = false;
     return nullptr;

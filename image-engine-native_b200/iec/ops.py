@@ -16,6 +16,9 @@ torch's current stream unless `stream` (an integer cudaStream_t) is given,
 and the calls return without waiting. Outputs that a call allocates belong
 to the stream it is queued on, as under torch.cuda.stream; inputs of another
 stream are the caller's to order. There is no CPU fallback.
+
+The operators have no gradients: where torch records them (outside
+torch.no_grad()), a tensor that requires one is refused.
 """
 
 from __future__ import annotations
@@ -57,16 +60,19 @@ def _dtype(t, what: str) -> int:
     return code
 
 
-def _elsewhere(t, device: int, what: str):
-    _bad(f"{what} is on {t.device}, the handle on cuda:{device}")
+def _known(t, device: int, what: str):
+    """Refuses a tensor of another device, or one whose gradient would be lost."""
+    if t.get_device() != device:
+        _bad(f"{what} is on {t.device}, the handle on cuda:{device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(f"{what} requires a gradient, which the operators do not have: detach it or call under torch.no_grad()")
 
 
 def _f32_vector(t, n: int, device: int, what: str) -> int:
     """The address of n contiguous floats, 0 for None."""
     if t is None:
         return 0
-    if t.get_device() != device:
-        _elsewhere(t, device, what)
+    _known(t, device, what)
     if t.dtype is not _F32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         _bad(f"{what} must be {n} contiguous float32 values")
     return t.data_ptr()
@@ -74,8 +80,7 @@ def _f32_vector(t, n: int, device: int, what: str) -> int:
 
 def _rows(t, shape, dtype, device: int, what: str) -> int:
     """The row stride of a matrix of `shape` whose rows are contiguous."""
-    if t.get_device() != device:
-        _elsewhere(t, device, what)
+    _known(t, device, what)
     if t.dtype is dtype and t.shape == shape:
         step, one = t.stride()
         if one == 1 or shape[1] <= 1:
@@ -86,8 +91,7 @@ def _rows(t, shape, dtype, device: int, what: str) -> int:
 
 def _maps(t, device: int, what: str):
     """(maps, pixels, channels, pixel stride, map stride) of n x ... x c."""
-    if t.get_device() != device:
-        _elsewhere(t, device, what)
+    _known(t, device, what)
     shape, stride = t.shape, t.stride()
     if len(shape) < 2:
         _bad(f"{what} must be maps x pixels (or height x width) x channels")
