@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 from contextlib import nullcontext
 from struct import Struct
+from struct import error as StructError
 
 import torch
 
@@ -51,6 +52,14 @@ _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream has the handle 0
 
 def _bad(message: str):
     raise IecError(ERR_INPUT, message)
+
+
+def _pack(layout, *values) -> bytes:
+    """An argument struct."""
+    try:
+        return layout.pack(*values)
+    except (StructError, OverflowError) as e:
+        raise IecError(ERR_INPUT, f"an argument is no number of its type's range: {e}") from e
 
 
 def _dtype(t, what: str) -> int:
@@ -202,7 +211,7 @@ class Ops:
         elif out.dtype is not x.dtype or out.shape != x.shape:
             _bad("out must have the shape and type of x")
         _, _, _, out_step, out_map_step = _maps(out, self._device, "out")
-        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
+        args = _pack(GROUP_NORM, x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
                                _f32_vector(beta, c, self._device, "beta"), out.data_ptr(), out_step, out_map_step, 0, 0, 0, 0, eps,
                                dtype, act)
         status = self._lib.iec_ops_group_norm(self._h, args, _stream(stream, self._device))
@@ -225,7 +234,7 @@ class Ops:
         n, pixels, c, step, map_step = _maps(x, self._device, "x")
         codes, code_step, scales, scale_step = _fp8_out(codes, scales, n * pixels, c, n * pixels, self._device,
                                                      stream)
-        args = GROUP_NORM.pack(x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
+        args = _pack(GROUP_NORM, x.data_ptr(), n, pixels, c, step, map_step, groups, _f32_vector(gamma, c, self._device, "gamma"),
                                _f32_vector(beta, c, self._device, "beta"), 0, 0, 0, codes.data_ptr(), code_step, scales.data_ptr(),
                                scale_step, eps, dtype, act)
         status = self._lib.iec_ops_group_norm_fp8(self._h, args, _stream(stream, self._device))
@@ -251,7 +260,7 @@ class Ops:
         step = _rows(x, shape, x.dtype, self._device, "x")
         scale_rows = rows if block_rows != BLOCK else -(-rows // BLOCK)
         codes, code_step, scales, scale_step = _fp8_out(codes, scales, rows, k, scale_rows, self._device, stream)
-        args = QUANTIZE.pack(x.data_ptr(), rows, k, step, block_rows, codes.data_ptr(), code_step, scales.data_ptr(),
+        args = _pack(QUANTIZE, x.data_ptr(), rows, k, step, block_rows, codes.data_ptr(), code_step, scales.data_ptr(),
                              scale_step, dtype)
         status = self._lib.iec_ops_quantize_fp8(self._h, args, _stream(stream, self._device))
         if status:
@@ -283,7 +292,7 @@ class Ops:
         res, res_step = 0, 0
         if residual is not None:
             res, res_step = residual.data_ptr(), _rows(residual, (m, n), out.dtype, dev, "residual")
-        args = MATMUL.pack(a.data_ptr(), _rows(a, a_shape, _FP8, dev, "a"),
+        args = _pack(MATMUL, a.data_ptr(), _rows(a, a_shape, _FP8, dev, "a"),
                            a_scales.data_ptr(), _rows(a_scales, (blocks, m), _F32, dev, "a_scales"),
                            w.data_ptr(), _rows(w, (n, k), _FP8, dev, "w"),
                            w_scales.data_ptr(), _rows(w_scales, (blocks, -(-n // BLOCK)), _F32, dev, "w_scales"),
