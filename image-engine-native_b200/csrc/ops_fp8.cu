@@ -62,8 +62,8 @@ void run_tiles(Device& dev, const Fp8MatmulSpec& q, Fp8Params p, cudaStream_t s)
   }
   p.tiles_m = (q.m + edge - 1) / edge;
   p.tiles_n = (q.n + edge - 1) / edge;
-  if ((long long)p.tiles_m * p.tiles_n >= 1 << 24 || FP8_GROUP * p.tiles_n >= 1 << 16)
-    throw Error(ERR_INPUT, "product too large for one launch");
+  // (2^20 columns are at most 2^13 tiles, a group of them 2^16: within what FastDiv divides by)
+  if ((long long)p.tiles_m * p.tiles_n >= 1 << 24) throw Error(ERR_INPUT, "product too large for one launch");
   p.tiles = p.tiles_m * p.tiles_n;
   p.div_group = FastDiv((uint32_t)(FP8_GROUP * p.tiles_n));
   p.div_rest = FastDiv((uint32_t)std::max(1, p.tiles_m % FP8_GROUP));

@@ -1,5 +1,5 @@
 """The 8-bit product where tests/test_ops_gpu.py does not reach (GPU tests):
-scales at the ends of f32's range."""
+scales at the ends of f32's range, as many columns as it takes."""
 
 import pytest
 
@@ -105,3 +105,23 @@ def test_zero_weights_beside_the_largest_values(ops):
     weights[7] = 0
     got = ops.matmul_fp8(*ops.quantize_fp8(x), *ops.quantize_fp8(weights, 128), dtype=torch.float32)
     assert (got[:, 7] == 0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 1 << 20, 32), (130, (1 << 20) - 127, 16), (1, (1 << 20) - 128, 144)])
+def test_as_many_columns_as_it_takes(ops, m, n, k):
+    g = gen(m)
+    (a, sa), (w, sw) = ops.quantize_fp8(randn(g, m, k)), ops.quantize_fp8(randn(g, n, k), 128)
+    got = ops.matmul_fp8(a, sa, w, sw).double()
+    want, size = product64(a, sa, w, sw)
+    assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -16 * size).all()
+
+
+def test_one_column_more_is_refused(ops):
+    import iec
+    from iec.ops import empty_codes
+
+    n = (1 << 20) + 1
+    with pytest.raises(iec.IecError) as e:
+        ops.matmul_fp8(empty_codes(1, 16, "cuda"), torch.ones((1, 1), device="cuda"), empty_codes(n, 16, "cuda"),
+                       torch.ones((1, -(-n // 128)), device="cuda"))
+    assert e.value.code == iec.ERR_INPUT and "columns" in str(e.value)
