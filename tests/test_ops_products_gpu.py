@@ -125,3 +125,88 @@ def test_one_column_more_is_refused(ops):
         ops.matmul_fp8(empty_codes(1, 16, "cuda"), torch.ones((1, 1), device="cuda"), empty_codes(n, 16, "cuda"),
                        torch.ones((1, -(-n // 128)), device="cuda"))
     assert e.value.code == iec.ERR_INPUT and "columns" in str(e.value)
+
+
+def kernels_of(ops, call):
+    """What `call` returns and the kernels it launches, from the launch record."""
+    import iec
+
+    iec.set_launch_timing(ops, True)
+    try:
+        out = call()
+        return out, [r["name"] for r in iec.launch_timing(ops)]
+    finally:
+        iec.set_launch_timing(ops, False)
+
+
+NONE, RELU, GELU, SIGMOID, SILU = range(5)
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+HALF = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+SMALL = {"f16": 2.0 ** -25, "bf16": 0.0, "f32": 0.0}  # half a subnormal step
+SINGLE, PAIR, SPLIT = "fp8_gemm_sm100<0>", "fp8_gemm_sm100<1>", "fp8_gemm_sm100<2>"
+# m, n, k: rows of every type start on 16 bytes; tiles, and blocks along k, are cut short
+TILES = [(2300, 2040, 1100, PAIR), (2304, 2048, 128, PAIR), (9400, 2040, 300, PAIR), (4090, 1528, 300, SINGLE), (100, 200, 2000, SPLIT)]
+
+
+def act64(v, act):
+    if act == RELU:
+        return torch.relu(v)
+    if act == GELU:
+        return 0.5 * v * torch.special.erfc(-v * 0.5 ** 0.5)
+    if act == SIGMOID:
+        return torch.sigmoid(v)
+    return v * torch.sigmoid(v) if act == SILU else v
+
+
+def operands(ops, m, n, k):
+    """Codes and scales whose products are about 1."""
+    g = gen(m + n + k)
+    (a, sa), (w, sw) = ops.quantize_fp8(randn(g, m, k) * k ** -0.5), ops.quantize_fp8(randn(g, n, k), 128)
+    return a, sa, w, sw, randn(g, n)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,n,k,kernel", TILES)
+def test_every_tile_shape_with_its_whole_epilogue(ops, m, n, k, kernel, dtype):
+    """Each kernel against the 64-bit product, through TMA: bias, activation
+    (slope at most 1.13, good to 2^-14 for 16 bits) and residual, the residual
+    in a tensor of its own, in the output, and in a wider output whose other
+    columns stay as they are."""
+    a, sa, w, sw, bias = operands(ops, m, n, k)
+    res = randn(gen(7), m, n).to(TYPES[dtype])
+    raw, size = product64(a, sa, w, sw)
+    raw = raw + bias.double()
+    slack = 1.13 * 2.0 ** -16 * (size + bias.double().abs())
+
+    def good(got, want, act):
+        curve = 0.0 if act in (NONE, RELU) else 2.0 ** (-19 if dtype == "f32" else -14) * act64(raw, act).abs()
+        off = (got.double() - want).abs() - HALF[dtype] * want.abs() - SMALL[dtype] - slack - curve
+        assert (off <= 0).all(), off.max().item()
+
+    got, names = kernels_of(ops, lambda: ops.matmul_fp8(a, sa, w, sw, bias, dtype=TYPES[dtype]))
+    assert names == [f"{kernel} {m}x{n}x{k}"]
+    good(got, raw, NONE)
+    for act in (NONE, RELU, GELU, SIGMOID, SILU):
+        want = act64(raw, act) + res.double()
+        got, names = kernels_of(ops, lambda: ops.matmul_fp8(a, sa, w, sw, bias, act, res, dtype=TYPES[dtype]))
+        assert names == [f"{kernel} {m}x{n}x{k}"]
+        good(got, want, act)
+        out = res.clone()
+        ops.matmul_fp8(a, sa, w, sw, bias, act, out, out=out)
+        assert torch.equal(out, got)
+        wide = torch.full((m + 1, n + 16), 7.0, device="cuda", dtype=TYPES[dtype])
+        wide[:m, :n] = res
+        ops.matmul_fp8(a, sa, w, sw, bias, act, wide[:m, :n], out=wide[:m, :n])
+        assert torch.equal(wide[:m, :n], got) and (wide[:m, n:] == 7).all() and (wide[m] == 7).all()
+        odd = torch.full((m, n + 5), 7.0, device="cuda", dtype=TYPES[dtype])  # rows that start anywhere: no TMA
+        ops.matmul_fp8(a, sa, w, sw, bias, act, res, out=odd[:, 2:n + 2])
+        assert torch.equal(odd[:, 2:n + 2], got) and (odd[:, :2] == 7).all() and (odd[:, n + 2:] == 7).all()
+
+
+@pytest.mark.parametrize("m,n,k,kernel", TILES)
+def test_every_tile_shape_sums_in_32_bits(ops, m, n, k, kernel):
+    a, sa, w, sw, _ = operands(ops, m, n, k)
+    want, _ = product64(a, sa, w, sw)
+    got, names = kernels_of(ops, lambda: ops.matmul_fp8(a, sa, w, sw, dtype=torch.float32))
+    assert names == [f"{kernel} {m}x{n}x{k}"]
+    assert ((got.double() - want).norm() / want.norm()).item() <= 2.0 ** -20
