@@ -208,10 +208,10 @@ DeviceScope::DeviceScope(Device& d) {
     cudaGetLastError();
     prev_ = -1;
   }
-  if (prev_ == d.ordinal() && !d.poisoned())
-    prev_ = -1;  // current already: nothing to change, nothing to restore
-  else
-    d.enter();
+  // Also where the device is the thread's already: its current context may be
+  // another one of the same device (40 ns).
+  d.enter();
+  if (prev_ == d.ordinal()) prev_ = -1;  // nothing to restore
   prev_device_ = g_scope_device;
   g_scope_device = &d;
 }
