@@ -311,7 +311,7 @@ void* Device::lasting_scratch(size_t bytes, cudaStream_t stream) {
   for (const auto& e : lasting_)
     if (e.stream == stream && e.capture == capture) last = &e;  // the newest is the largest
   if (last && last->buffer.size() >= bytes) return last->buffer.get();
-  const size_t least = last ? 2 * last->buffer.size() : capture ? 0 : (size_t)1 << 20;
+  const size_t least = last ? 2 * last->buffer.size() : 0;  // (as much as is needed on a new stream: there may be many)
   RelaxedCapture relaxed;
   lasting_.erase(std::remove_if(lasting_.begin(), lasting_.end(),
                                 [](const LastingScratch& e) { return e.graph_gone && *e.graph_gone; }),

@@ -1,5 +1,5 @@
-"""Captured operators (GPU tests): a graph owns the scratch of the calls that
-it captured. The maps here take the two kernels of the group normalisation
+"""The operators' scratch (GPU tests): a graph owns that of the calls that it
+captured, a stream keeps what its calls need. The maps here take the two kernels of the group normalisation
 that pass pairs through scratch."""
 
 from contextlib import closing
@@ -118,6 +118,29 @@ def test_scratch_goes_with_its_graph(ops):
         used.append(torch.cuda.mem_get_info()[0])
     assert torch.equal(out, want)
     assert used[3] - used[-1] < 32 << 20, [u >> 20 for u in used]
+
+
+def test_a_stream_keeps_no_more_than_its_calls_need(ops):
+    """300 streams, each with a map whose pairs take less than 128 KB."""
+    x = maps(8, 1, 5000, 130)[0]  # channels that are no whole vectors: the two kernels
+    out = torch.empty_like(x)
+    ops.group_norm(x, 5, out=out)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.ExternalStream(s) for s in _streams(300)]
+    before = torch.cuda.mem_get_info()[0]
+    for s in streams:
+        with torch.cuda.stream(s):
+            ops.group_norm(x, 5, out=out)
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] < 100 << 20
+
+
+def _streams(count):
+    """More streams than torch's pool has: made by the CUDA runtime."""
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    made = [runtime.cudaStreamCreateWithFlags(1) for _ in range(count)]
+    assert all(err == runtime.cudaError_t.cudaSuccess for err, _ in made)
+    return [int(s) for _, s in made]
 
 
 def test_a_graph_outlives_larger_and_smaller_captures(ops):
