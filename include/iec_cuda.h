@@ -337,7 +337,9 @@ typedef struct iec_ops iec_ops;
 /* Types of the values at a device pointer. */
 typedef enum iec_dtype { IEC_F16 = 0, IEC_BF16 = 1, IEC_F32 = 2 } iec_dtype;
 
-/* Activations: v, max(v, 0), v Phi(v), 1 / (1 + e^-v), v / (1 + e^-v). */
+/* Activations: v, max(v, 0), v Phi(v), 1 / (1 + e^-v), v / (1 + e^-v). In f32
+ * before the result is rounded; sigmoids below 2^-126 and Phi(v) below v =
+ * -13.2 may be 0, and for 16-bit results Phi's tail is good to 2^-14 of itself. */
 typedef enum iec_act {
   IEC_ACT_NONE = 0,
   IEC_ACT_RELU = 1,
