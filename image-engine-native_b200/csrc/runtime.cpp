@@ -204,14 +204,13 @@ thread_local Device* g_scope_device = nullptr;
 Device* scoped_device() { return g_scope_device; }
 
 DeviceScope::DeviceScope(Device& d) {
-  if (cudaGetDevice(&prev_) != cudaSuccess) {
-    cudaGetLastError();
-    prev_ = -1;
+  if (!d.current()) {
+    if (cudaGetDevice(&prev_) != cudaSuccess) {
+      cudaGetLastError();
+      prev_ = -1;
+    }
+    d.enter();
   }
-  // Also where the device is the thread's already: its current context may be
-  // another one of the same device (40 ns).
-  d.enter();
-  if (prev_ == d.ordinal()) prev_ = -1;  // nothing to restore
   prev_device_ = g_scope_device;
   g_scope_device = &d;
 }
@@ -245,6 +244,12 @@ Device::Device(const Options& opt) {
   host_err_.reserve(256);
   IEC_CUDA(cudaMemset(dev_err_.get(), 0, 256));
   IEC_CUDA(cudaDeviceSynchronize());
+  void* entry = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  IEC_CUDA(cudaGetDriverEntryPoint("cuCtxGetCurrent", &entry, cudaEnableDefault, &found));
+  if (found != cudaDriverEntryPointSuccess) throw Error(ERR_GPU, "the driver has no cuCtxGetCurrent");
+  get_context_ = reinterpret_cast<GetContext>(entry);
+  if (get_context_(&context_) != CUDA_SUCCESS) throw Error(ERR_GPU, "no current context");
   if (prev >= 0) cudaSetDevice(prev);
 }
 
@@ -359,6 +364,11 @@ float Device::timed_ms(size_t i) {
   float ms = 0.0f;
   IEC_CUDA(cudaEventElapsedTime(&ms, timed_[i].a, timed_[i].b));
   return ms;
+}
+
+bool Device::current() const {
+  CUcontext now = nullptr;
+  return !poisoned() && get_context_(&now) == CUDA_SUCCESS && now == context_;
 }
 
 void Device::enter() {

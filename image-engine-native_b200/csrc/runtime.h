@@ -148,6 +148,10 @@ class Device {
   int timeout_ms() const { return timeout_ms_; }
   int batch_chunk() const { return batch_chunk_; }
 
+  // Whether the device's primary context is the calling thread's current one
+  // (its current device may be this one with another context), and the device
+  // is not poisoned.
+  bool current() const;
   // Make this device current on the calling thread; throws if poisoned.
   void enter();
   // Wait for `stream` to drain, polling at most timeout_ms; a timeout or a
@@ -216,6 +220,9 @@ class Device {
   int batch_chunk_ = 0;
   cudaStream_t stream_ = nullptr;
   cudaStream_t copy_stream_ = nullptr;
+  using GetContext = CUresult (*)(CUcontext*);
+  GetContext get_context_ = nullptr;
+  CUcontext context_ = nullptr;  // the device's primary one
   DeviceBuffer dev_err_;
   std::vector<std::pair<cudaStream_t, DeviceBuffer>> scratch_;
   struct LastingScratch {
