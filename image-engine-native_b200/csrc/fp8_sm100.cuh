@@ -24,8 +24,8 @@
 // run; where the rows of out or residual do not start on 16 bytes, they are
 // written through shared memory with plain accesses. All waits are bounded.
 //
-// What it measured: 16384 x 8192 x 2048 to bf16 274 us in a burst (2,000
-// TFLOP/s), 316 sustained under the power cap; 8192^3 484 and 557 us. The
+// What it measured: 16384 x 8192 x 2048 to bf16 280 us in a burst (1,965
+// TFLOP/s), 320 sustained under the power cap; 8192^3 485 and 561 us. The
 // bound is the accumulators' way back: per SM and block 128 x 256 values read
 // from TMEM and added, next to 512 cycles of MMAs (with the loads and MMAs
 // alone, and the output: 226 us). 256 x 256 is the largest tile whose sums (128

@@ -12,20 +12,25 @@
 // crosses HBM once each way, in one launch; the CTAs of a cluster split the
 // pixels and join their statistics over distributed shared memory.
 //
-// 4 x 64 x 64 x 512 f16 with SiLU (34 MB): 11 us, of which the loads take 2.6,
+// 4 x 64 x 64 x 512 f16 with SiLU (34 MB): 12 us, of which the loads take 2.6,
 // the statistics 2 and results and stores 4.5, one after another; a single
 // small map, 16 x 16 x 512: 4.8 us. To e4m3, where groups end inside blocks
 // of 128 channels, segments of whole groups and blocks are long and few; CTAs
 // then write single blocks and read the groups around them twice (32 x 32 x
-// 768, groups of 24: 6.4 us in 6 x 16 CTAs, 9.7 in 2 x 16; 32 x 32 x 640,
-// groups of 20: 6.7 against 13.6).
+// 768, groups of 24: 6.2 us in 6 x 16 CTAs, 9.7 in 2 x 16; 32 x 32 x 640,
+// groups of 20: 6.6 against 13.6).
 //
 // norm_stats + norm_apply: larger maps. The first kernel reduces chunks of
 // pixels, a cluster of CTAs each, to (mean, sum of squared deviations) per
 // group; the second joins the chunks' pairs and applies them, walking the
 // pixels backwards, since the last ones are the likeliest to be in L2 still.
 // 2 x 768 x 512 x 128 bf16 (201 MB, twice the size of a map that L2 holds):
-// 113 us, 45 and 68 of it; 8 x 128 x 128 x 256 f16 to e4m3: 46 us.
+// 114 us, 45 and 69 of it. 8 x 128 x 128 x 256 f16 to e4m3: 47 us, of which
+// norm_apply takes 25 without an activation (as to f16), 31 with SiLU and 43 with
+// GELU: with 16 warps an SM (128 registers) it issues in half of its cycles, its
+// warps waiting for instructions, for one another and for exponentials, whose
+// unit SiLU keeps busy for 39 % of the time. Channels that are no whole vectors
+// are read one by one: 3 x 137 x 153 x 321 f16 to e4m3 77 us (61 MB).
 //
 // Statistics: each thread takes a few pixels at a time from registers, their
 // mean and the squared deviations around it, and joins that to what it has

@@ -85,7 +85,7 @@ ResidentPlan plan_segment(Device& dev, const NormSpec& p, bool fp8, int seg, boo
   // As many CTAs as fill the GPU, but at least two steps each; a cluster size
   // that the GPU's parts divide badly is made smaller. Only where all clusters
   // run at once: one after another, their loads, statistics and stores take
-  // turns (8 x 128 x 128 x 256 f16: 90 us in four waves of clusters of 16, 46
+  // turns (8 x 128 x 128 x 256 f16: 90 us in four waves of clusters of 16, 47
   // in chunks through L2).
   const long long spread = dev.sms() / std::max<long long>(1, (long long)segs * p.n);
   const long long fill = (p.pixels + 2LL * q.rows - 1) / (2LL * q.rows);
