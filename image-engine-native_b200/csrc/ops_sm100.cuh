@@ -74,7 +74,7 @@ __device__ __forceinline__ float2 fmul2_ftz(float2 a, float2 b) {
 // rounded once), and 0 below -87.3, where they are less than 2^-126; of a NaN
 // they are 0 too. Quantised, no more e4m3 codes come out beside
 // the nearest one than with exact exponentials and quotients in f32 (SiLU of 4 x
-// 128 x 128 x 256 values: 22 and 34 of 16.8 M).
+// 128 x 128 x 256 values: 26 and 34 of 16.8 M).
 __device__ __forceinline__ float2 op_sigmoid_pair(float2 v) {
   const float2 t = fmul2(make_float2(fmaxf(v.x, -87.68f), fmaxf(v.y, -87.68f)), both(-1.4426950408889634f));
   const float2 e = make_float2(op_ex2(t.x), op_ex2(t.y));
@@ -109,8 +109,8 @@ __device__ __forceinline__ float2 op_gelu_pair(float2 v) {
 // = 1 / (1 + p a), y = p a t, and q a polynomial fitted in the same way (to
 // 2^-26) with q(0) = 1 / 2. Good to 2^-20 of Phi(-a) up to a = 4, 2^-18 up to 6,
 // 2^-16 up to 13.2, since the exponent is rounded, and 0 beyond; v (1 + erf(v / sqrt 2)) / 2 in
-// f32 is off by 2^-10 of itself at -4. 8 x 128 x 128 x 256 f16 to e4m3: 57 us (68
-// with erff, 89 with erfcf), 28 codes of 16.8 M beside the nearest one (38 with
+// f32 is off by 2^-10 of itself at -4. 8 x 128 x 128 x 256 f16 to e4m3: 58 us (68
+// with erff, 89 with erfcf), 26 codes of 16.8 M beside the nearest one (38 with
 // erff); a product of 8192 x 4096 x 1024 to f32: 75 us (155 with erfcf).
 __device__ __forceinline__ float2 op_gelu_pair_32(float2 v) {
   const float2 m = make_float2(fmaxf(-fabsf(v.x), -13.3f), fmaxf(-fabsf(v.y), -13.3f));  // -a

@@ -126,21 +126,17 @@ def test_a_stream_keeps_no_more_than_its_calls_need(ops):
     out = torch.empty_like(x)
     ops.group_norm(x, 5, out=out)
     torch.cuda.synchronize()
-    streams = [torch.cuda.ExternalStream(s) for s in _streams(300)]
-    before = torch.cuda.mem_get_info()[0]
-    for s in streams:
-        with torch.cuda.stream(s):
-            ops.group_norm(x, 5, out=out)
-    torch.cuda.synchronize()
-    assert before - torch.cuda.mem_get_info()[0] < 100 << 20
-
-
-def _streams(count):
-    """More streams than torch's pool has: made by the CUDA runtime."""
-    runtime = pytest.importorskip("cuda.bindings.runtime")
-    made = [runtime.cudaStreamCreateWithFlags(1) for _ in range(count)]
+    runtime = pytest.importorskip("cuda.bindings.runtime")  # (torch's own streams are a pool of 32)
+    made = [runtime.cudaStreamCreateWithFlags(1) for _ in range(300)]
     assert all(err == runtime.cudaError_t.cudaSuccess for err, _ in made)
-    return [int(s) for _, s in made]
+    before = torch.cuda.mem_get_info()[0]
+    for _, s in made:
+        ops.group_norm(x, 5, out=out, stream=int(s))
+    torch.cuda.synchronize()
+    kept = before - torch.cuda.mem_get_info()[0]
+    for _, s in made:
+        runtime.cudaStreamDestroy(s)
+    assert kept < 100 << 20
 
 
 def test_a_graph_outlives_larger_and_smaller_captures(ops):

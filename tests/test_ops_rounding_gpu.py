@@ -45,9 +45,8 @@ def test_scales_and_factors_are_rounded_once(ops, rows, k, block_rows, dtype):
 def test_a_groups_rstd_is_nearly_rounded_once(ops, pixels, c):
     """Groups of one channel that hold 1 and -1, equally often: every sum of
     them is exact, the mean 0, the variance 1, and 1 + eps has no rounding for
-    multiples of 2^-22 below 3. The result is 1 / sqrt(1 + eps) itself: a Newton
-    step leaves half of the 2^-24 that its residual is rounded by, then the
-    result is rounded, 1.5 * 2^-24."""
+    multiples of 2^-22 below 3. The result is 1 / sqrt(1 + eps) itself, 2^-24 of
+    it if it is rounded once; half as much again is left for a step towards it."""
     x = torch.ones(1, pixels, c, device="cuda")
     x[:, 1::2] = -1
     g = torch.Generator()
