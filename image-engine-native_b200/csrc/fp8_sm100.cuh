@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
               v[q + 2] = y.x;
               v[q + 3] = y.y;
             }
-            op_act_vec<ACT, 8 * (int)sizeof(T), V>(v);
+            op_act_vec<ACT, T, V>(v);
             uint4* chunk = reinterpret_cast<uint4*>(patch + (j >> 3) * 4096 + lane * 128 + (((j ^ lane) & 7) << 4));
             if (RES) add_16<T>(v, *chunk);
             *chunk = make_16<T>(v);
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1)
 #pragma unroll
           for (int u = 0; u < U; u++) {
             const int r = r0 + u * stride;
-            op_act_vec<ACT, 8 * (int)sizeof(T), 4>(v[u]);
+            op_act_vec<ACT, T, 4>(v[u]);
             T* out = static_cast<T*>(p.out) + (mt * 128 + r) * p.out_stride + col;
             if (r < rows)
 #pragma unroll

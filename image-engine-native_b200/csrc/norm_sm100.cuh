@@ -345,7 +345,7 @@ struct NormResident {
 
 template <class T, bool FP8, bool AL>
 __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec p, const NormResident q) {
-  constexpr int BITS = FP8 ? 8 : 8 * (int)sizeof(T);
+  using R = std::conditional_t<FP8, uint8_t, T>;
   constexpr int VE = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
   const int rank = blockIdx.x, ctas = gridDim.x, seg = blockIdx.y, map = blockIdx.z;
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 1) norm_resident(const NormSpec 
       float v[VE];
       Vec<T, VE, AL>::expand(i < n ? data[i * stride] : make_uint4(0, 0, 0, 0), v);
       affine.apply(v);
-      op_act_vec<ACT, BITS, VE>(v);
+      op_act_vec<ACT, R, VE>(v);
       if (FP8) {
         const float sc = store_fp8<VE, AL>(codes + i * code_step, mine && i < n, v);
         if (scale_at && i < n) scale_at[i * q.rows] = sc;
@@ -671,7 +671,7 @@ __device__ __forceinline__ void norm_join_all(const NormSpec& p, const NormChunk
 
 template <class T, int VE, bool FP8, bool AL>
 __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p, const NormChunks q) {
-  constexpr int BITS = FP8 ? 8 : 8 * (int)sizeof(T);
+  using R = std::conditional_t<FP8, uint8_t, T>;
   using V = Vec<T, VE, AL>;
   extern __shared__ __align__(16) float2 stat[];  // of the tile's groups
   // the pixels backwards, the latest map first
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, 2) norm_apply(const NormSpec p,
         float v[VE];
         V::expand(raw[u], v);
         affine.apply(v);
-        op_act_vec<ACT, BITS, VE>(v);
+        op_act_vec<ACT, R, VE>(v);
         if constexpr (FP8) {
           const float sc = store_fp8<VE, AL>(codes + u * (long long)p.q.code_stride, live && u < some, v);
           mine = lane == u ? sc : mine;
@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_fp8_odd(const NormSpe
         v[j] = block * FP8_BLOCK + j * 32 + lane < p.c ? to_f32(x[px * p.x_stride + j * 32]) : 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = fmaf(v[j] - mean[j], scale[j], beta[j]);
-      op_act_vec<ACT, 8, 4>(v);
+      op_act_vec<ACT, uint8_t, 4>(v);
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (block * FP8_BLOCK + j * 32 + lane < p.c) top = max(top, abs_bits(v[j]));

@@ -72,9 +72,9 @@ __device__ __forceinline__ float2 fmul2_ftz(float2 a, float2 b) {
 // which stay in f32's range for all d up to 2^126.5, where v is clamped. They
 // are good to 2^-20 of themselves up to |v| = 8, to 2^-18 up to 87 (v log2(e) is
 // rounded once), and 0 below -87.3, where they are less than 2^-126; of a NaN
-// they are 0 too. Quantised, no more e4m3 codes come out beside
-// the nearest one than with exact exponentials and quotients in f32 (SiLU of 4 x
-// 128 x 128 x 256 values: 26 and 34 of 16.8 M).
+// they are 0 too. Quantised, no more e4m3 codes come out beside the nearest one
+// than with exact exponentials and quotients in f32 (SiLU of 4 x 128 x 128 x 256
+// values: 26 and 34 of 16.8 M).
 __device__ __forceinline__ float2 op_sigmoid_pair(float2 v) {
   const float2 t = fmul2(make_float2(fmaxf(v.x, -87.68f), fmaxf(v.y, -87.68f)), both(-1.4426950408889634f));
   const float2 e = make_float2(op_ex2(t.x), op_ex2(t.y));
@@ -86,21 +86,35 @@ __device__ __forceinline__ float2 op_sigmoid_pair(float2 v) {
 // Phi(-a), a = |v|. Phi(-a) = 2^(s(a) - a^2 log2(e) / 2), where s = log2(e^(a^2 /
 // 2) Phi(-a)) goes from -1 to -5 over 0 to 13.2 and is a polynomial here, fitted
 // to it (least largest error, by linear programming over 1500 Chebyshev points):
-// good to 2^-15 of Phi(-a) up to a = 6, 2^-14 up to 13.2, and 0 beyond, below
-// 2^-126. (With one or two degrees less the tail is off by 2^-13 and 2^-11 of
-// itself, which is seen beside f16's rounding of 2^-11.) A third of erfcf's
-// instructions. NaN stays NaN.
+// good to 2^-14 of Phi(-a) and better. For f16 up to a = 5.85, where a Phi(-a) is
+// less than half its smallest step; for bf16 up to 13.2, and 0 beyond, below
+// 2^-126. (With a degree less the tails are off by 2^-11 and 2^-13 of themselves.)
+// A quarter to a third of erfcf's instructions. NaN stays NaN.
+template <class R>
 __device__ __forceinline__ float2 op_gelu_pair(float2 v) {
-  const float2 m = make_float2(fmaxf(-fabsf(v.x), -13.2f), fmaxf(-fabsf(v.y), -13.2f));  // -a
-  float2 s = ffma2(both(1.923425197e-9f), m, both(1.403363541e-7f));
-  s = ffma2(s, m, both(4.502811407e-6f));
-  s = ffma2(s, m, both(8.410552982e-5f));
-  s = ffma2(s, m, both(1.024093712e-3f));
-  s = ffma2(s, m, both(8.679608814e-3f));
-  s = ffma2(s, m, both(5.398480967e-2f));
-  s = ffma2(s, m, both(2.625868917e-1f));
-  s = ffma2(s, m, both(1.150994f));
-  s = ffma2(s, m, both(-1.000029564f));
+  constexpr bool F16 = std::is_same<R, __half>::value;
+  constexpr float most = F16 ? 5.85f : 13.2f;
+  const float2 m = make_float2(fmaxf(-fabsf(v.x), -most), fmaxf(-fabsf(v.y), -most));  // -a
+  float2 s;
+  if constexpr (F16) {
+    s = ffma2(both(1.831785198e-6f), m, both(6.154859875e-5f));
+    s = ffma2(s, m, both(9.302141261e-4f));
+    s = ffma2(s, m, both(8.506965823e-3f));
+    s = ffma2(s, m, both(5.395872518e-2f));
+    s = ffma2(s, m, both(2.628822327e-1f));
+    s = ffma2(s, m, both(1.151250839f));
+    s = ffma2(s, m, both(-9.999953508e-1f));
+  } else {
+    s = ffma2(both(1.923425197e-9f), m, both(1.403363541e-7f));
+    s = ffma2(s, m, both(4.502811407e-6f));
+    s = ffma2(s, m, both(8.410552982e-5f));
+    s = ffma2(s, m, both(1.024093712e-3f));
+    s = ffma2(s, m, both(8.679608814e-3f));
+    s = ffma2(s, m, both(5.398480967e-2f));
+    s = ffma2(s, m, both(2.625868917e-1f));
+    s = ffma2(s, m, both(1.150994f));
+    s = ffma2(s, m, both(-1.000029564f));
+  }
   s = ffma2(fmul2(m, both(-0.72134752f)), m, s);
   return ffma2(m, make_float2(op_ex2(s.x), op_ex2(s.y)), make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f)));
 }
@@ -108,10 +122,11 @@ __device__ __forceinline__ float2 op_gelu_pair(float2 v) {
 // The same for results of 8 and 32 bits, with Phi(-a) = e^(-a^2 / 2) t q(y), t
 // = 1 / (1 + p a), y = p a t, and q a polynomial fitted in the same way (to
 // 2^-26) with q(0) = 1 / 2. Good to 2^-20 of Phi(-a) up to a = 4, 2^-18 up to 6,
-// 2^-16 up to 13.2, since the exponent is rounded, and 0 beyond; v (1 + erf(v / sqrt 2)) / 2 in
-// f32 is off by 2^-10 of itself at -4. 8 x 128 x 128 x 256 f16 to e4m3: 58 us (68
-// with erff, 89 with erfcf), 26 codes of 16.8 M beside the nearest one (38 with
-// erff); a product of 8192 x 4096 x 1024 to f32: 75 us (155 with erfcf).
+// 2^-16 up to 13.2, since the exponent is rounded, and 0 beyond; v (1 + erf(v /
+// sqrt 2)) / 2 in f32 is off by 2^-10 of itself at -4. 8 x 128 x 128 x 256 f16 to
+// e4m3: 58 us (68 with erff, 89 with erfcf), 26 codes of 16.8 M beside the nearest
+// one in 4 x 128 x 128 x 256 (38 with erff); a product of 8192 x 4096 x 1024 to
+// f32: 75 us (155 with erfcf).
 __device__ __forceinline__ float2 op_gelu_pair_32(float2 v) {
   const float2 m = make_float2(fmaxf(-fabsf(v.x), -13.3f), fmaxf(-fabsf(v.y), -13.3f));  // -a
   const float2 pa = fmul2(m, both(-0.264f)), d = fadd2(pa, both(1.0f));
@@ -129,34 +144,38 @@ __device__ __forceinline__ float2 op_gelu_pair_32(float2 v) {
   return ffma2(m, fmul2(q, g), make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f)));
 }
 
-// The activation of N values for results of BITS (8, 16 or 32) bits; the
-// formula's own f32 functions where the result keeps f32's. The products that
-// end an activation are not contracted with what is added to them, so that
-// every kernel and path rounds the same. NaN stays NaN.
-template <int ACT, int BITS, int N>
+// The activation of N values for results of type R (uint8_t: e4m3 codes). The
+// products that end an activation are not contracted with what is added to
+// them, so that every kernel and path rounds the same. NaN stays NaN.
+template <int ACT, class R, int N>
 __device__ __forceinline__ void op_act_vec(float* v) {
+  constexpr bool SHORT = sizeof(R) == 2;
   if constexpr (ACT == OP_RELU) {
 #pragma unroll
     for (int e = 0; e < N; e++) v[e] = v[e] < 0.0f ? 0.0f : v[e];
-  } else if constexpr (ACT == OP_GELU) {
+  } else if constexpr (ACT != OP_NONE && ACT != OP_GELU && sizeof(R) == 4) {
+    // A reciprocal each (of what is above 2^126 it is 0): no value's last bits
+    // depend on its neighbour's.
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const float s = op_rcp(1.0f + expf(-v[e]));
+      v[e] = ACT == OP_SILU ? __fmul_rn(v[e], s) : s;
+    }
+  } else if constexpr (ACT != OP_NONE) {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-      const float2 x = make_float2(v[e], v[N == 1 ? e : e + 1]), y = BITS == 16 ? op_gelu_pair(x) : op_gelu_pair_32(x);
+      const float2 x = make_float2(v[e], v[N == 1 ? e : e + 1]);
+      float2 y;
+      if constexpr (ACT == OP_GELU && SHORT)
+        y = op_gelu_pair<R>(x);
+      else if constexpr (ACT == OP_GELU)
+        y = op_gelu_pair_32(x);
+      else
+        y = op_sigmoid_pair(x);
+      if constexpr (ACT == OP_SILU) y = fmul2(x, y);
+      if constexpr (ACT == OP_SIGMOID) y = make_float2(x.x != x.x ? x.x : y.x, x.y != x.y ? x.y : y.y);
       v[e] = y.x;
       if (N > 1) v[e + 1] = y.y;
-    }
-  } else if constexpr (ACT == OP_SIGMOID || ACT == OP_SILU) {
-    if constexpr (BITS == 32) {
-#pragma unroll
-      for (int e = 0; e < N; e++) v[e] = __fdividef(ACT == OP_SILU ? v[e] : 1.0f, 1.0f + expf(-v[e]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const float2 x = make_float2(v[e], v[N == 1 ? e : e + 1]), s = op_sigmoid_pair(x);
-        const float2 y = ACT == OP_SILU ? fmul2(x, s) : make_float2(x.x != x.x ? x.x : s.x, x.y != x.y ? x.y : s.y);
-        v[e] = y.x;
-        if (N > 1) v[e + 1] = y.y;
-      }
     }
   }
 }

@@ -2,10 +2,10 @@
 product without values along k is act(bias), a normalisation with gamma 0 is
 act(beta).
 
-Tolerances, u the output type's unit roundoff: results of f32 are the
-formula's own f32 functions, each within two units: 2^-21 of the value. For
-16 bits u + 2^-18: the exponent v log2(e) is rounded once, by up to 2^-17 / 2
-at |v| = 87, 2^-18.5 of the exponential. Below -87.3 the sigmoid is less than
+Tolerances, u the output type's unit roundoff: for f32 2^-21 of the value, two
+units each for an exponential, a sum, a quotient and a product. For 16 bits u +
+2^-18: the exponent v log2(e) is rounded once, by up to 2^-17 / 2 at |v| = 87,
+2^-18.5 of the exponential. Below -87.3 the sigmoid is less than
 2^-126 and may be 0: 2^-119 of a SiLU, since |v| < 128 where that matters.
 GELU: a Phi(-a), a = |v|, has its exponent a^2 log2(e) / 2 rounded twice, which
 moves it by a^2 2^-24 of itself, next to 2^-20 for what else is rounded; for 16
